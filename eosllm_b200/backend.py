@@ -47,6 +47,19 @@ def build() -> str:
     return LIB_PATH
 
 
+
+
+class KvQ8(C.Structure):
+    """eosi_cuda_kv_q8_t: a pool of 8-bit key/value cache pages."""
+    _fields_ = [("pages", C.c_void_p), ("n_pages", C.c_uint32), ("n_kv_head", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class AttnBatch(C.Structure):
+    """eosi_cuda_attn_batch_t: sequences that share a prefix of the cache."""
+    _fields_ = [(n, C.c_void_p) for n in ("prefix_table", "prefix_len", "table", "seq_len", "row0")] + \
+               [(n, C.c_uint32) for n in ("max_prefix", "table_stride", "max_len", "n_seq", "n_rows", "max_rows")]
+
+
 _vp = C.c_void_p
 _u32 = C.c_uint32
 _u64 = C.c_uint64
@@ -76,6 +89,12 @@ _SIGNATURES = {
     "eosi_cuda_q4_k_quantize_dev": (C.c_int, [_vp, _vp, _sz, _vp]),
     "eosi_cuda_fill_gauss_dev": (C.c_int, [_vp, _sz, _u64, _u64, C.c_float, _vp]),
     "eosi_cuda_q4_k_from_gauss_dev": (C.c_int, [_vp, _sz, _u64, C.c_float, _vp]),
+    "eosi_cuda_kv_q8_page_bytes": (_sz, [_u32, _u32]),
+    "eosi_cuda_kv_q8_write_dev": (C.c_int, [_vp, _vp, _vp, _u64, _u32, _vp, _vp, _u32, _vp, _u32, _vp]),
+    "eosi_cuda_kv_q8_read_dev": (C.c_int, [_vp, _vp, _vp, _u64, _u32, _vp, _vp, _u32, _vp, _u32, _vp]),
+    "eosi_cuda_kv_q8_attn_scratch_bytes": (_sz, [_vp, _vp, _u32]),
+    "eosi_cuda_kv_q8_attn_dev": (C.c_int, [_vp, _vp, _vp, _u64, _vp, _u64, _u32, C.c_float, _vp, _sz, _vp]),
+    "eosi_cuda_verify_draft_dev": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _u32, _vp, _u32, _u32, _vp, _vp, _vp]),
     "eosi_cuda_take_device_errors": (C.c_int, [C.POINTER(C.c_uint32)]),
     "eosi_cuda_set_kernel_variant": (C.c_int, [C.c_int, C.c_int]),
     "eosi_cuda_matmul_q4_k_noalloc": (C.c_int, [_vp, _vp, _vp, _u32, _u32, _u32, _vp]),
@@ -296,3 +315,65 @@ def prefill_prepare_weights_dev(w, n, k, w_prep, stream=0) -> None:
 def prefill_dev(a, w_prep, c, m, n, k, scratch, stream=0) -> None:
     check(load().eosi_cuda_q4_k_prefill_dev(_ptr(a), _ptr(w_prep), _ptr(c), m, n, k, _ptr(scratch),
                                             stream or None), "eosi_cuda_q4_k_prefill_dev")
+
+
+# ---------------------------------------------------------------------------
+# 8-bit key/value cache, attention over it, draft verification.  Integer
+# tensors are 32-bit; None is a NULL pointer.
+# ---------------------------------------------------------------------------
+KV_PAGE = 128  # tokens of a cache page
+NO_TOKEN = 0xFFFFFFFF
+
+
+def _optr(x):
+    return None if x is None else (_ptr(x) or None)
+
+
+def kv_q8_page_bytes(n_kv_head: int, head_dim: int) -> int:
+    return int(load().eosi_cuda_kv_q8_page_bytes(n_kv_head, head_dim))
+
+
+def kv_q8_pool(pages, n_pages: int, n_kv_head: int, head_dim: int) -> KvQ8:
+    """Description of a pool of cache pages (n_pages * kv_q8_page_bytes bytes)."""
+    return KvQ8(_ptr(pages), n_pages, n_kv_head, head_dim)
+
+
+def kv_q8_write_dev(pool: KvQ8, k, v, row_stride, n_rows, row0, table, table_stride, pos, n_seq, stream=0) -> None:
+    """Quantise f32 key and value rows into the cache."""
+    check(load().eosi_cuda_kv_q8_write_dev(C.byref(pool), _optr(k), _optr(v), row_stride, n_rows, _optr(row0),
+                                           _optr(table), table_stride, _optr(pos), n_seq, stream or None),
+          "eosi_cuda_kv_q8_write_dev")
+
+
+def kv_q8_read_dev(pool: KvQ8, k, v, row_stride, n_rows, row0, table, table_stride, pos, n_seq, stream=0) -> None:
+    """The cache's key and value rows as f32."""
+    check(load().eosi_cuda_kv_q8_read_dev(C.byref(pool), _optr(k), _optr(v), row_stride, n_rows, _optr(row0),
+                                          _optr(table), table_stride, _optr(pos), n_seq, stream or None),
+          "eosi_cuda_kv_q8_read_dev")
+
+
+def attn_batch(*, table, table_stride, seq_len, max_len, n_seq, n_rows, max_rows, row0=None, prefix_table=None,
+               prefix_len=None, max_prefix=0) -> AttnBatch:
+    """Description of a batch for kv_q8_attn_dev (the tensors must outlive it)."""
+    return AttnBatch(_optr(prefix_table), _optr(prefix_len), _optr(table), _optr(seq_len), _optr(row0), max_prefix,
+                     table_stride, max_len, n_seq, n_rows, max_rows)
+
+
+def kv_q8_attn_scratch_bytes(pool: KvQ8, batch: AttnBatch, n_head: int) -> int:
+    return int(load().eosi_cuda_kv_q8_attn_scratch_bytes(C.byref(pool), C.byref(batch), n_head))
+
+
+def kv_q8_attn_dev(pool: KvQ8, batch: AttnBatch, q, q_stride, out, out_stride, n_head, scale, scratch, scratch_bytes,
+                   stream=0) -> None:
+    """Attention of a batch that shares a prefix, over the 8-bit cache."""
+    check(load().eosi_cuda_kv_q8_attn_dev(C.byref(pool), C.byref(batch), _optr(q), q_stride, _optr(out), out_stride,
+                                          n_head, scale, _optr(scratch), scratch_bytes, stream or None),
+          "eosi_cuda_kv_q8_attn_dev")
+
+
+def verify_draft_dev(p, q, row_stride, drafts, n_draft, max_draft, u, n_seq, n_vocab, tokens, n_tokens,
+                     stream=0) -> None:
+    """Accept drafted tokens against the target's probabilities and draw the next one."""
+    check(load().eosi_cuda_verify_draft_dev(_optr(p), _optr(q), row_stride, _optr(drafts), _optr(n_draft), max_draft,
+                                            _optr(u), n_seq, n_vocab, _optr(tokens), _optr(n_tokens), stream or None),
+          "eosi_cuda_verify_draft_dev")

@@ -26,6 +26,7 @@
 #include "eosllm_cuda.h"
 #include "eos_common.cuh"
 #include "eos_kernels.h"
+#include "kv_q8.cuh"
 
 namespace {
 
@@ -573,6 +574,72 @@ int dev_prologue(DevInfo** info, std::initializer_list<const void*> ptrs = {}) {
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// ---- arguments of the 8-bit cache entry points -----------------------------
+int kv_pool_args(const eosi_cuda_kv_q8_t* kv, eos::KvPool& pool) {
+  if (kv == nullptr || kv->pages == nullptr) return fail(EOS_E_INVALID_ARG, "kv cache: NULL pointer argument");
+  if (!al16(kv->pages)) return fail(EOS_E_INVALID_ARG, "kv cache: pages must be 16-byte aligned");
+  if (kv->n_kv_head == 0 || kv->n_kv_head > 65535u) return fail(EOS_E_INVALID_ARG, "kv cache: n_kv_head=%u", kv->n_kv_head);
+  if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+    return fail(EOS_E_UNSUPPORTED, "kv cache: head_dim=%u is not 64, 128 or 256", kv->head_dim);
+  pool = eos::KvPool{static_cast<uint8_t*>(kv->pages), kv->n_pages, kv->n_kv_head, kv->head_dim};
+  return EOS_OK;
+}
+
+int kv_rows_args(const uint32_t* row0, uint32_t n_rows, uint32_t n_seq, uint32_t table_stride) {
+  if (n_seq > 0 && row0 == nullptr && n_rows % n_seq)
+    return fail(EOS_E_INVALID_ARG, "kv cache: n_rows=%u is not a multiple of n_seq=%u (pass row0)", n_rows, n_seq);
+  if (table_stride > UINT32_MAX / EOSI_CUDA_KV_PAGE)
+    return fail(EOS_E_INVALID_ARG, "kv cache: table_stride=%u", table_stride);
+  return EOS_OK;
+}
+
+// *info stays NULL when there is nothing to do.
+int kv_copy_args(const eosi_cuda_kv_q8_t* kv, const float* k, const float* v, uint64_t row_stride, uint32_t n_rows,
+                 const uint32_t* row0, const uint32_t* table, uint32_t table_stride, const uint32_t* pos,
+                 uint32_t n_seq, eos::KvPool& pool, eos::KvRowSet& rows, DevInfo** info) {
+  int rc = kv_pool_args(kv, pool);
+  if (rc == EOS_OK) rc = kv_rows_args(row0, n_rows, n_seq, table_stride);
+  if (rc != EOS_OK) return rc;
+  if (row_stride % 4u || row_stride < (uint64_t)pool.n_kv_head * pool.head_dim)
+    return fail(EOS_E_INVALID_ARG, "kv cache: row_stride=%llu must be a multiple of 4 and hold n_kv_head * head_dim",
+                (unsigned long long)row_stride);
+  if ((uint64_t)n_rows * pool.n_kv_head > (1ull << 31))
+    return fail(EOS_E_INVALID_ARG, "kv cache: n_rows=%u times n_kv_head=%u exceeds 2^31", n_rows, pool.n_kv_head);
+  if (n_rows == 0 || n_seq == 0) return EOS_OK;
+  if (k == nullptr || v == nullptr || table == nullptr || pos == nullptr)
+    return fail(EOS_E_INVALID_ARG, "NULL pointer argument");
+  if (!al16(k) || !al16(v)) return fail(EOS_E_INVALID_ARG, "device pointers must be 16-byte aligned");
+  rows = eos::KvRowSet{row0, table, pos, n_rows, n_seq, table_stride};
+  return dev_prologue(info, {pool.pages, k, v, row0, table, pos});
+}
+
+int attn_batch_args(const eosi_cuda_attn_batch_t* b, const eos::KvPool& pool, uint32_t n_head, eos::KvAttnBatch& out) {
+  if (b == nullptr) return fail(EOS_E_INVALID_ARG, "NULL pointer argument");
+  int rc = kv_rows_args(b->row0, b->n_rows, b->n_seq, b->table_stride);
+  if (rc != EOS_OK) return rc;
+  if (n_head == 0 || n_head % pool.n_kv_head)
+    return fail(EOS_E_INVALID_ARG, "kv attention: n_head=%u is not a multiple of n_kv_head=%u", n_head, pool.n_kv_head);
+  if (b->n_seq > EOSI_CUDA_ATTN_MAX_SEQ)
+    return fail(EOS_E_UNSUPPORTED, "kv attention: %u sequences (at most %u)", b->n_seq, EOSI_CUDA_ATTN_MAX_SEQ);
+  if ((uint64_t)b->n_rows * n_head > (1ull << 28))
+    return fail(EOS_E_INVALID_ARG, "kv attention: n_rows=%u times n_head=%u exceeds 2^28", b->n_rows, n_head);
+  if (b->n_seq > 0 && b->n_rows > 0) {
+    if (b->max_rows == 0 || b->max_rows > b->n_rows || (b->row0 == nullptr && b->max_rows < b->n_rows / b->n_seq))
+      return fail(EOS_E_INVALID_ARG, "kv attention: max_rows=%u of n_rows=%u", b->max_rows, b->n_rows);
+    if (b->seq_len == nullptr || (b->max_len > 0 && b->table == nullptr) ||
+        (b->max_prefix > 0 && (b->prefix_table == nullptr || b->prefix_len == nullptr)))
+      return fail(EOS_E_INVALID_ARG, "NULL pointer argument");
+  }
+  if ((uint64_t)b->max_len > (uint64_t)b->table_stride * EOSI_CUDA_KV_PAGE)
+    return fail(EOS_E_INVALID_ARG, "kv attention: max_len=%u exceeds %u pages", b->max_len, b->table_stride);
+  if (b->max_prefix > (1u << 30) || b->max_len > (1u << 30))
+    return fail(EOS_E_INVALID_ARG, "kv attention: lengths above 2^30 tokens");
+  out = eos::KvAttnBatch{b->max_prefix ? b->prefix_table : nullptr, b->max_prefix ? b->prefix_len : nullptr,
+                         b->table, b->seq_len, b->row0, b->max_prefix, b->table_stride, b->max_len,
+                         b->n_seq, b->n_rows, b->max_rows};
+  return EOS_OK;
+}
+
 }  // namespace
 
 namespace eos {
@@ -898,6 +965,90 @@ int eosi_cuda_q4_k_from_gauss_dev(void* dst, size_t n_elements, uint64_t seed, f
   if (rc != EOS_OK) return rc;
   EOS_CK(eos::launch_q4k_from_gauss((uint8_t*)dst, n_elements / 256u, seed, 0, sigma, (cudaStream_t)stream),
          "q4_k generator kernel");
+  return EOS_OK;
+}
+
+// ---- 8-bit key/value cache, attention over it, draft verification ---------
+size_t eosi_cuda_kv_q8_page_bytes(uint32_t n_kv_head, uint32_t head_dim) {
+  return (size_t)n_kv_head * eos::kv_block_bytes(head_dim);
+}
+
+int eosi_cuda_kv_q8_write_dev(const eosi_cuda_kv_q8_t* kv, const float* k, const float* v, uint64_t row_stride,
+                              uint32_t n_rows, const uint32_t* row0, const uint32_t* table, uint32_t table_stride,
+                              const uint32_t* pos, uint32_t n_seq, void* stream) {
+  eos::KvPool pool;
+  eos::KvRowSet rows;
+  DevInfo* info = nullptr;
+  const int rc = kv_copy_args(kv, k, v, row_stride, n_rows, row0, table, table_stride, pos, n_seq, pool, rows, &info);
+  if (rc != EOS_OK || info == nullptr) return rc;
+  EOS_CK(eos::launch_kv_write(pool, rows, k, v, row_stride, info->err_d, (cudaStream_t)stream), "kv write kernel");
+  return EOS_OK;
+}
+
+int eosi_cuda_kv_q8_read_dev(const eosi_cuda_kv_q8_t* kv, float* k, float* v, uint64_t row_stride, uint32_t n_rows,
+                             const uint32_t* row0, const uint32_t* table, uint32_t table_stride, const uint32_t* pos,
+                             uint32_t n_seq, void* stream) {
+  eos::KvPool pool;
+  eos::KvRowSet rows;
+  DevInfo* info = nullptr;
+  const int rc = kv_copy_args(kv, k, v, row_stride, n_rows, row0, table, table_stride, pos, n_seq, pool, rows, &info);
+  if (rc != EOS_OK || info == nullptr) return rc;
+  EOS_CK(eos::launch_kv_read(pool, rows, k, v, row_stride, info->err_d, (cudaStream_t)stream), "kv read kernel");
+  return EOS_OK;
+}
+
+size_t eosi_cuda_kv_q8_attn_scratch_bytes(const eosi_cuda_kv_q8_t* kv, const eosi_cuda_attn_batch_t* batch,
+                                          uint32_t n_head) {
+  eos::KvPool pool;
+  eos::KvAttnBatch b;
+  if (kv_pool_args(kv, pool) != EOS_OK || attn_batch_args(batch, pool, n_head, b) != EOS_OK) return 0;
+  return eos::kv_attn_scratch_bytes(pool, b, n_head);
+}
+
+int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t* kv, const eosi_cuda_attn_batch_t* batch, const float* q,
+                             uint64_t q_stride, float* out, uint64_t out_stride, uint32_t n_head, float scale,
+                             void* scratch, size_t scratch_bytes, void* stream) {
+  eos::KvPool pool;
+  eos::KvAttnBatch b;
+  int rc = kv_pool_args(kv, pool);
+  if (rc == EOS_OK) rc = attn_batch_args(batch, pool, n_head, b);
+  if (rc != EOS_OK) return rc;
+  const uint64_t width = (uint64_t)n_head * pool.head_dim;
+  if (q_stride < width || q_stride % 4u || out_stride < width || out_stride % 4u)
+    return fail(EOS_E_INVALID_ARG, "kv attention: strides must be multiples of 4 and hold n_head * head_dim floats");
+  if (b.n_rows == 0 || b.n_seq == 0) return EOS_OK;
+  if (q == nullptr || out == nullptr || scratch == nullptr) return fail(EOS_E_INVALID_ARG, "NULL pointer argument");
+  if (!al16(q) || !al16(out) || !al16(scratch))
+    return fail(EOS_E_INVALID_ARG, "device pointers must be 16-byte aligned");
+  const size_t need = eos::kv_attn_scratch_bytes(pool, b, n_head);
+  if (scratch_bytes < need)
+    return fail(EOS_E_INVALID_ARG, "kv attention: %zu bytes of scratch, %zu needed", scratch_bytes, need);
+  DevInfo* info = nullptr;
+  rc = dev_prologue(&info, {pool.pages, b.prefix_table, b.prefix_len, b.table, b.seq_len, b.row0, q, out, scratch});
+  if (rc != EOS_OK) return rc;
+  EOS_CK(eos::launch_kv_attn(pool, b, q, q_stride, out, out_stride, n_head, scale, scratch, info->err_d,
+                             (cudaStream_t)stream),
+         "kv attention kernel");
+  return EOS_OK;
+}
+
+int eosi_cuda_verify_draft_dev(const float* p, const float* q, uint64_t stride, const uint32_t* drafts,
+                               const uint32_t* n_draft, uint32_t max_draft, const float* u, uint32_t n_seq,
+                               uint32_t n_vocab, uint32_t* tokens, uint32_t* n_tokens, void* stream) {
+  if (n_vocab == 0 || stride < n_vocab || max_draft > 65535u)
+    return fail(EOS_E_INVALID_ARG, "verify: n_vocab=%u stride=%llu max_draft=%u", n_vocab, (unsigned long long)stride,
+                max_draft);
+  if (n_seq == 0) return EOS_OK;
+  if (p == nullptr || u == nullptr || tokens == nullptr || n_tokens == nullptr ||
+      (max_draft > 0 && (q == nullptr || drafts == nullptr)))
+    return fail(EOS_E_INVALID_ARG, "NULL pointer argument");
+  DevInfo* info = nullptr;
+  const int rc = dev_prologue(&info, {p, max_draft ? q : nullptr, max_draft ? drafts : nullptr, n_draft, u, tokens,
+                                      n_tokens});
+  if (rc != EOS_OK) return rc;
+  EOS_CK(eos::launch_verify_draft(p, q, stride, drafts, n_draft, max_draft, u, n_seq, n_vocab, tokens, n_tokens,
+                                  (cudaStream_t)stream),
+         "draft verification kernel");
   return EOS_OK;
 }
 

@@ -36,6 +36,7 @@ enum : uint32_t {
   EOS_DEVERR_WAIT_ACT = 1u << 2,    // activation tile never arrived
   EOS_DEVERR_DRAIN = 1u << 3,       // in-flight copies did not drain on exit
   EOS_DEVERR_PEER = 1u << 4,        // a peer flag wait ran out
+  EOS_DEVERR_RANGE = 1u << 5,       // a page, position or length out of its range was left out
 };
 
 // One second: the bound on every spin-wait in this library's kernels.

@@ -92,4 +92,37 @@ cudaError_t launch_q80_quantize(const float* src, uint8_t* dst, size_t n_el, cud
 cudaError_t launch_q4k_from_gauss(uint8_t* dst, size_t nblocks, uint64_t seed, uint64_t offset, float sigma,
                                   cudaStream_t st);
 
+// ---- 8-bit paged key/value cache (kv_q8.cu, kv_q8_attn.cu) ----------------
+struct KvPool {
+  uint8_t* pages;
+  uint32_t n_pages, n_kv_head, head_dim;  // head_dim 64, 128 or 256
+};
+// Rows of a batch and where they sit in the cache (see KvCopyParams).
+struct KvRowSet {
+  const uint32_t* row0;
+  const uint32_t* table;
+  const uint32_t* pos;
+  uint32_t n_rows, n_seq, table_stride;
+};
+cudaError_t launch_kv_write(const KvPool& kv, const KvRowSet& rows, const float* k, const float* v,
+                            uint64_t row_stride, uint32_t* err, cudaStream_t st);
+cudaError_t launch_kv_read(const KvPool& kv, const KvRowSet& rows, float* k, float* v, uint64_t row_stride,
+                           uint32_t* err, cudaStream_t st);
+struct KvAttnBatch {
+  const uint32_t* prefix_table;
+  const uint32_t* prefix_len;
+  const uint32_t* table;
+  const uint32_t* seq_len;
+  const uint32_t* row0;
+  uint32_t max_prefix, table_stride, max_len, n_seq, n_rows, max_rows;
+};
+size_t kv_attn_scratch_bytes(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head);
+cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* q, uint64_t q_stride, float* out,
+                           uint64_t out_stride, uint32_t n_head, float scale, void* scratch,
+                           uint32_t* err, cudaStream_t st);
+// Verification of drafted tokens (verify_draft.cu).
+cudaError_t launch_verify_draft(const float* p, const float* q, uint64_t stride, const uint32_t* drafts,
+                                const uint32_t* n_draft, uint32_t max_draft, const float* u, uint32_t n_seq,
+                                uint32_t n_vocab, uint32_t* tokens, uint32_t* n_token, cudaStream_t st);
+
 }  // namespace eos

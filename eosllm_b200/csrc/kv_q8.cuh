@@ -1,0 +1,110 @@
+// kv_q8.cuh -- the 8-bit paged key/value cache: page layout, row geometry
+// and the row quantizer shared by the cache kernels (kv_q8.cu) and the
+// attention that reads the cache (kv_q8_attn.cu).
+//
+// A cache is a pool of pages of 128 tokens.  Page p holds, for kv head h, one
+// block of kv_block_bytes(HD) bytes at ((p * n_kv_head) + h) blocks:
+//   K      int8 [128 tokens][HD]    a matrix operand with HD contiguous
+//   V      int8 [4][HD][32 tokens]  a matrix operand with tokens contiguous,
+//                                   one 32-token quarter after the other
+//   scales f32 [4][2][32]           per quarter: 32 key scales, 32 value scales
+// value = int8 * scale, one scale per (token, head) row of HD elements.
+//
+// Both matrices are stored in the order in which the tensor core reads them
+// from shared memory, so a block is copied there byte for byte (one bulk
+// copy) and needs no conversion:
+//   K rows are swizzled in 16-byte chunks: HD = 128 as 128-byte rows (chunk ^=
+//   token % 8), HD = 256 as two such 128-dimension panels, HD = 64 as 64-byte
+//   rows (chunk ^= token / 2 % 4);
+//   V rows are 32 bytes (chunk ^= dim / 4 % 2), and token u = g + 8 j of a
+//   quarter (g < 8, j < 4) sits at position 4 g + j: the accumulator fragment
+//   of the score product leaves tokens g, g + 8, g + 16, g + 24 in one
+//   thread, which then writes its four probabilities as one word.  The order
+//   of the tokens inside a quarter does not matter to the sum over them.
+#pragma once
+
+#include "eos_common.cuh"
+
+namespace eos {
+
+constexpr uint32_t kKvPage = 128;  // tokens of a page
+constexpr uint32_t kKvQuarter = 32;
+
+__host__ __device__ constexpr uint32_t kv_block_bytes(uint32_t hd) { return 2u * kKvPage * hd + 1024u; }
+
+// Byte offsets inside a block.
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t kv_k_offset(uint32_t token, uint32_t dim) {
+  if constexpr (HD == 64)
+    return token * 64u + ((((dim >> 4) ^ (token >> 1)) & 3u) << 4) + (dim & 15u);
+  return (dim >> 7) * (kKvPage * 128u) + token * 128u + ((((dim >> 4) ^ token) & 7u) << 4) + (dim & 15u);
+}
+__device__ __forceinline__ uint32_t kv_v_position(uint32_t token) {  // inside the token's quarter
+  return 4u * (token & 7u) + ((token >> 3) & 3u);
+}
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t kv_v_offset(uint32_t token, uint32_t dim) {
+  const uint32_t p = kv_v_position(token);
+  return kKvPage * HD + (token >> 5) * (HD * kKvQuarter) + dim * 32u + (((p >> 4) ^ (dim >> 2)) & 1u) * 16u + (p & 15u);
+}
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t kv_scale_offset(uint32_t token, uint32_t value) {  // value: 0 key, 1 value scale
+  return 2u * kKvPage * HD + (token >> 5) * 256u + value * 128u + (token & 31u) * 4u;
+}
+
+// Rows of a batch.  Row r of sequence i (row0[i] <= r < row0[i + 1]; row0 ==
+// nullptr: n_rows / n_seq rows each) is the (r - row0[i])-th.  Device values
+// outside [0, n_rows] are clamped.
+struct KvRows {
+  const uint32_t* row0;
+  uint32_t n_seq, n_rows, per_seq;
+};
+__device__ __forceinline__ uint32_t kv_row_start(const KvRows& b, uint32_t i) {
+  const uint32_t r = b.row0 != nullptr ? b.row0[i] : i * b.per_seq;
+  return r < b.n_rows ? r : b.n_rows;
+}
+// The last sequence that starts at or before row r (rows behind the last
+// sequence give n_seq).
+__device__ __forceinline__ uint32_t kv_row_seq(const KvRows& b, uint32_t r) {
+  if (b.row0 == nullptr) return r / b.per_seq;
+  uint32_t lo = 0, hi = b.n_seq;  // start(lo) <= r (or lo == 0), start(hi) > r or hi == n_seq
+  if (kv_row_start(b, b.n_seq) <= r) return b.n_seq;
+  while (hi - lo > 1u) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (kv_row_start(b, mid) <= r) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// ---- the row quantizer ----------------------------------------------------
+// scale = fl32(max|x| / 127); q = the integer nearest to 127 x / max|x| (ties
+// to even) of the real quotient: the f32 estimate is off by at most 127 *
+// 2^-23 < 1e-4, so wherever it lies 1e-4 away from a half it decides, and
+// otherwise (about one element in 5000) the f64 quotient does, whose rounding
+// cannot move it across a half (127 x is exact, and a quotient of two floats
+// that is not a half differs from it by more than 2^-33 relative).  A row that
+// holds a NaN or an infinity gets that as its scale and q = 0: it reads back
+// as NaN.
+struct KvRowScale {
+  float scale, amax, inv;
+  bool finite, tiny;
+};
+__device__ __forceinline__ KvRowScale kv_row_scale(uint32_t amax_bits) {
+  KvRowScale s;
+  s.amax = __uint_as_float(amax_bits);
+  s.finite = amax_bits < 0x7f800000u;
+  s.tiny = s.amax < 7.8886e-31f;  // 2^-100: 127 / max|x| may overflow
+  s.scale = __fdiv_rn(s.amax, 127.0f);
+  s.inv = (s.finite && !s.tiny) ? __fdiv_rn(127.0f, s.amax) : 0.0f;
+  return s;
+}
+__device__ __forceinline__ int32_t kv_quant(float x, const KvRowScale& s) {
+  const float y = __fmul_rn(x, s.inv);
+  const float r = rintf(y);
+  if (fabsf(__fsub_rn(y, r)) <= 0.4999f && !s.tiny) return (int32_t)r;
+  if (!s.finite || s.amax == 0.0f) return 0;
+  return (int32_t)rint(__ddiv_rn(127.0 * (double)x, (double)s.amax));
+}
+
+}  // namespace eos

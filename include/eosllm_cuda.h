@@ -217,6 +217,112 @@ EOSLLM_CUDA_API int eosi_cuda_q4_k_prefill_prepare_weights_dev(const void *w, ui
 EOSLLM_CUDA_API int eosi_cuda_q4_k_prefill_dev(const float *a, const void *w_prep, float *c, uint32_t m, uint32_t n,
                                                uint32_t k, void *scratch, void *stream);
 
+/* ---- 8-bit key/value cache, attention over it, draft verification -----------
+ * For hosts with several sequences on the device: key and value rows are
+ * quantised as they enter a paged cache, a batch of sequences that share a
+ * prefix attends to it, and drafted tokens are verified against the target's
+ * probabilities.  The reference has no counterpart (its paged and speculative
+ * schedulers are stubs, src/sched/paged_kv.c, src/sched/speculative.c; its
+ * cache is f32, src/modality/text/text.c:220-226).  All pointers are device
+ * memory of the current device unless said otherwise; every call is
+ * asynchronous on `stream`, allocates nothing and may be captured into a CUDA
+ * graph: lengths, positions and page tables are read from device memory when
+ * the work runs, so a replayed graph sees their new values.  A page index,
+ * position or length outside its stated range is left out (the row or page is
+ * skipped, the length cut) and sets a bit that eosi_cuda_take_device_errors
+ * reports.
+ *
+ * Cache: a pool of n_pages pages of EOSI_CUDA_KV_PAGE tokens, each
+ * eosi_cuda_kv_q8_page_bytes(n_kv_head, head_dim) bytes, one after the other,
+ * 16-byte aligned; contents are opaque and need no initialisation.  One row
+ * (the head_dim elements x of one token and kv head, keys and values apart) is
+ * held as int8 q and one f32 scale: scale = max|x| / 127 in f32, q_i = the
+ * integer nearest to 127 x_i / max|x| (ties to even, decided on the exact
+ * quotient), its value q_i * scale in f32; a row that holds a NaN or an
+ * infinity reads back as NaN.  head_dim is 64, 128 or 256 (EOS_E_UNSUPPORTED
+ * otherwise). */
+#define EOSI_CUDA_KV_PAGE 128
+typedef struct {
+    void *pages;
+    uint32_t n_pages, n_kv_head, head_dim;
+} eosi_cuda_kv_q8_t;
+EOSLLM_CUDA_API size_t eosi_cuda_kv_q8_page_bytes(uint32_t n_kv_head, uint32_t head_dim);
+
+/* Quantises rows into the cache (write), or the cache's rows as f32 (read):
+ * row r, head h at k / v + r * row_stride + h * head_dim floats (16-byte
+ * aligned, row_stride a multiple of 4 and at least n_kv_head * head_dim).
+ * Sequence i owns rows [row0[i], row0[i + 1]) (row0: n_seq + 1 words; NULL:
+ * n_rows / n_seq each), which sit at positions pos[i], pos[i] + 1, ... ;
+ * position j of sequence i lives in page table[i * table_stride + j / 128].
+ * Rows behind the last sequence, and every token not written, stay as they
+ * were.  Two rows of one call must not share a (page, slot): distinct
+ * sequences write distinct pages. */
+EOSLLM_CUDA_API int eosi_cuda_kv_q8_write_dev(const eosi_cuda_kv_q8_t *kv, const float *k, const float *v,
+                                              uint64_t row_stride, uint32_t n_rows, const uint32_t *row0,
+                                              const uint32_t *table, uint32_t table_stride, const uint32_t *pos,
+                                              uint32_t n_seq, void *stream);
+EOSLLM_CUDA_API int eosi_cuda_kv_q8_read_dev(const eosi_cuda_kv_q8_t *kv, float *k, float *v, uint64_t row_stride,
+                                             uint32_t n_rows, const uint32_t *row0, const uint32_t *table,
+                                             uint32_t table_stride, const uint32_t *pos, uint32_t n_seq,
+                                             void *stream);
+
+/* Attention of n_seq sequences (at most EOSI_CUDA_ATTN_MAX_SEQ) that share a
+ * prefix of the cache.  Sequence i has n_i = row0[i + 1] - row0[i] query rows
+ * (at most max_rows; row0 NULL: n_rows / n_seq each) and, behind the prefix,
+ * seq_len[i] tokens of its own (its rows' keys and values included, already
+ * written; at most max_len) in the pages table[i * table_stride + ...].  Its
+ * row t, head h attends to the prefix_len[0] tokens (at most max_prefix) of
+ * the pages prefix_table[...] and to its own tokens 0 .. seq_len[i] - n_i + t:
+ *   out = sum_j softmax_j(scale * <q, k_j>) v_j    (kv head h * n_kv_head / n_head)
+ * and 0 where no token is visible.  max_prefix = 0: no prefix (both prefix
+ * pointers may be NULL).  max_len <= 128 * table_stride.  The prefix's pages
+ * are read once for all sequences.  Row r, head h of q and out is at
+ * r * stride + h * head_dim floats (16-byte aligned, strides multiples of 4
+ * and at least n_head * head_dim); rows of out behind the last sequence stay
+ * as they were.  n_head is a multiple of kv->n_kv_head.
+ * f32 in, f32 out: q is held as 24-bit integers (scaled by its row's
+ * maximum), a row's probabilities as 23-bit integers, products and sums of
+ * both with the int8 cache are exact integers, and the softmax statistics are
+ * f32.  Results do not depend on timing.  A query row or a visible cache row
+ * that holds a NaN or an infinity gives a row of NaN.
+ * scratch: eosi_cuda_kv_q8_attn_scratch_bytes(kv, batch, n_head) bytes, 16-byte
+ * aligned, not shared by calls that may overlap. */
+#define EOSI_CUDA_ATTN_MAX_SEQ 1024
+typedef struct {
+    const uint32_t *prefix_table, *prefix_len;
+    const uint32_t *table, *seq_len;
+    const uint32_t *row0;
+    uint32_t max_prefix, table_stride, max_len;
+    uint32_t n_seq, n_rows, max_rows;
+} eosi_cuda_attn_batch_t;
+EOSLLM_CUDA_API size_t eosi_cuda_kv_q8_attn_scratch_bytes(const eosi_cuda_kv_q8_t *kv,
+                                                          const eosi_cuda_attn_batch_t *batch, uint32_t n_head);
+EOSLLM_CUDA_API int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t *kv, const eosi_cuda_attn_batch_t *batch,
+                                             const float *q, uint64_t q_stride, float *out, uint64_t out_stride,
+                                             uint32_t n_head, float scale, void *scratch, size_t scratch_bytes,
+                                             void *stream);
+
+/* Verifies drafted tokens.  Sequence i has n_draft[i] <= max_draft drafted
+ * tokens drafts[i * max_draft + j] (n_draft NULL: max_draft each; larger
+ * values count as max_draft), the target's probabilities p_j at
+ * p + (i * (max_draft + 1) + j) * stride for j = 0 .. n_draft[i], the
+ * draft's q_j at q + (i * max_draft + j) * stride, and uniform numbers
+ * u[i * (max_draft + 1) + j].  Leading drafts x_j with u_j q_j(x_j) < p_j(x_j)
+ * are accepted (a token outside the vocabulary is not); then one token is
+ * drawn with the last number of the row, u[i * (max_draft + 1) + max_draft]:
+ * from max(p_a - q_a, 0) after a rejection at a (from p_a where that is 0
+ * everywhere), else from p of row n_draft[i].  The draw is the lowest v whose
+ * running sum of weights exceeds u times the whole sum; sums are f64, so the
+ * rows need not sum to 1; weights that are not positive and finite count 0.
+ * tokens[i * (max_draft + 1) ...] gets the accepted tokens and the drawn one,
+ * n_tokens[i] of them, and 0xffffffff behind them (a row without any weight
+ * draws no token).  max_draft = 0 draws one token from p alone (q and drafts
+ * may be NULL). */
+EOSLLM_CUDA_API int eosi_cuda_verify_draft_dev(const float *p, const float *q, uint64_t stride,
+                                               const uint32_t *drafts, const uint32_t *n_draft, uint32_t max_draft,
+                                               const float *u, uint32_t n_seq, uint32_t n_vocab, uint32_t *tokens,
+                                               uint32_t *n_tokens, void *stream);
+
 /* ---- device-resident Llama decoder ------------------------------------------
  * The work of eosi_text_open / eosi_text_step / eosi_text_close
  * (src/modality/text/text.h:62-78, text.c:131-436 of the reference) with
