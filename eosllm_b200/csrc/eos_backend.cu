@@ -13,6 +13,7 @@
 // Device-pointer layer: enqueue-only wrappers around the same launchers.
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -637,6 +638,8 @@ int attn_batch_args(const eosi_cuda_attn_batch_t* b, const eos::KvPool& pool, ui
   out = eos::KvAttnBatch{b->max_prefix ? b->prefix_table : nullptr, b->max_prefix ? b->prefix_len : nullptr,
                          b->table, b->seq_len, b->row0, b->max_prefix, b->table_stride, b->max_len,
                          b->n_seq, b->n_rows, b->max_rows};
+  if (eos::kv_attn_work_bound(pool, out, n_head) >= (1ull << 31))
+    return fail(EOS_E_INVALID_ARG, "kv attention: too many pages times heads times row groups (2^31)");
   return EOS_OK;
 }
 
@@ -1013,6 +1016,7 @@ int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t* kv, const eosi_cuda_attn_b
   int rc = kv_pool_args(kv, pool);
   if (rc == EOS_OK) rc = attn_batch_args(batch, pool, n_head, b);
   if (rc != EOS_OK) return rc;
+  if (!std::isfinite(scale)) return fail(EOS_E_INVALID_ARG, "kv attention: scale is not finite");
   const uint64_t width = (uint64_t)n_head * pool.head_dim;
   if (q_stride < width || q_stride % 4u || out_stride < width || out_stride % 4u)
     return fail(EOS_E_INVALID_ARG, "kv attention: strides must be multiples of 4 and hold n_head * head_dim floats");
@@ -1026,8 +1030,8 @@ int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t* kv, const eosi_cuda_attn_b
   DevInfo* info = nullptr;
   rc = dev_prologue(&info, {pool.pages, b.prefix_table, b.prefix_len, b.table, b.seq_len, b.row0, q, out, scratch});
   if (rc != EOS_OK) return rc;
-  EOS_CK(eos::launch_kv_attn(pool, b, q, q_stride, out, out_stride, n_head, scale, scratch, info->err_d,
-                             (cudaStream_t)stream),
+  EOS_CK(eos::launch_kv_attn(pool, b, q, q_stride, out, out_stride, n_head, scale, scratch, info->num_sms,
+                             info->err_d, (cudaStream_t)stream),
          "kv attention kernel");
   return EOS_OK;
 }

@@ -116,9 +116,11 @@ struct KvAttnBatch {
   const uint32_t* row0;
   uint32_t max_prefix, table_stride, max_len, n_seq, n_rows, max_rows;
 };
+constexpr uint32_t EOS_ATTN_MAX_SEQ = 1024;  // EOSI_CUDA_ATTN_MAX_SEQ
 size_t kv_attn_scratch_bytes(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head);
+uint64_t kv_attn_work_bound(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head);  // must stay below 2^31
 cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* q, uint64_t q_stride, float* out,
-                           uint64_t out_stride, uint32_t n_head, float scale, void* scratch,
+                           uint64_t out_stride, uint32_t n_head, float scale, void* scratch, int num_sms,
                            uint32_t* err, cudaStream_t st);
 // Verification of drafted tokens (verify_draft.cu).
 cudaError_t launch_verify_draft(const float* p, const float* q, uint64_t stride, const uint32_t* drafts,

@@ -63,12 +63,11 @@ __device__ __forceinline__ uint32_t kv_row_start(const KvRows& b, uint32_t i) {
   const uint32_t r = b.row0 != nullptr ? b.row0[i] : i * b.per_seq;
   return r < b.n_rows ? r : b.n_rows;
 }
-// The last sequence that starts at or before row r (rows behind the last
-// sequence give n_seq).
+// The sequence of row r (rows before the first or behind the last give n_seq).
 __device__ __forceinline__ uint32_t kv_row_seq(const KvRows& b, uint32_t r) {
   if (b.row0 == nullptr) return r / b.per_seq;
-  uint32_t lo = 0, hi = b.n_seq;  // start(lo) <= r (or lo == 0), start(hi) > r or hi == n_seq
-  if (kv_row_start(b, b.n_seq) <= r) return b.n_seq;
+  uint32_t lo = 0, hi = b.n_seq;  // start(lo) <= r < start(hi)
+  if (kv_row_start(b, b.n_seq) <= r || r < kv_row_start(b, 0)) return b.n_seq;
   while (hi - lo > 1u) {
     const uint32_t mid = (lo + hi) >> 1;
     if (kv_row_start(b, mid) <= r) lo = mid;
@@ -78,7 +77,7 @@ __device__ __forceinline__ uint32_t kv_row_seq(const KvRows& b, uint32_t r) {
 }
 
 // ---- the row quantizer ----------------------------------------------------
-// scale = fl32(max|x| / 127); q = the integer nearest to 127 x / max|x| (ties
+// scale = max|x| * fl32(1 / 127) in f32; q = the integer nearest to 127 x / max|x| (ties
 // to even) of the real quotient: the f32 estimate is off by at most 127 *
 // 2^-23 < 1e-4, so wherever it lies 1e-4 away from a half it decides, and
 // otherwise (about one element in 5000) the f64 quotient does, whose rounding
@@ -95,7 +94,7 @@ __device__ __forceinline__ KvRowScale kv_row_scale(uint32_t amax_bits) {
   s.amax = __uint_as_float(amax_bits);
   s.finite = amax_bits < 0x7f800000u;
   s.tiny = s.amax < 7.8886e-31f;  // 2^-100: 127 / max|x| may overflow
-  s.scale = __fdiv_rn(s.amax, 127.0f);
+  s.scale = __fmul_rn(s.amax, 1.0f / 127.0f);
   s.inv = (s.finite && !s.tiny) ? __fdiv_rn(127.0f, s.amax) : 0.0f;
   return s;
 }

@@ -1,14 +1,73 @@
 // kv_q8_attn.cu -- attention of a batch of sequences that share a prefix,
-// over the 8-bit paged cache (layout: kv_q8.cuh).
+// over the 8-bit paged cache (layout: kv_q8.cuh), on the sm_100a tensor cores.
 //
 // Row t of the n_i rows of sequence i, head h, kv head g = h n_kv / n_head:
 //   S_j = scale <q, k_j> over the prefix's tokens and the sequence's own
 //   tokens 0 .. len_i - n_i + t;  out = sum_j softmax(S)_j v_j;  no token
 //   visible: out = 0.
+//
+// Arithmetic.  Keys and values stay the integers they are in the cache: a
+// query row is scaled to integers of 24 bits and split into three signed
+// 8-bit digits, a tile's probabilities (times the value scales) are integers
+// of 23 bits split into three unsigned ones, and both products are
+// tcgen05.mma kind::i8 with exact s32 sums -- no conversion of the cache, no
+// 16-bit rounding anywhere.  The digits are further columns of the same
+// product (N = 3 rows), so a page of keys is one M = 128 (tokens) operand and
+// a page of values one M = 128 (dimensions) operand whatever the number of
+// rows.  s32 to f32: |sum| < 2^22, so sum + (bits of 1.5 2^23) is a float 1.5
+// 2^23 + sum (an integer add and an f32 add, not the conversion pipe).  A
+// probability p times weight w becomes an integer as the mantissa of the
+// float 2^23 + p w, whose three low bytes are the digits.
+//
+// Scores are compared before the row's query scale and the softmax scale are
+// applied (z = sum * key scale), and the exponent is fma(z, c, -reference): a
+// rounding of c or of the reference is common to the row and cancels.
+//
+// One pass with a running maximum and sum per row; each tile's product is
+// folded into f32 registers, so rounding does not grow with the number of
+// tokens beyond an f32 sum over tiles.
+//
+// Work split.  A unit is (kv head, group of up to RT rows, the pages they
+// see): the prefix with all rows of all sequences (its pages are read once
+// per row group), and each sequence's own pages with its rows.  The units'
+// tiles (pages) form one line, cut into equal pieces, one per CTA, whatever
+// the mixture of lengths; a CTA's piece of a unit leaves a partial (maximum,
+// sum, unnormalised output) per row, and a second kernel joins a row's
+// partials.  Lengths live on the device: every CTA computes the line's layout
+// from them, so a captured call follows them.
+//
+// A CTA: warps 0..7 score and fold, warp 8 copies pages (bulk copies, one for
+// a whole page), warp 9 issues the products.  The score product of a tile is
+// issued before the value product of the tile before it, so the tensor core
+// works while the softmax does.  A tile's probabilities take the place of its
+// keys in shared memory.
 #include "eos_kernels.h"
 #include "kv_q8.cuh"
 
 namespace eos {
+
+constexpr uint32_t kAttnMaxCtas = 320;    // bound on the grid (scratch is sized with it)
+constexpr uint32_t kAttnThreads = 320;    // 8 softmax warps, a copy warp, a product warp
+constexpr uint32_t kAttnRows = 16;        // rows of a group: three digits of each are the columns of a product
+constexpr uint32_t kAttnMl = 8;           // floats per partial row: maximum, 3 unused, 4 partial sums
+constexpr float kAttnQMax = 8300000.0f;   // largest query integer (three balanced digits hold 127 * 65793)
+constexpr float kAttnMagic = 12582912.0f; // 1.5 * 2^23
+
+// Division of x < 2^31 by a launch constant: a multiplication (error below
+// 1 / d for these x, so the quotient is exact).
+struct AttnDiv {
+  uint32_t d, shift;
+  uint64_t mul;
+};
+__device__ __forceinline__ uint32_t attn_div(uint32_t x, const AttnDiv& v) {
+  return (uint32_t)(__umul64hi((uint64_t)x << 32, v.mul) >> v.shift);
+}
+inline AttnDiv attn_divisor(uint32_t d) {  // mul = ceil(2^(32 + s) / d), 2^(s - 1) < d <= 2^s
+  AttnDiv v{d, 0, 0};
+  while ((1ull << v.shift) < d) ++v.shift;
+  v.mul = (uint64_t)((((unsigned __int128)1 << (32u + v.shift)) + d - 1u) / d);
+  return v;
+}
 
 struct KvAttnParams {
   KvRows rows;
@@ -17,101 +76,1008 @@ struct KvAttnParams {
   const uint32_t* prefix_len;
   const uint32_t* table;
   const uint32_t* seq_len;
-  uint32_t max_prefix, table_stride, max_len;
-  uint32_t n_pages, n_head, n_kv_head;
+  uint32_t max_prefix, table_stride, max_len, max_rows;
+  uint32_t n_pages, n_head, n_kv_head, group;
+  AttnDiv by_group, by_kv_head;
   const float* q;
   float* out;
   uint64_t q_stride, out_stride;
   float scale_log2;  // scale * log2(e)
+  uint32_t* plan;    // quantum, prefix tiles, prefix row groups, prefix work, then the sequences' running work
+  float *po, *pml;   // prefix partials: [unit + CTA][half][row][HD], [unit + CTA][half][row][kAttnMl]
+  float *so, *sml;   // the sequences' partials, with seq_cap rows
+  uint32_t seq_cap, seq_groups;  // rows of a sequence partial; row groups reserved per sequence
   uint32_t* err;
 };
 
-// One CTA of 128 threads per (row, head): a page at a time, thread = token
-// for the scores, thread = dimension (HD / 128 each) for the values.
-template <uint32_t HD>
-__global__ void __launch_bounds__(128) kv_attn_simple_kernel(const KvAttnParams p) {
-  __shared__ float qs[HD], ps[kKvPage], red[4];
-  const uint32_t r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const uint32_t i = kv_row_seq(p.rows, r);
-  if (i >= p.rows.n_seq) return;
-  const uint32_t r0 = kv_row_start(p.rows, i), r1 = kv_row_start(p.rows, i + 1u);
-  const uint32_t g = (uint32_t)(((uint64_t)h * p.n_kv_head) / p.n_head);
-  for (uint32_t d = tid; d < HD; d += 128u) qs[d] = p.q[r * p.q_stride + h * HD + d];
-  constexpr uint32_t ND = (HD + 127u) / 128u;
-  float o[ND] = {}, m = -INFINITY, l = 0.0f;
-  for (uint32_t part = 0; part < 2; ++part) {
-    uint32_t len = 0;
-    if (part == 0) {
-      len = p.prefix_len != nullptr ? *p.prefix_len : 0u;
-      if (len > p.max_prefix) {
-        report(p.err, EOS_DEVERR_RANGE);
-        len = p.max_prefix;
-      }
+__host__ __device__ constexpr uint32_t attn_ceil(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
+
+// A unit's length on the line: its tiles behind kAttnStart places for what
+// every unit costs besides (its queries, its partial).
+constexpr uint32_t kAttnStart = 1;
+__host__ __device__ constexpr uint32_t attn_cost(uint32_t tiles) { return tiles ? tiles + kAttnStart : 0u; }
+
+// Rows and tokens of a sequence, cut to their bounds.
+struct AttnSeq {
+  uint32_t r0, n, len;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const KvAttnParams& p, uint32_t i) {
+  AttnSeq s;
+  const uint32_t len = p.seq_len[i], r1 = kv_row_start(p.rows, i + 1u);
+  s.r0 = kv_row_start(p.rows, i);
+  s.n = r1 > s.r0 ? r1 - s.r0 : 0u;
+  s.len = len < p.max_len ? len : p.max_len;
+  return s;
+}
+// Places of a sequence on the line (rows beyond max_rows are left out).
+__device__ __forceinline__ uint32_t attn_seq_work(const KvAttnParams& p, const AttnSeq& s) {
+  const uint32_t n = s.n < p.max_rows ? s.n : p.max_rows;
+  return p.n_kv_head * attn_ceil(n * p.group, kAttnRows) * attn_cost(attn_ceil(s.len, kKvPage));
+}
+
+struct AttnPlan {
+  uint32_t quantum, tp, rgp, wp, rows_p, prefix;
+  AttnSeq mine;  // sequence `lane`
+};
+
+// One piece of a unit (the whole copy warp computes it).
+struct AttnSeg {
+  uint32_t head, rg;        // kv head, row group
+  uint32_t step;            // places of the line that the piece takes
+  uint32_t tile0, tiles;    // pages [tile0, tile0 + tiles) of the unit
+  uint32_t seq;             // sequence, or n_seq for the prefix
+  uint32_t row0, rows;      // first (query row * group + head in group) of the group, how many
+  uint32_t base_row;        // query row of the unit's row 0
+  uint32_t len, n;          // tokens of the unit; rows of the sequence
+  uint32_t unit;            // partial index without the CTA
+};
+
+__device__ __forceinline__ AttnSeg attn_segment(const KvAttnParams& p, const AttnPlan& pl, const uint32_t* cum,
+                                                uint32_t w, uint32_t w1) {
+  AttnSeg s;
+  uint32_t tiles, x, u, at;
+  if (w < pl.wp) {
+    tiles = pl.tp;
+    x = w;
+    u = x / attn_cost(tiles);
+    at = x - u * attn_cost(tiles);
+    s.head = u / pl.rgp;
+    s.rg = u - s.head * pl.rgp;
+    s.seq = p.rows.n_seq;
+    s.base_row = 0;
+    s.len = pl.prefix;
+    s.n = 0;
+    s.row0 = s.rg * kAttnRows;
+    s.rows = pl.rows_p * p.group - s.row0;
+    s.unit = u;
+  } else {
+    x = w - pl.wp;
+    uint32_t lo = 0, hi = p.rows.n_seq;  // cum[lo] <= x < cum[hi]
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (cum[mid] <= x) lo = mid;
+      else hi = mid;
+    }
+    x -= cum[lo];
+    // the first 32 sequences sit in the lanes' registers
+    AttnSeq q;
+    if (lo < 32u) {
+      q.r0 = __shfl_sync(0xffffffffu, pl.mine.r0, lo);
+      q.n = __shfl_sync(0xffffffffu, pl.mine.n, lo);
+      q.len = __shfl_sync(0xffffffffu, pl.mine.len, lo);
     } else {
-      uint32_t all = p.seq_len[i];
-      if (all > p.max_len) {
-        report(p.err, EOS_DEVERR_RANGE);
-        all = p.max_len;
-      }
-      const int64_t seen = (int64_t)all - (int64_t)(r1 - r0) + 1 + (int64_t)(r - r0);
-      len = seen > 0 ? (uint32_t)seen : 0u;
+      q = attn_seq(p, lo);
     }
-    const uint32_t* table = part == 0 ? p.prefix_table : p.table + (size_t)i * p.table_stride;
-    for (uint32_t t0 = 0; t0 < len; t0 += kKvPage) {
-      const uint32_t page = table[t0 / kKvPage];
-      if (page >= p.n_pages) {
-        report(p.err, EOS_DEVERR_RANGE);
-        continue;
-      }
-      const uint8_t* blk = p.pages + ((size_t)page * p.n_kv_head + g) * kv_block_bytes(HD);
-      __syncthreads();
-      const bool on = t0 + tid < len;
-      float s = -INFINITY, vs = 0.0f;
-      if (on) {
-        float acc = 0.0f;
-        for (uint32_t d = 0; d < HD; ++d) acc = fmaf((float)(int8_t)blk[kv_k_offset<HD>(tid, d)], qs[d], acc);
-        s = acc * *reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(tid, 0)) * p.scale_log2;
-        vs = *reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(tid, 1));
-      }
-      float cm = s;
-      for (int sh = 16; sh > 0; sh >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, sh));
-      if ((tid & 31u) == 0) red[tid >> 5] = cm;
-      __syncthreads();
-      const float nm = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-      const float mu = nm == -INFINITY ? 0.0f : nm;
-      const float f = exp2f(m - mu), e = on ? exp2f(s - mu) : 0.0f;
-      float ls = e;
-      for (int sh = 16; sh > 0; sh >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, sh);
-      ps[tid] = on ? e * vs : 0.0f;
-      __syncthreads();
-      if ((tid & 31u) == 0) red[tid >> 5] = ls;
-      __syncthreads();
-      l = fmaf(l, f, red[0] + red[1] + red[2] + red[3]);
-      m = nm;
-#pragma unroll
-      for (uint32_t x = 0; x < ND; ++x) {
-        const uint32_t d = x * 128u + tid;
-        o[x] *= f;
-        if (d < HD)
-          for (uint32_t t = 0; t < kKvPage; ++t)
-            if (t0 + t < len) o[x] = fmaf(ps[t], (float)(int8_t)blk[kv_v_offset<HD>(t, d)], o[x]);
-      }
-    }
+    const uint32_t n = q.n < p.max_rows ? q.n : p.max_rows;
+    tiles = attn_ceil(q.len, kKvPage);
+    u = x / attn_cost(tiles);
+    at = x - u * attn_cost(tiles);
+    s.rg = attn_div(u, p.by_kv_head);
+    s.head = u - s.rg * p.n_kv_head;
+    s.seq = lo;
+    s.base_row = q.r0;
+    s.len = q.len;
+    s.n = q.n;
+    s.row0 = s.rg * kAttnRows;
+    s.rows = n * p.group - s.row0;
+    s.unit = lo * p.seq_groups * p.n_kv_head + u;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (uint32_t x = 0; x < ND; ++x) {
-    const uint32_t d = x * 128u + tid;
-    if (d < HD) p.out[r * p.out_stride + h * HD + d] = o[x] * inv;
+  if (s.rows > kAttnRows) s.rows = kAttnRows;
+  s.step = attn_cost(tiles) - at;
+  if (s.step > w1 - w) s.step = w1 - w;
+  s.tile0 = at > kAttnStart ? at - kAttnStart : 0u;
+  s.tiles = at + s.step > kAttnStart ? at + s.step - kAttnStart - s.tile0 : 0u;
+  return s;
+}
+
+// ---- tcgen05 --------------------------------------------------------------
+// K-major shared-memory operand: start address >> 4, LBO 16 B (unused when
+// swizzled), SBO = 8 rows, version 1, layout type (2: 128-byte swizzle, 4:
+// 64-byte, 6: 32-byte).  Advancing K by 32 bytes adds 2 to the start field.
+__device__ __forceinline__ uint64_t attn_desc(uint32_t addr, uint32_t row_bytes) {
+  const uint64_t type = row_bytes == 128u ? 2u : (row_bytes == 64u ? 4u : 6u);
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)((8u * row_bytes) >> 4) << 32) |
+         ((uint64_t)1u << 46) | (type << 61);
+}
+// Instruction descriptor, kind::i8: D s32, A s8, B s8 or u8, both K-major.
+__device__ constexpr uint32_t attn_idesc(bool b_signed, uint32_t n) {
+  return (2u << 4) | (1u << 7) | ((b_signed ? 1u : 0u) << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void attn_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void attn_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void attn_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void attn_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void attn_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 16 TMEM lanes x 8 columns: thread t gets r[0..1] = lane t / 4, columns
+// 2 (t % 4) + {0, 1}, and r[2..3] the same columns of lane t / 4 + 8.
+__device__ __forceinline__ void attn_ld(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void attn_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void attn_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float attn_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Pairs of f32 (the two columns of an accumulator fragment).
+__device__ __forceinline__ uint64_t attn_pack(float2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 attn_unpack(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ float2 attn_fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(attn_pack(a)), "l"(attn_pack(b)), "l"(attn_pack(c)));
+  return attn_unpack(d);
+}
+__device__ __forceinline__ float2 attn_add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(attn_pack(a)), "l"(attn_pack(b)));
+  return attn_unpack(d);
+}
+__device__ __forceinline__ float2 attn_mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(attn_pack(a)), "l"(attn_pack(b)));
+  return attn_unpack(d);
+}
+__device__ __forceinline__ float2 attn_two(float x) { return make_float2(x, x); }
+// s32 sums below 2^22 as floats.
+__device__ __forceinline__ float2 attn_float(uint32_t a, uint32_t b) {
+  return attn_add2(make_float2(__uint_as_float(a + 0x4B400000u), __uint_as_float(b + 0x4B400000u)),
+                   attn_two(-kAttnMagic));
+}
+// Value sums: D2 65536 + D1 256 + D0, every bit (a bias of the low digit
+// would add up over the tiles).
+__device__ __forceinline__ float2 attn_join_value(const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
+  return attn_fma2(attn_float(d2[0], d2[1]), attn_two(65536.0f),
+                   attn_fma2(attn_float(d1[0], d1[1]), attn_two(256.0f), attn_float(d0[0], d0[1])));
+}
+// Score sums: D2 256 + D1 + floor(D0 / 256), in units of 256 (less than one
+// unit off, of about 2^22 for a typical score).
+__device__ __forceinline__ float2 attn_join_score(const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
+  const uint32_t y0 = d1[0] + (uint32_t)((int32_t)d0[0] >> 8), y1 = d1[1] + (uint32_t)((int32_t)d0[1] >> 8);
+  return attn_fma2(attn_float(d2[0], d2[1]), attn_two(256.0f), attn_float(y0, y1));
+}
+// Bytes 0, 1 and 2 of four words as three words.
+__device__ __forceinline__ void attn_digits(const uint32_t* b, uint32_t* w) {
+  const uint32_t lo01 = __byte_perm(b[0], b[1], 0x5140), lo23 = __byte_perm(b[2], b[3], 0x5140);
+  w[0] = __byte_perm(lo01, lo23, 0x5410);
+  w[1] = __byte_perm(lo01, lo23, 0x7632);
+  w[2] = __byte_perm(__byte_perm(b[0], b[1], 0x0062), __byte_perm(b[2], b[3], 0x0062), 0x5410);
+}
+
+// mbar_wait, reading the clock only once in 64 polls: its read takes longer
+// than a tile's waits.
+__device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < 64u; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    for (uint32_t i = 0; i < 64u; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (global_timer_ns() - t0 > EOS_WAIT_LIMIT_NS) return false;
   }
 }
 
-size_t kv_attn_scratch_bytes(const KvPool&, const KvAttnBatch&, uint32_t) { return 16; }
+// One look at a barrier, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// ---- geometry of a CTA ------------------------------------------------------
+template <uint32_t HD>
+struct AttnGeo {
+  static constexpr uint32_t kBlock = kv_block_bytes(HD);
+  static constexpr uint32_t kQRow = HD < 128u ? HD : 128u;      // bytes of an operand row of K and Q
+  static constexpr uint32_t kPanels = HD <= 128u ? 1u : HD / 128u;
+  static constexpr uint32_t kQBytes = 3u * kAttnRows * HD;      // a job's query digits
+  static constexpr uint32_t kCtas = HD <= 128u ? 2u : 1u;       // per SM
+  static constexpr uint32_t kStages = HD == 64u ? 5u : 3u;      // as many blocks as shared memory holds
+  static constexpr uint32_t kAcc = 64u;                         // TMEM columns between accumulators (48 used)
+  static constexpr uint32_t kTmem = HD <= 128u ? 256u : 512u;   // scores of two tiles, values of two tiles
+  static constexpr uint32_t kControl = 2048u;  // barriers, scales, maxima; also what a 64-dimension value operand reads past its end
+  static_assert(3u * kAttnRows * kKvPage <= kKvPage * HD, "a tile's probabilities take the place of its keys");
+  static_assert(kAttnRows * HD * 4u <= kBlock, "a job's queries fit a stage");
+  static constexpr uint32_t smem(uint32_t n_seq) {
+    return kQBytes + kStages * kBlock + kControl + ((n_seq + 1u) * 4u + 15u) / 16u * 16u + 1024u;
+  }
+};
+
+// A piece of a unit as the copy warp hands it to the others.
+struct AttnJob {
+  uint32_t tiles;           // 0: no further piece
+  uint32_t tile0, rows, row0, len, n, unit, prefix;
+};
+
+struct AttnBars {
+  uint64_t full[5], empty[5], q_ready, job_free, done;
+  uint64_t s_full[2], s_free[2], p_ready[2], o_full[2], xmax[2];  // per half
+  uint32_t tmem, ok[5];
+  AttnJob job[2];
+};
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kernel(const KvAttnParams p) {
+  using G = AttnGeo<HD>;
+  constexpr uint32_t RT = kAttnRows, S = G::kStages;
+  constexpr uint32_t NC = RT / 8u;                           // column chunks of 8
+  constexpr uint32_t MH = HD <= 128u ? 1u : HD / 128u;       // value products of 128 dimensions
+  extern __shared__ uint8_t attn_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(attn_smem_raw) + 1023u) & ~uintptr_t(1023));
+  uint8_t* qop = smem;                                       // query digits
+  uint8_t* stages = smem + G::kQBytes;
+  uint8_t* control = stages + S * G::kBlock;
+  AttnBars& bar = *reinterpret_cast<AttnBars*>(control);
+  float* qs = reinterpret_cast<float*>(control + 512u);      // [2][RT] query scales
+  float* xm = qs + 2u * RT;                                  // [half][2][4][RT] tile maxima per quarter
+  uint32_t* cum = reinterpret_cast<uint32_t*>(control + G::kControl);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+  // the copy warp's first loads fly while the barriers are set up
+  AttnSeq first{0, 0, 0};
+  uint32_t prefix_len = 0, rows_end = 0;
+  if (warp == 8) {
+    if (p.prefix_len != nullptr) prefix_len = *p.prefix_len;
+    rows_end = kv_row_start(p.rows, p.rows.n_seq);
+    if (lane < p.rows.n_seq) first = attn_seq(p, lane);
+  }
+  if (tid == 0) {
+    for (uint32_t s = 0; s < S; ++s) {
+      mbar_init(&bar.full[s], 1);
+      mbar_init(&bar.empty[s], 1);
+    }
+    mbar_init(&bar.q_ready, 8);
+    mbar_init(&bar.job_free, 8);
+    mbar_init(&bar.done, 1);
+    for (uint32_t h = 0; h < 2u; ++h) {
+      mbar_init(&bar.s_full[h], 1);
+      mbar_init(&bar.s_free[h], 4);
+      mbar_init(&bar.p_ready[h], 4);
+      mbar_init(&bar.o_full[h], 1);
+      mbar_init(&bar.xmax[h], 4);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
+                 "r"(G::kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  attn_fence_before();
+  __syncthreads();
+  attn_fence_after();
+  pdl_trigger();  // the joining kernel may start; it waits for this grid's completion
+  const uint32_t tmem = bar.tmem;
+  // TMEM: scores of half h at h kAcc, value sums at (2 + h MH + mh) kAcc
+
+  if (warp == 8) {
+    // ---- the line's layout: prefix units, then the sequences' (running work in cum) ----
+    uint32_t carry = 0;
+    AttnPlan pl;
+    pl.mine = first;
+    for (uint32_t i0 = 0; i0 < p.rows.n_seq; i0 += 32u) {
+      uint32_t w = 0;
+      const bool in = i0 + lane < p.rows.n_seq;
+      if (in) w = attn_seq_work(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
+      uint32_t c = w;
+#pragma unroll
+      for (uint32_t o = 1; o < 32u; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c += t;
+      }
+      if (in) cum[i0 + lane] = carry + c - w;
+      carry += __shfl_sync(0xffffffffu, c, 31);
+    }
+    if (lane == 0) cum[p.rows.n_seq] = carry;
+    __syncwarp();
+    pl.prefix = prefix_len < p.max_prefix ? prefix_len : p.max_prefix;
+    pl.rows_p = rows_end;
+    pl.tp = attn_ceil(pl.prefix, kKvPage);
+    pl.rgp = attn_ceil(pl.rows_p * p.group, RT);
+    pl.wp = p.n_kv_head * pl.rgp * attn_cost(pl.tp);
+    const uint32_t total = pl.wp + carry;
+    pl.quantum = attn_ceil(total, gridDim.x);
+    const uint64_t w_lo = (uint64_t)blockIdx.x * pl.quantum;
+    uint32_t w = w_lo < total ? (uint32_t)w_lo : total;
+    const uint32_t w1 = w_lo + pl.quantum < total ? (uint32_t)(w_lo + pl.quantum) : total;
+    // ---- jobs: a stage with the piece's queries, then one per page ----
+    uint32_t x = 0, nj = 0;  // stages used; jobs
+    bool live = true;
+    auto stage_free = [&]() {  // lane 0: stage x % S may be filled
+      if (x >= S && !attn_wait(&bar.empty[x % S], (x / S - 1u) & 1u)) {
+        report(p.err, EOS_DEVERR_WAIT_EMPTY);
+        return false;
+      }
+      return true;
+    };
+    auto agree = [&](bool v) { return __shfl_sync(0xffffffffu, v ? 1u : 0u, 0) != 0u; };
+    for (bool more = true; more && live; ++nj) {
+      AttnSeg s{};
+      while (w < w1) {  // the next piece that holds a tile
+        s = attn_segment(p, pl, cum, w, w1);
+        w += s.step;
+        if (s.tiles > 0) break;
+      }
+      more = s.tiles > 0;
+      const uint32_t* table = s.seq == p.rows.n_seq ? p.prefix_table : p.table + (size_t)s.seq * p.table_stride;
+      uint32_t mine = lane < s.tiles ? table[s.tile0 + lane] : 0u;
+      if (lane == 0) {
+        live = stage_free();
+        if (live && nj > 0 && !attn_wait(&bar.job_free, (nj - 1u) & 1u)) {
+          report(p.err, EOS_DEVERR_WAIT_EMPTY);
+          live = false;
+        }
+        if (live) {
+          bar.job[nj & 1u] = AttnJob{s.tiles, s.tile0, s.rows, s.row0, s.len, s.n, s.unit, s.seq == p.rows.n_seq ? 1u : 0u};
+          if (more) mbar_arrive_expect_tx(&bar.full[x % S], s.rows * HD * 4u);
+          else mbar_arrive(&bar.full[x % S]);
+        }
+      }
+      live = agree(live);
+      if (!live) break;
+      if (more && lane < s.rows) {
+        const uint32_t fr = s.row0 + lane, xr = attn_div(fr, p.by_group);
+        attn_bulk(smem_u32(stages + (x % S) * G::kBlock + lane * HD * 4u),
+                  p.q + (size_t)(s.base_row + xr) * p.q_stride + (size_t)(s.head * p.group + fr - xr * p.group) * HD,
+                  HD * 4u, &bar.full[x % S]);
+      }
+      ++x;
+      for (uint32_t j = 0; j < s.tiles; ++j) {
+        if (j > 0 && j % 32u == 0) mine = j + lane < s.tiles ? table[s.tile0 + j + lane] : 0u;
+        const uint32_t page = __shfl_sync(0xffffffffu, mine, j % 32u);
+        if (lane == 0) {
+          const uint32_t st = x % S;
+          live = stage_free();
+          if (!live) {
+          } else if (page >= p.n_pages) {
+            report(p.err, EOS_DEVERR_RANGE);
+            bar.ok[st] = 0u;
+            mbar_arrive(&bar.full[st]);
+          } else {
+            bar.ok[st] = 1u;
+            const uint8_t* src = p.pages + ((size_t)page * p.n_kv_head + s.head) * G::kBlock;
+            const uint32_t dst = smem_u32(stages + st * G::kBlock);
+            const uint32_t left = s.len - (s.tile0 + j) * kKvPage;
+            if (left >= kKvPage) {
+              mbar_arrive_expect_tx(&bar.full[st], G::kBlock);
+              attn_bulk(dst, src, G::kBlock, &bar.full[st]);
+            } else {  // the rows, quarters and scales that hold tokens
+              const uint32_t kr = (left + 7u) / 8u * 8u * G::kQRow, nq = attn_ceil(left, kKvQuarter);
+              const uint32_t vb = nq * HD * kKvQuarter, sb = nq * 256u;
+              mbar_arrive_expect_tx(&bar.full[st], G::kPanels * kr + vb + sb);
+              for (uint32_t pn = 0; pn < G::kPanels; ++pn)
+                attn_bulk(dst + pn * kKvPage * 128u, src + pn * kKvPage * 128u, kr, &bar.full[st]);
+              attn_bulk(dst + kKvPage * HD, src + kKvPage * HD, vb, &bar.full[st]);
+              attn_bulk(dst + 2u * kKvPage * HD, src + 2u * kKvPage * HD, sb, &bar.full[st]);
+            }
+          }
+        }
+        live = agree(live);
+        if (!live) break;
+        ++x;
+      }
+    }
+    if (blockIdx.x == 0) {  // the layout for the joining kernel; lengths and rows beyond their bounds
+      if (lane == 0) {
+        p.plan[0] = pl.quantum;
+        p.plan[1] = pl.tp;
+        p.plan[2] = pl.rgp;
+        p.plan[3] = pl.wp;
+        if (prefix_len > p.max_prefix) report(p.err, EOS_DEVERR_RANGE);
+      }
+      for (uint32_t i = lane; i <= p.rows.n_seq; i += 32u) {
+        p.plan[4u + i] = cum[i];
+        if (i < p.rows.n_seq && (p.seq_len[i] > p.max_len || attn_seq(p, i).n > p.max_rows))
+          report(p.err, EOS_DEVERR_RANGE);
+      }
+    }
+    // never leave copies in flight: every stage's last use has landed
+    if (lane == 0)
+      for (uint32_t y = x > S ? x - S : 0u; y < x; ++y)
+        if (!attn_wait(&bar.full[y % S], (y / S) & 1u)) report(p.err, EOS_DEVERR_DRAIN);
+  } else if (warp == 9) {
+    // ---- products: tile j of a job belongs to half j % 2 ----
+    if (lane == 0) {
+      bool live = true;
+      uint32_t x = 0;               // stages used before the job
+      uint32_t ns0 = 0, ns1 = 0;    // score products issued, per half
+      uint32_t nv0 = 0, nv1 = 0;    // value products issued
+      for (uint32_t nj = 0; live; ++nj) {
+        if (!attn_wait(&bar.q_ready, nj & 1u)) {
+          report(p.err, EOS_DEVERR_WAIT_ACT);
+          break;
+        }
+        const uint32_t tiles = bar.job[nj & 1u].tiles;
+        if (tiles == 0) break;
+        attn_fence_after();
+        mbar_arrive(&bar.empty[x % S]);  // the queries have been read
+        uint32_t js = 0, jv = 0, jo0 = 0, jo1 = 1, polls = 0;  // next score tile; values done; next value tile per half
+        uint64_t t0 = 0;
+        while (jv < tiles) {
+          bool moved = false;
+          {
+            const uint32_t h = js & 1u, y = x + 1u + js;
+            if (js < tiles && mbar_test(&bar.full[y % S], (y / S) & 1u) &&
+                ((h ? ns1 : ns0) == 0 || mbar_test(&bar.s_free[h], ((h ? ns1 : ns0) - 1u) & 1u))) {
+              attn_fence_after();
+              const uint32_t ka = smem_u32(stages + (y % S) * G::kBlock), qa = smem_u32(qop);
+              constexpr uint32_t id = attn_idesc(true, 3u * RT);
+#pragma unroll
+              for (uint32_t ks = 0; ks < HD / 32u; ++ks) {
+                const uint32_t panel = ks / 4u, off = (ks % 4u) * 32u;
+                attn_mma(tmem + h * G::kAcc, attn_desc(ka + panel * kKvPage * 128u + off, G::kQRow),
+                         attn_desc(qa + panel * 3u * RT * 128u + off, G::kQRow), id, ks > 0 ? 1u : 0u);
+              }
+              attn_commit(&bar.s_full[h]);
+              ++(h ? ns1 : ns0);
+              ++js;
+              moved = true;
+            }
+          }
+#pragma unroll
+          for (uint32_t h = 0; h < 2u; ++h) {
+            uint32_t& jo = h ? jo1 : jo0;
+            uint32_t& nv = h ? nv1 : nv0;
+            if (jo < js && mbar_test(&bar.p_ready[h], nv & 1u)) {
+              attn_fence_after();
+              const uint32_t st = (x + 1u + jo) % S;
+              const uint32_t sa = smem_u32(stages + st * G::kBlock);
+              constexpr uint32_t id = attn_idesc(false, 3u * RT);
+#pragma unroll
+              for (uint32_t mh = 0; mh < MH; ++mh)
+#pragma unroll
+                for (uint32_t qd = 0; qd < 4u; ++qd)
+                  attn_mma(tmem + G::kAcc * (2u + h * MH + mh),
+                           attn_desc(sa + kKvPage * HD + qd * HD * kKvQuarter + mh * 128u * kKvQuarter, 32u),
+                           attn_desc(sa + qd * 32u, 128u), id, qd > 0 ? 1u : 0u);
+              attn_commit(&bar.o_full[h]);
+              attn_commit(&bar.empty[st]);
+              ++nv;
+              jo += 2u;
+              ++jv;
+              moved = true;
+            }
+          }
+          if (moved) {
+            polls = 0;
+            t0 = 0;
+          } else if (++polls % 256u == 0) {  // bounded, like every wait
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > EOS_WAIT_LIMIT_NS) {
+              report(p.err, EOS_DEVERR_WAIT_FULL);
+              live = false;
+              break;
+            }
+          }
+        }
+        x += 1u + tiles;
+      }
+      // TMEM is freed, and shared memory left, only after every product issued has completed
+      attn_commit(&bar.done);
+      if (!attn_wait(&bar.done, 0)) report(p.err, EOS_DEVERR_DRAIN);
+    }
+  } else {
+    // ---- softmax and folding: warps 4 h + quarter work on the tiles of half h ----
+    const uint32_t quad = warp & 3u, half = warp >> 2, g = lane >> 2, cq = lane & 3u;
+    uint32_t x = 0;               // stages used before the job
+    uint32_t n_own = 0, n_other = 0;  // tiles of this half and of the other before the job
+    // job n's queries (in stage y) as three signed digits each, rows warp, warp + 8
+    auto prepare = [&](uint32_t n, uint32_t y) {
+      if (!__all_sync(0xffffffffu, attn_wait(&bar.full[y % S], (y / S) & 1u))) return false;
+      const uint32_t rows = bar.job[n & 1u].rows;
+      const float* raw = reinterpret_cast<const float*>(stages + (y % S) * G::kBlock);
+      if (bar.job[n & 1u].tiles > 0) {
+#pragma unroll
+        for (uint32_t r = warp; r < RT; r += 8u) {
+          float scale = 0.0f;
+          if (r < rows) {
+            float4 v[G::kPanels];
+            uint32_t amax = 0;
+#pragma unroll
+            for (uint32_t pn = 0; pn < G::kPanels; ++pn) {
+              v[pn] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (HD >= 128u || lane < HD / 4u) v[pn] = *reinterpret_cast<const float4*>(raw + r * HD + pn * 128u + lane * 4u);
+              amax = max(max(amax, __float_as_uint(v[pn].x) & 0x7fffffffu), __float_as_uint(v[pn].y) & 0x7fffffffu);
+              amax = max(max(amax, __float_as_uint(v[pn].z) & 0x7fffffffu), __float_as_uint(v[pn].w) & 0x7fffffffu);
+            }
+            amax = __reduce_max_sync(0xffffffffu, amax);
+            const bool finite = amax < 0x7f800000u;
+            const float top = fmaxf(__uint_as_float(amax), 1e-30f);
+            // a negative scale turns the integers' sign: larger products are larger scores
+            const float inv = finite ? __fdiv_rn(p.scale_log2 < 0.0f ? -kAttnQMax : kAttnQMax, top) : 0.0f;
+            // (above 0, so that a hidden token's -infinity stays one when the softmax scale is 0)
+            scale = finite ? fmaxf(__fdiv_rn(top, kAttnQMax) * (256.0f * fabsf(p.scale_log2)), 1e-37f) : NAN;
+#pragma unroll
+            for (uint32_t pn = 0; pn < G::kPanels; ++pn) {
+              const float f[4] = {v[pn].x, v[pn].y, v[pn].z, v[pn].w};
+              uint32_t b[4], d[3];
+#pragma unroll
+              for (uint32_t e = 0; e < 4u; ++e)  // balanced digits: bytes of (x + 0x808080) ^ 0x808080
+                b[e] = (uint32_t)((finite ? __float2int_rn(f[e] * inv) : 0) + 0x808080) ^ 0x808080u;
+              attn_digits(b, d);
+              if (HD >= 128u || lane < HD / 4u) {
+#pragma unroll
+                for (uint32_t e = 0; e < 3u; ++e) {
+                  const uint32_t row = e * RT + r;
+                  const uint32_t sw = G::kQRow == 128u ? (row & 7u) : ((row >> 1) & 3u);
+                  *reinterpret_cast<uint32_t*>(qop + pn * 3u * RT * 128u + row * G::kQRow +
+                                               (((lane >> 2) ^ sw) << 4) + (lane & 3u) * 4u) = d[e];
+                }
+              }
+            }
+          }
+          if (lane == 0) qs[(n & 1u) * RT + r] = scale;
+        }
+      }
+      attn_fence_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bar.job_free);
+        mbar_arrive(&bar.q_ready);
+      }
+      return true;
+    };
+    bool live = prepare(0, 0);
+    for (uint32_t nj = 0; live; ++nj) {
+      live = __all_sync(0xffffffffu, attn_wait(&bar.q_ready, nj & 1u)) != 0;
+      if (!live) break;
+      const AttnJob s = bar.job[nj & 1u];
+      if (s.tiles == 0) break;
+      const uint32_t nact = s.rows > 8u ? 2u : 1u;  // chunks of 8 columns in use
+      // this thread's columns 8 y + 2 cq + {0, 1}
+      float2 qsc[NC], m[NC], l[NC], f[NC], o[NC][MH][4];
+#pragma unroll
+      for (uint32_t y = 0; y < NC; ++y) {
+        qsc[y] = *reinterpret_cast<const float2*>(qs + (nj & 1u) * RT + 8u * y + 2u * cq);
+        m[y] = attn_two(-INFINITY);
+        l[y] = attn_two(0.0f);
+        f[y] = attn_two(1.0f);
+#pragma unroll
+        for (uint32_t mh = 0; mh < MH; ++mh)
+#pragma unroll
+          for (uint32_t j = 0; j < 4u; ++j) o[y][mh][j] = attn_two(0.0f);
+      }
+      // tokens that column `col` sees; all columns see those below `common`
+      auto limit = [&](uint32_t col) -> uint32_t {
+        if (s.prefix) return s.len;
+        const int64_t seen = (int64_t)s.len - (int64_t)s.n + 1 + (int64_t)attn_div(s.row0 + col, p.by_group);
+        return seen <= 0 ? 0u : (seen < (int64_t)s.len ? (uint32_t)seen : s.len);
+      };
+      const uint32_t common = limit(0);
+      float fold = 0.0f;       // the last tile's probability unit
+      uint32_t it = n_own;     // tiles of this half so far
+      // o = o f + unit * (value product of the tile before)
+      auto fold_tile = [&]() {
+        if (!__all_sync(0xffffffffu, attn_wait(&bar.o_full[half], (it - 1u) & 1u))) return false;
+        attn_fence_after();
+        if (HD >= 128u || quad * 32u < HD) {
+          const float2 unit = attn_two(fold);
+#pragma unroll
+          for (uint32_t y = 0; y < NC; ++y) {
+            if (y >= nact) break;  // warp-uniform
+#pragma unroll
+            for (uint32_t mh = 0; mh < MH; ++mh) {
+              uint32_t r[3][8];
+#pragma unroll
+              for (uint32_t e = 0; e < 3u; ++e)
+#pragma unroll
+                for (uint32_t hh = 0; hh < 2u; ++hh)
+                  attn_ld(tmem + G::kAcc * (2u + half * MH + mh) + ((quad * 32u + 16u * hh) << 16) + e * RT + 8u * y,
+                          &r[e][4u * hh]);
+              attn_ld_wait();
+#pragma unroll
+              for (uint32_t j = 0; j < 4u; ++j)
+                o[y][mh][j] = attn_fma2(attn_join_value(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), unit,
+                                        attn_mul2(o[y][mh][j], f[y]));
+            }
+          }
+        }
+        attn_fence_before();
+        return true;
+      };
+      for (uint32_t t = half; t < s.tiles && live; t += 2u) {
+        const uint32_t pos = x + 1u + t, st = pos % S;
+        // the scores, and (already complete) the page, whose scales are read here
+        live = __all_sync(0xffffffffu, attn_wait(&bar.s_full[half], it & 1u) &&
+                                           attn_wait(&bar.full[st], (pos / S) & 1u)) != 0;
+        if (!live) break;
+        attn_fence_after();
+        const uint32_t tok0 = (s.tile0 + t) * kKvPage;
+        const uint8_t* sc = stages + st * G::kBlock + 2u * kKvPage * HD;
+        const uint32_t avail = bar.ok[st] ? s.len - tok0 : 0u;  // tokens of the tile (may exceed a page)
+        // unit of the probabilities: a power of two from the tile's largest value scale
+        uint32_t top = 0;
+#pragma unroll
+        for (uint32_t q = 0; q < 4u; ++q) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(sc + q * 256u + 128u + lane * 4u);
+          if (q * 32u + lane < avail && v < 0x7f800000u && v > top) top = v;
+        }
+        top = __reduce_max_sync(0xffffffffu, top) >> 23;
+        top = top < 23u ? 23u : top;
+        const float up = __uint_as_float((276u - top) << 23);           // 2^(22 - exponent)
+        const float unit = __uint_as_float((top - 22u) << 23);          // 2^(exponent - 22)
+        // this thread's four tokens: quarter quad, g + 8 j
+        float ks[4], vw[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) {
+          const uint32_t u = g + 8u * j;
+          const bool in = quad * 32u + u < avail;
+          const float kv = *reinterpret_cast<const float*>(sc + quad * 256u + u * 4u);
+          const float vv = *reinterpret_cast<const float*>(sc + quad * 256u + 128u + u * 4u);
+          const bool sound = vv < INFINITY;                             // a NaN or infinite value row: NaN score
+          ks[j] = in ? (sound ? kv : NAN) : 0.0f;
+          vw[j] = in && sound ? vv * up : 0.0f;
+        }
+        const bool whole = avail >= kKvPage && tok0 + kKvPage <= common;  // nothing to mask
+        float* xmt = xm + (half * 2u + (it & 1u)) * 4u * RT + 2u * cq;
+        float2 sv[NC][4];
+#pragma unroll
+        for (uint32_t y = 0; y < NC; ++y) {
+          if (y >= nact) break;  // warp-uniform
+          uint32_t r[3][8];
+#pragma unroll
+          for (uint32_t e = 0; e < 3u; ++e)
+#pragma unroll
+            for (uint32_t hh = 0; hh < 2u; ++hh)
+              attn_ld(tmem + half * G::kAcc + ((quad * 32u + 16u * hh) << 16) + e * RT + 8u * y, &r[e][4u * hh]);
+          attn_ld_wait();
+#pragma unroll
+          for (uint32_t j = 0; j < 4u; ++j)
+            sv[y][j] = attn_mul2(attn_join_score(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), attn_two(ks[j]));
+          if (!whole) {
+            const uint32_t col = 8u * y + 2u * cq;
+            const uint32_t lim0 = limit(col), lim1 = limit(col + 1u);
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) {
+              const uint32_t tok = quad * 32u + g + 8u * j;
+              if (tok >= avail || tok0 + tok >= lim0) sv[y][j].x = -INFINITY;
+              if (tok >= avail || tok0 + tok >= lim1) sv[y][j].y = -INFINITY;
+            }
+          }
+          float2 mx = make_float2(fmaxf(fmaxf(sv[y][0].x, sv[y][1].x), fmaxf(sv[y][2].x, sv[y][3].x)),
+                                  fmaxf(fmaxf(sv[y][0].y, sv[y][1].y), fmaxf(sv[y][2].y, sv[y][3].y)));
+#pragma unroll
+          for (uint32_t o2 = 4; o2 < 32u; o2 <<= 1) {
+            mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o2));
+            mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o2));
+          }
+          if (g == 0) *reinterpret_cast<float2*>(xmt + quad * RT + 8u * y) = mx;
+        }
+        attn_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.s_free[half]);
+          mbar_arrive(&bar.xmax[half]);
+        }
+        if (t > half) live = fold_tile();
+        if (live) live = __all_sync(0xffffffffu, attn_wait(&bar.xmax[half], it & 1u)) != 0;
+        if (!live) break;
+        uint8_t* pop = stages + st * G::kBlock;  // the probabilities take the place of the keys
+#pragma unroll
+        for (uint32_t y = 0; y < NC; ++y) {
+          if (y >= nact) break;  // warp-uniform
+          const uint32_t col = 8u * y + 2u * cq;
+          const float2 m0 = *reinterpret_cast<const float2*>(xmt + 8u * y),
+                       m1 = *reinterpret_cast<const float2*>(xmt + RT + 8u * y),
+                       m2 = *reinterpret_cast<const float2*>(xmt + 2u * RT + 8u * y),
+                       m3 = *reinterpret_cast<const float2*>(xmt + 3u * RT + 8u * y);
+          // the reference is rounded up, so that no probability exceeds 1
+          const float t0 = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x)), t1 = fmaxf(fmaxf(m0.y, m1.y), fmaxf(m2.y, m3.y));
+          const float2 nm = make_float2(fmaxf(t0 == -INFINITY ? t0 : __fmul_ru(t0, qsc[y].x), m[y].x),
+                                        fmaxf(t1 == -INFINITY ? t1 : __fmul_ru(t1, qsc[y].y), m[y].y));
+          const float2 neg = make_float2(nm.x == -INFINITY ? 0.0f : -nm.x, nm.y == -INFINITY ? 0.0f : -nm.y);
+          f[y] = make_float2(attn_ex2(m[y].x + neg.x), attn_ex2(m[y].y + neg.y));
+          m[y] = nm;
+          uint32_t b0[4], b1[4], d[3];
+          float2 ls = attn_two(0.0f);
+#pragma unroll
+          for (uint32_t j = 0; j < 4u; ++j) {
+            const float2 z = attn_fma2(sv[y][j], qsc[y], neg);
+            const float2 e = make_float2(attn_ex2(z.x), attn_ex2(z.y));
+            ls = attn_add2(ls, e);
+            const float2 w = attn_fma2(e, attn_two(vw[j]), attn_two(8388608.0f));
+            b0[j] = __float_as_uint(w.x);
+            b1[j] = __float_as_uint(w.y);
+          }
+          l[y] = attn_fma2(l[y], f[y], ls);
+          // row e RT + col of digit e, this thread's four tokens: one word
+          uint8_t* at = pop + (g & 3u) * 4u;
+          const uint32_t chunk = 2u * quad + (g >> 2);
+          attn_digits(b0, d);
+#pragma unroll
+          for (uint32_t e = 0; e < 3u; ++e)
+            *reinterpret_cast<uint32_t*>(at + (e * RT + col) * kKvPage + ((chunk ^ (col & 7u)) << 4)) = d[e];
+          attn_digits(b1, d);
+#pragma unroll
+          for (uint32_t e = 0; e < 3u; ++e)
+            *reinterpret_cast<uint32_t*>(at + (e * RT + col + 1u) * kKvPage + ((chunk ^ ((col + 1u) & 7u)) << 4)) = d[e];
+        }
+        fold = unit;
+        ++it;
+        attn_fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_ready[half]);
+      }
+      // the next job's queries, once both halves' score products have read
+      // this one's; then this half's last value product
+      const bool some = s.tiles > half;
+      const uint32_t others = (s.tiles + half) / 2u;
+      n_own += s.tiles - others;
+      n_other += others;
+      x += 1u + s.tiles;
+      if (live && others > 0)
+        live = __all_sync(0xffffffffu, attn_wait(&bar.s_full[half ^ 1u], (n_other - 1u) & 1u)) != 0;
+      if (live) live = prepare(nj + 1u, x);
+      if (live && some) live = fold_tile();
+      if (!live) break;
+      // the partial of this piece and half
+      const size_t id = 2u * (size_t)(s.unit + blockIdx.x) + half;
+      const uint32_t cap = s.prefix ? RT : p.seq_cap;
+      float* po = (s.prefix ? p.po : p.so) + id * cap * HD;
+      float* pml = (s.prefix ? p.pml : p.sml) + id * cap * kAttnMl;
+#pragma unroll
+      for (uint32_t y = 0; y < NC; ++y) {
+        if (y >= nact) break;  // warp-uniform
+        float2 ls = l[y];
+#pragma unroll
+        for (uint32_t o2 = 4; o2 < 32u; o2 <<= 1) {
+          ls.x += __shfl_xor_sync(0xffffffffu, ls.x, o2);
+          ls.y += __shfl_xor_sync(0xffffffffu, ls.y, o2);
+        }
+#pragma unroll
+        for (uint32_t z = 0; z < 2u; ++z) {
+          const uint32_t col = 8u * y + 2u * cq + z;
+          if (col >= s.rows) continue;
+          if (g == 0) {
+            pml[col * kAttnMl + 4u + quad] = z ? ls.y : ls.x;
+            if (quad == 0) pml[col * kAttnMl] = z ? m[y].y : m[y].x;
+          }
+          if (some && (HD >= 128u || quad * 32u < HD)) {
+#pragma unroll
+            for (uint32_t mh = 0; mh < MH; ++mh)
+#pragma unroll
+              for (uint32_t j = 0; j < 4u; ++j)
+                po[(size_t)col * HD + mh * 128u + quad * 32u + g + 8u * j] = z ? o[y][mh][j].y : o[y][mh][j].x;
+          }
+        }
+      }
+    }
+    if (!live) report(p.err, EOS_DEVERR_WAIT_ACT);
+  }
+  attn_fence_before();
+  __syncthreads();
+  if (warp == 9)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kTmem) : "memory");
+}
+
+// Joins a row's partials: one warp per (row, head), lane l holding HD / 32
+// neighbouring elements.  Weights are relative to the largest maximum; the
+// order of the sums is the line's, so results do not depend on timing.
+template <uint32_t HD>
+__global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) {
+  constexpr uint32_t E = HD / 32u, RT = kAttnRows;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint64_t x = (uint64_t)blockIdx.x * 2u + (threadIdx.x >> 5);
+  if (x >= (uint64_t)p.rows.n_rows * p.n_head) return;  // warp-uniform
+  const uint32_t hw = attn_div((uint32_t)x, p.by_group);  // row * n_kv_head + kv head
+  const uint32_t r = attn_div(hw, p.by_kv_head), g = hw - r * p.n_kv_head, hh = (uint32_t)x - hw * p.group;
+  const uint32_t h = g * p.group + hh;
+  const uint32_t i = kv_row_seq(p.rows, r);
+  if (i >= p.rows.n_seq) return;
+  pdl_wait();
+  const uint32_t t = r - kv_row_start(p.rows, i);
+  if (t >= p.max_rows) return;  // reported by the attention kernel
+  const uint32_t quantum = __ldcg(p.plan), tp = __ldcg(p.plan + 1), rgp = __ldcg(p.plan + 2), wp = __ldcg(p.plan + 3);
+  // ids of the row's partials: [first, last] of the prefix and of its sequence
+  struct Part {
+    const float *o, *ml;
+    uint32_t n, o_step, ml_step;
+  } part[2] = {};
+  auto set = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t w, uint32_t tiles,
+                 uint32_t row) {
+    if (tiles == 0) return;
+    const uint32_t c0 = (w + kAttnStart) / quantum, c1 = (w + kAttnStart + tiles - 1u) / quantum;
+    a.n = 2u * (c1 - c0 + 1u);  // two halves each
+    a.o_step = cap * HD;
+    a.ml_step = cap * kAttnMl;
+    a.o = o + ((size_t)2u * (unit + c0) * cap + row) * HD;
+    a.ml = ml + ((size_t)2u * (unit + c0) * cap + row) * kAttnMl;
+  };
+  {
+    const uint32_t fr = r * p.group + hh, rg = fr / RT, unit = g * rgp + rg;
+    set(part[0], p.po, p.pml, RT, unit, unit * attn_cost(tp), tp, fr % RT);
+  }
+  {
+    uint32_t len = p.seq_len[i];
+    len = len < p.max_len ? len : p.max_len;
+    const uint32_t fr = t * p.group + hh, rg = fr / RT, u = rg * p.n_kv_head + g, tiles = attn_ceil(len, kKvPage);
+    set(part[1], p.so, p.sml, p.seq_cap, i * p.seq_groups * p.n_kv_head + u, wp + __ldcg(p.plan + 4u + i) + u * attn_cost(tiles),
+        tiles, fr % RT);
+  }
+  // partial k of the row; lane k looks after its weight
+  const uint32_t n = part[0].n + part[1].n;
+  auto ml_of = [&](uint32_t k) {
+    return k < part[0].n ? part[0].ml + (size_t)k * part[0].ml_step
+                         : part[1].ml + (size_t)(k - part[0].n) * part[1].ml_step;
+  };
+  auto o_of = [&](uint32_t k) {
+    return (k < part[0].n ? part[0].o + (size_t)k * part[0].o_step
+                          : part[1].o + (size_t)(k - part[0].n) * part[1].o_step) + lane * E;
+  };
+  float top = -INFINITY;
+  for (uint32_t k = lane; k < n; k += 32u) top = fmaxf(top, __ldcg(ml_of(k)));
+#pragma unroll
+  for (uint32_t o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float mu = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f, acc[E];
+#pragma unroll
+  for (uint32_t e = 0; e < E; ++e) acc[e] = 0.0f;
+  for (uint32_t k0 = 0; k0 < n; k0 += 32u) {
+    float f = 0.0f, lk = 0.0f;
+    if (k0 + lane < n) {
+      const float4 ls = __ldcg(reinterpret_cast<const float4*>(ml_of(k0 + lane)) + 1);
+      lk = (ls.x + ls.y) + (ls.z + ls.w);
+      f = attn_ex2(__ldcg(ml_of(k0 + lane)) - mu);
+      if (lk == 0.0f) f = 0.0f;  // no tile, or no visible token: its output may be unwritten
+    }
+    float lw = f * lk;
+#pragma unroll
+    for (uint32_t o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
+    l += lw;
+    const uint32_t m = n - k0 < 32u ? n - k0 : 32u;
+    for (uint32_t b = 0; b < m; b += 8u) {  // eight partials' loads in flight
+      float v[8][E];
+#pragma unroll
+      for (uint32_t z = 0; z < 8u; ++z)
+        if (b + z < m) {
+          const float* src = o_of(k0 + b + z);
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) v[z][e] = __ldcg(src + e);
+        }
+#pragma unroll
+      for (uint32_t z = 0; z < 8u; ++z) {
+        const float w = __shfl_sync(0xffffffffu, f, b + z);
+        if (b + z < m && w != 0.0f)
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) acc[e] = fmaf(w, v[z][e], acc[e]);
+      }
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+  float* dst = p.out + (size_t)r * p.out_stride + (size_t)h * HD + lane * E;
+#pragma unroll
+  for (uint32_t e = 0; e < E; ++e) dst[e] = acc[e] * inv;
+}
+
+namespace {
+
+struct AttnScratch {
+  size_t plan, po, pml, so, sml, bytes;
+  uint32_t seq_cap, seq_groups;
+};
+AttnScratch attn_scratch(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
+  const uint32_t group = n_head / kv.n_kv_head, rt = kAttnRows;
+  AttnScratch s{};
+  auto put = [&](size_t bytes) {
+    const size_t at = s.bytes;
+    s.bytes += (bytes + 255u) & ~(size_t)255u;
+    return at;
+  };
+  s.plan = put(4u * ((size_t)b.n_seq + 5u));
+  const size_t np = b.max_prefix ? (size_t)kv.n_kv_head * (((size_t)b.n_rows * group + rt - 1u) / rt) + kAttnMaxCtas : 0u;
+  s.po = put(2u * np * rt * kv.head_dim * 4u);
+  s.pml = put(2u * np * rt * kAttnMl * 4u);
+  const size_t most = (size_t)b.max_rows * group;
+  s.seq_cap = most < rt ? (uint32_t)most : rt;
+  s.seq_groups = (uint32_t)((most + rt - 1u) / rt);
+  const size_t ns = b.max_len ? (size_t)b.n_seq * s.seq_groups * kv.n_kv_head + kAttnMaxCtas : 0u;
+  s.so = put(2u * ns * s.seq_cap * kv.head_dim * 4u);
+  s.sml = put(2u * ns * s.seq_cap * kAttnMl * 4u);
+  return s;
+}
+
+template <uint32_t HD>
+cudaError_t attn_launch(const KvAttnParams& p, int num_sms, uint64_t work, cudaStream_t st) {
+  using G = AttnGeo<HD>;
+  static SmemAttr attr;
+  const uint32_t smem = G::smem(p.rows.n_seq);
+  cudaError_t e = ensure_smem_attr((const void*)kv_attn_kernel<HD>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
+  if (e != cudaSuccess) return e;
+  uint64_t grid = (uint64_t)G::kCtas * (uint32_t)num_sms;
+  if (grid > kAttnMaxCtas) grid = kAttnMaxCtas;
+  if (grid > work) grid = work;
+  if (grid == 0) grid = 1;
+  kv_attn_kernel<HD><<<(uint32_t)grid, kAttnThreads, smem, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((uint32_t)(((uint64_t)p.rows.n_rows * p.n_head + 1u) / 2u));
+  cfg.blockDim = dim3(64);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<HD>, p);
+}
+
+}  // namespace
+
+size_t kv_attn_scratch_bytes(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
+  return attn_scratch(kv, b, n_head).bytes;
+}
+
+// The line of tiles of the largest lengths (its words are 32-bit).
+uint64_t kv_attn_work_bound(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
+  const uint32_t group = n_head / kv.n_kv_head, rt = kAttnRows;
+  const uint64_t tp = (b.max_prefix + kKvPage - 1u) / kKvPage, ts = (b.max_len + kKvPage - 1u) / kKvPage;
+  const uint64_t rp = ((uint64_t)b.n_rows * group + rt - 1u) / rt;
+  uint64_t rs = (uint64_t)b.n_seq * (((uint64_t)b.max_rows * group + rt - 1u) / rt);
+  const uint64_t by_rows = rp + b.n_seq;  // sequences share n_rows
+  if (rs > by_rows) rs = by_rows;
+  return kv.n_kv_head * (rp * (tp + kAttnStart) + rs * (ts + kAttnStart));
+}
 
 cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* q, uint64_t q_stride, float* out,
-                           uint64_t out_stride, uint32_t n_head, float scale, void*, uint32_t* err,
-                           cudaStream_t st) {
+                           uint64_t out_stride, uint32_t n_head, float scale, void* scratch, int num_sms,
+                           uint32_t* err, cudaStream_t st) {
   if (b.n_rows == 0 || b.n_seq == 0) return cudaSuccess;
+  const AttnScratch s = attn_scratch(kv, b, n_head);
+  uint8_t* ws = static_cast<uint8_t*>(scratch);
   KvAttnParams p{};
   p.rows = KvRows{b.row0, b.n_seq, b.n_rows, b.row0 ? 0u : b.n_rows / b.n_seq};
   p.pages = kv.pages;
@@ -122,20 +1088,30 @@ cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* 
   p.max_prefix = b.max_prefix;
   p.table_stride = b.table_stride;
   p.max_len = b.max_len;
+  p.max_rows = b.max_rows;
   p.n_pages = kv.n_pages;
   p.n_head = n_head;
   p.n_kv_head = kv.n_kv_head;
+  p.group = n_head / kv.n_kv_head;
+  p.by_group = attn_divisor(p.group);
+  p.by_kv_head = attn_divisor(kv.n_kv_head);
   p.q = q;
   p.out = out;
   p.q_stride = q_stride;
   p.out_stride = out_stride;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.plan = reinterpret_cast<uint32_t*>(ws + s.plan);
+  p.po = reinterpret_cast<float*>(ws + s.po);
+  p.pml = reinterpret_cast<float*>(ws + s.pml);
+  p.so = reinterpret_cast<float*>(ws + s.so);
+  p.sml = reinterpret_cast<float*>(ws + s.sml);
+  p.seq_cap = s.seq_cap;
+  p.seq_groups = s.seq_groups;
   p.err = err;
-  const dim3 grid(b.n_rows, n_head);
-  if (kv.head_dim == 64) kv_attn_simple_kernel<64><<<grid, 128, 0, st>>>(p);
-  else if (kv.head_dim == 128) kv_attn_simple_kernel<128><<<grid, 128, 0, st>>>(p);
-  else kv_attn_simple_kernel<256><<<grid, 128, 0, st>>>(p);
-  return cudaGetLastError();
+  const uint64_t work = kv_attn_work_bound(kv, b, n_head);
+  if (kv.head_dim == 64) return attn_launch<64>(p, num_sms, work, st);
+  if (kv.head_dim == 128) return attn_launch<128>(p, num_sms, work, st);
+  return attn_launch<256>(p, num_sms, work, st);
 }
 
 }  // namespace eos

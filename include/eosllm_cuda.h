@@ -236,7 +236,7 @@ EOSLLM_CUDA_API int eosi_cuda_q4_k_prefill_dev(const float *a, const void *w_pre
  * eosi_cuda_kv_q8_page_bytes(n_kv_head, head_dim) bytes, one after the other,
  * 16-byte aligned; contents are opaque and need no initialisation.  One row
  * (the head_dim elements x of one token and kv head, keys and values apart) is
- * held as int8 q and one f32 scale: scale = max|x| / 127 in f32, q_i = the
+ * held as int8 q and one f32 scale: scale = max|x| * (1 / 127) in f32, q_i = the
  * integer nearest to 127 x_i / max|x| (ties to even, decided on the exact
  * quotient), its value q_i * scale in f32; a row that holds a NaN or an
  * infinity reads back as NaN.  head_dim is 64, 128 or 256 (EOS_E_UNSUPPORTED

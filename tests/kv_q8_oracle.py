@@ -11,7 +11,7 @@ def stored(x):
     x = np.asarray(x, np.float32)
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         a = np.max(np.abs(x), axis=-1, keepdims=True)
-        scale = (a / np.float32(127.0)).astype(np.float32)
+        scale = (a * (np.float32(1.0) / np.float32(127.0))).astype(np.float32)
         den = np.where(a > 0, a, 1).astype(np.float64)
         q = np.rint(127.0 * x.astype(np.float64) / den)
         q = np.where(np.isfinite(a), q, 0.0)

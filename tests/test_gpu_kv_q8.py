@@ -271,6 +271,14 @@ def test_extreme_scales(gpu, hd):
     Batch(gpu, 4, 2, hd, 260, [140, 10], [2, 2], seed=8, edit=edit).check()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1e-20, 3.0])
+def test_softmax_scales(gpu, scale):
+    """Scale 0 averages the visible values; a negative one turns the order."""
+    def edit(b):
+        b.scale = scale
+    Batch(gpu, 4, 2, 128, 140, [20, 3], [3, 1], seed=17, q_gain=0.5, edit=edit).check()
+
+
 def test_nan_and_infinity_reach_only_rows_that_see_them(gpu):
     def edit(b):
         b.ks[0][3, 0, 5] = np.nan      # seen by every row of sequence 0's heads 0, 1

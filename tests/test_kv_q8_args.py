@@ -61,14 +61,15 @@ def test_attention_refusals(cuda_lib, buf):
     base = dict(table=a, table_stride=2, seq_len=a, max_len=256, n_seq=2, n_rows=4, max_rows=2, row0=a, prefix_table=a,
                 prefix_len=a, max_prefix=100)
 
-    def st(p=None, n_head=4, q=a, qs=512, out=a, os_=512, scratch=a, nbytes=1 << 40, **kw):
+    def st(p=None, n_head=4, q=a, qs=512, out=a, os_=512, scratch=a, nbytes=1 << 40, scale=0.1, **kw):
         p = pool(buf) if p is None else p
         b = B.attn_batch(**{**base, **kw})
-        return cuda_lib.eosi_cuda_kv_q8_attn_dev(C.byref(p), C.byref(b), q, qs, out, os_, n_head, 0.1, scratch, nbytes,
+        return cuda_lib.eosi_cuda_kv_q8_attn_dev(C.byref(p), C.byref(b), q, qs, out, os_, n_head, scale, scratch, nbytes,
                                                  None)
 
     assert st(n_head=3) == B.EOS_E_INVALID_ARG         # not a multiple of the 2 kv heads
     assert st(n_head=0) == B.EOS_E_INVALID_ARG
+    assert st(scale=float("nan")) == B.EOS_E_INVALID_ARG and st(scale=float("inf")) == B.EOS_E_INVALID_ARG
     assert st(qs=508) == B.EOS_E_INVALID_ARG and st(qs=514) == B.EOS_E_INVALID_ARG and st(os_=508) == B.EOS_E_INVALID_ARG
     for kw in (dict(q=None), dict(out=None), dict(scratch=None), dict(seq_len=None), dict(table=None),
                dict(prefix_table=None), dict(prefix_len=None)):
