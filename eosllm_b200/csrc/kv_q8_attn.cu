@@ -86,7 +86,10 @@ struct KvAttnParams {
   uint32_t* plan;    // quantum, prefix tiles, prefix row groups, prefix work, then the sequences' running work
   float *po, *pml;   // prefix partials: [unit + CTA][half][row][HD], [unit + CTA][half][row][kAttnMl]
   float *so, *sml;   // the sequences' partials, with seq_cap rows
-  uint32_t seq_cap, seq_groups;  // rows of a sequence partial; row groups reserved per sequence
+  uint32_t prefix_cap, seq_cap;  // rows of a partial
+  uint32_t seq_groups;           // row groups reserved per sequence
+  // pages per CTA where the few-rows kernel has the prefix (the sequences), else 0: the line has them
+  uint32_t prefix_run, prefix_runs, seq_run, seq_runs;
   uint32_t* err;
 };
 
@@ -290,6 +293,315 @@ __device__ __forceinline__ void attn_digits(const uint32_t* b, uint32_t* w) {
   w[2] = __byte_perm(__byte_perm(b[0], b[1], 0x0062), __byte_perm(b[2], b[3], 0x0062), 0x5410);
 }
 
+// A query row as integers: scale maps score integers (in units of 256) to log2
+// scores; a negative softmax scale turns the integers' sign, so larger products
+// are larger scores.
+struct AttnQScale {
+  float inv, scale;
+  bool finite;
+};
+__device__ __forceinline__ uint32_t attn_absmax(uint32_t amax, float4 v) {
+  amax = max(max(amax, __float_as_uint(v.x) & 0x7fffffffu), __float_as_uint(v.y) & 0x7fffffffu);
+  return max(max(amax, __float_as_uint(v.z) & 0x7fffffffu), __float_as_uint(v.w) & 0x7fffffffu);
+}
+__device__ __forceinline__ AttnQScale attn_query_scale(uint32_t amax, float scale_log2) {
+  AttnQScale s;
+  s.finite = amax < 0x7f800000u;
+  const float top = fmaxf(__uint_as_float(amax), 1e-30f);
+  s.inv = s.finite ? __fdiv_rn(scale_log2 < 0.0f ? -kAttnQMax : kAttnQMax, top) : 0.0f;
+  // (above 0, so that a hidden token's -infinity stays one when the softmax scale is 0)
+  s.scale = s.finite ? fmaxf(__fdiv_rn(top, kAttnQMax) * (256.0f * fabsf(scale_log2)), 1e-37f) : NAN;
+  return s;
+}
+// Three balanced digits of four elements: bytes of (x + 0x808080) ^ 0x808080.
+__device__ __forceinline__ void attn_query_digits(float4 v, const AttnQScale& s, uint32_t* d) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  uint32_t b[4];
+#pragma unroll
+  for (uint32_t e = 0; e < 4u; ++e)
+    b[e] = (uint32_t)((s.finite ? __float2int_rn(f[e] * s.inv) : 0) + 0x808080) ^ 0x808080u;
+  attn_digits(b, d);
+}
+__device__ __forceinline__ float attn_warp_max(float x) {
+#pragma unroll
+  for (uint32_t b = 16; b > 0; b >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
+  return x;
+}
+
+// ---- few rows: integer dot products on the CUDA cores -------------------------
+// Up to kFewRows rows (query rows times heads of the kv head) against the pages
+// [first, first + pages_per_cta) of a unit, one CTA of 128 threads per (unit,
+// run of pages).  Reading the cache is what bounds it: 2 HD + 8 bytes per token
+// against 6 HD / 4 dp4a per token and row, so up to four rows stay below the
+// memory's time.  No barrier or tensor memory to set up and several CTAs per
+// SM, each with a page's loads in flight: units of a page or two (a
+// sequence's own tokens, a decode step) take one round trip to memory.
+// Same digits and sums as the tensor-core kernel: s32 sums over 16 dimensions
+// (scores) and over a page (values) are exact.
+constexpr uint32_t kFewRows = 4;
+constexpr uint32_t kFewThreads = 128;
+
+__device__ __forceinline__ int32_t attn_dp4a_su(uint32_t a, uint32_t b, int32_t c) {  // s8 x u8
+  int32_t d;
+  asm("dp4a.s32.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint4 attn_ld_stream(const void* src) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(src));
+  return v;
+}
+
+// Grid (pages / pages_per_cta, kv heads, sequences); prefix: one "sequence" of
+// all rows.
+template <uint32_t HD, uint32_t R>
+__global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnParams p, uint32_t prefix,
+                                                                  uint32_t pages_per_cta) {
+  constexpr uint32_t CL = HD / 16u;                    // 16-byte chunks of a key row = lanes per token
+  constexpr uint32_t DT = HD <= 128u ? 1u : HD / 128u; // dimensions per thread
+  constexpr uint32_t QT = HD == 64u ? 2u : 4u;         // quarters of the values per thread
+  __shared__ __align__(16) uint32_t qd[R][3][HD / 4u]; // query digits
+  __shared__ float qscale[R];
+  __shared__ __align__(16) uint8_t pd[R][3][kKvPage];  // probability digits by position
+  __shared__ float red[2][4][R + 1u];                  // per warp: maxima, largest value scale
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t g = blockIdx.y;
+  AttnSeq s{0, 0, 0};
+  const uint32_t* table = p.prefix_table;
+  if (prefix) {
+    s.len = p.prefix_len != nullptr ? *p.prefix_len : 0u;
+    s.n = kv_row_start(p.rows, p.rows.n_seq);
+    if (s.len > p.max_prefix) {
+      s.len = p.max_prefix;
+      if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
+    }
+  } else {
+    s = attn_seq(p, blockIdx.z);
+    table = p.table + (size_t)blockIdx.z * p.table_stride;
+    if (blockIdx.x == 0 && tid == 0 && (p.seq_len[blockIdx.z] > p.max_len || s.n > p.max_rows))
+      report(p.err, EOS_DEVERR_RANGE);
+  }
+  const uint32_t first = blockIdx.x * pages_per_cta;
+  const uint32_t pages = attn_ceil(s.len, kKvPage);
+  uint32_t rows = (prefix || s.n < p.max_rows ? s.n : p.max_rows) * p.group;
+  if (rows > R) rows = R;  // (the host chose R >= rows)
+  pdl_trigger();
+  if (first >= pages || rows == 0) return;  // the joining kernel knows which runs exist
+  const uint32_t last = first + pages_per_cta < pages ? first + pages_per_cta : pages;
+  const int32_t seen0 = (int32_t)s.len - (int32_t)s.n + 1;  // tokens a sequence's first row sees (may be negative)
+  // warp r: row r's digits
+  if (warp < R) {
+    float scale = 0.0f;
+    constexpr uint32_t QF = HD <= 128u ? 1u : HD / 128u;
+    uint32_t d[QF][3];
+#pragma unroll
+    for (uint32_t c = 0; c < QF; ++c) d[c][0] = d[c][1] = d[c][2] = 0u;
+    if (warp < rows) {
+      const uint32_t xr = attn_div(warp, p.by_group);
+      const float* src = p.q + (size_t)(s.r0 + xr) * p.q_stride + (size_t)(g * p.group + warp - xr * p.group) * HD;
+      float4 v[QF];
+      uint32_t amax = 0;
+#pragma unroll
+      for (uint32_t c = 0; c < QF; ++c) {
+        v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (HD >= 128u || lane < HD / 4u) v[c] = *reinterpret_cast<const float4*>(src + c * 128u + lane * 4u);
+        amax = attn_absmax(amax, v[c]);
+      }
+      amax = __reduce_max_sync(0xffffffffu, amax);
+      const AttnQScale qsc = attn_query_scale(amax, p.scale_log2);
+      scale = qsc.scale;
+#pragma unroll
+      for (uint32_t c = 0; c < QF; ++c) attn_query_digits(v[c], qsc, d[c]);
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < QF; ++c)
+      if (HD >= 128u || lane < HD / 4u)
+#pragma unroll
+        for (uint32_t e = 0; e < 3u; ++e) qd[warp][e][c * 32u + lane] = d[c][e];
+    if (lane == 0) qscale[warp] = scale;
+  }
+  __syncthreads();
+  // score side: lane's chunk of the key rows, tokens 32 warp + i (32 / CL) + lane / CL
+  const uint32_t lc = lane % CL, lt = lane / CL;
+  uint32_t qw[R][3][4];
+  float qsc[R];
+#pragma unroll
+  for (uint32_t r = 0; r < R; ++r) {
+    qsc[r] = qscale[r];
+#pragma unroll
+    for (uint32_t e = 0; e < 3u; ++e) {
+      const uint4 v = *reinterpret_cast<const uint4*>(&qd[r][e][lc * 4u]);
+      qw[r][e][0] = v.x;
+      qw[r][e][1] = v.y;
+      qw[r][e][2] = v.z;
+      qw[r][e][3] = v.w;
+    }
+  }
+  // after the reduction over the CL lanes of a token, this lane holds token `own`
+  const uint32_t own = warp * 32u + lc * (32u / CL) + lt;
+  // value side: this thread's dimension(s) and quarters
+  const uint32_t dim0 = HD == 64u ? (tid & 63u) : tid, q0 = HD == 64u ? (tid >> 6) * 2u : 0u;
+  float o[R][DT], m[R], l[R];
+#pragma unroll
+  for (uint32_t r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d) o[r][d] = 0.0f;
+  }
+  for (uint32_t pg = first; pg < last; ++pg) {
+    const uint32_t page = table[pg];
+    if (page >= p.n_pages) {  // hidden
+      if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
+      continue;
+    }
+    const uint8_t* blk = p.pages + ((size_t)page * p.n_kv_head + g) * kv_block_bytes(HD);
+    const uint32_t avail = s.len - pg * kKvPage;  // tokens (may exceed a page)
+    uint4 kw[CL], vw[DT][QT][2];
+#pragma unroll
+    for (uint32_t i = 0; i < CL; ++i) {
+      const uint32_t t = warp * 32u + i * (32u / CL) + lt;
+      kw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (t < avail) kw[i] = attn_ld_stream(blk + kv_k_offset<HD>(t, lc * 16u));
+    }
+    float ks = 0.0f, vs = 0.0f;
+    if (own < avail) {
+      ks = __ldg(reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(own, 0)));
+      vs = __ldg(reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(own, 1)));
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+      for (uint32_t q = 0; q < QT; ++q)
+#pragma unroll
+        for (uint32_t c = 0; c < 2u; ++c) {
+          const uint32_t dim = dim0 + d * 128u;
+          vw[d][q][c] = make_uint4(0u, 0u, 0u, 0u);
+          if ((q0 + q) * kKvQuarter < avail)
+            vw[d][q][c] = attn_ld_stream(blk + kKvPage * HD + (q0 + q) * (HD * kKvQuarter) + dim * 32u +
+                                         ((c ^ (dim >> 2)) & 1u) * 16u);
+        }
+    if (!(vs < INFINITY)) {  // a NaN or infinite value row: NaN score
+      ks = NAN;
+      vs = 0.0f;
+    }
+    // scores
+    float z[R];
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      float part[CL];
+#pragma unroll
+      for (uint32_t i = 0; i < CL; ++i) {
+        int32_t a[3];
+#pragma unroll
+        for (uint32_t e = 0; e < 3u; ++e) {
+          a[e] = __dp4a((int)kw[i].x, (int)qw[r][e][0], 0);
+          a[e] = __dp4a((int)kw[i].y, (int)qw[r][e][1], a[e]);
+          a[e] = __dp4a((int)kw[i].z, (int)qw[r][e][2], a[e]);
+          a[e] = __dp4a((int)kw[i].w, (int)qw[r][e][3], a[e]);
+        }
+        // below 2^18 each: (a2 2^8 + a1) is exact in s32; a0 / 256 joins as a float
+        part[i] = fmaf((float)a[0], 1.0f / 256.0f, (float)(a[2] * 256 + a[1]));
+      }
+      // sums over the token's lanes, each lane ending with one token
+#pragma unroll
+      for (uint32_t b = CL / 2u; b > 0; b >>= 1) {
+        const bool up = (lane & b) != 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < CL; ++i) {
+          if (i >= b) break;
+          const float give = up ? part[i] : part[i + b], keep = up ? part[i + b] : part[i];
+          part[i] = keep + __shfl_xor_sync(0xffffffffu, give, b);
+        }
+      }
+      const int32_t seen = prefix ? (int32_t)s.len : seen0 + (int32_t)attn_div(r, p.by_group);
+      const int32_t tok = (int32_t)(pg * kKvPage + own);
+      z[r] = own < avail && tok < seen ? part[0] * ks : -INFINITY;
+      const float mx = attn_warp_max(z[r]);
+      if (lane == 0) red[pg & 1u][warp][r] = mx;
+    }
+    {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs));
+      if (lane == 0) red[pg & 1u][warp][R] = __uint_as_float(top);
+    }
+    __syncthreads();
+    const float(*rd)[R + 1u] = red[pg & 1u];
+    uint32_t top = __float_as_uint(fmaxf(fmaxf(rd[0][R], rd[1][R]), fmaxf(rd[2][R], rd[3][R]))) >> 23;
+    top = top < 23u ? 23u : top;
+    const float up = __uint_as_float((276u - top) << 23), unit = __uint_as_float((top - 22u) << 23);
+    float f[R];
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      const float mt = fmaxf(fmaxf(rd[0][r], rd[1][r]), fmaxf(rd[2][r], rd[3][r]));
+      const float nm = fmaxf(mt == -INFINITY ? mt : __fmul_ru(mt, qsc[r]), m[r]);
+      const float neg = nm == -INFINITY ? 0.0f : -nm;
+      f[r] = attn_ex2(m[r] + neg);
+      m[r] = nm;
+      const float e = attn_ex2(fmaf(z[r], qsc[r], neg));
+      l[r] = fmaf(l[r], f[r], e);  // this token's share
+      const uint32_t w = __float_as_uint(fmaf(e, vs * up, 8388608.0f));
+      uint8_t* at = &pd[r][0][warp * 32u + kv_v_position(own)];
+      at[0] = (uint8_t)w;
+      at[kKvPage] = (uint8_t)(w >> 8);
+      at[2u * kKvPage] = (uint8_t)(w >> 16);
+    }
+    __syncthreads();
+    // values
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      int32_t a[DT][3];
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d) a[d][0] = a[d][1] = a[d][2] = 0;
+#pragma unroll
+      for (uint32_t e = 0; e < 3u; ++e)
+#pragma unroll
+        for (uint32_t q = 0; q < QT; ++q)
+#pragma unroll
+          for (uint32_t c = 0; c < 2u; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(&pd[r][e][(q0 + q) * kKvQuarter + c * 16u]);
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d) {
+              a[d][e] = attn_dp4a_su(vw[d][q][c].x, w.x, a[d][e]);
+              a[d][e] = attn_dp4a_su(vw[d][q][c].y, w.y, a[d][e]);
+              a[d][e] = attn_dp4a_su(vw[d][q][c].z, w.z, a[d][e]);
+              a[d][e] = attn_dp4a_su(vw[d][q][c].w, w.w, a[d][e]);
+            }
+          }
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d) {
+        const float v = fmaf((float)a[d][2], 65536.0f, fmaf((float)a[d][1], 256.0f, (float)a[d][0]));
+        o[r][d] = fmaf(v, unit, o[r][d] * f[r]);
+      }
+    }
+    // (the next page's red[] is the other buffer, and its pd[] follows a barrier that every warp reaches after these reads)
+  }
+  // partial: all l shares, one maximum, the outputs
+  const uint32_t cap = prefix ? p.prefix_cap : p.seq_cap;
+  const size_t id = ((size_t)(prefix ? 0u : blockIdx.z) * p.n_kv_head + g) * gridDim.x + blockIdx.x;
+  float* po = (prefix ? p.po : p.so) + id * cap * HD;
+  float* pml = (prefix ? p.pml : p.sml) + id * cap * kAttnMl;
+#pragma unroll
+  for (uint32_t r = 0; r < R; ++r) {
+    float ls = l[r];
+#pragma unroll
+    for (uint32_t b = 16; b > 0; b >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, b);
+    if (r >= rows) continue;
+    if (lane == 0) pml[r * kAttnMl + 4u + warp] = ls;
+    if (tid == 0) pml[r * kAttnMl] = m[r];
+    if constexpr (HD == 64) {  // two threads hold the halves of a dimension's sum
+      __shared__ float oh[R][64];
+      if (tid >= 64u) oh[r][tid & 63u] = o[r][0];
+      __syncthreads();
+      if (tid < 64u) po[(size_t)r * HD + tid] = o[r][0] + oh[r][tid];
+    } else {
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d) po[(size_t)r * HD + d * 128u + tid] = o[r][d];
+    }
+  }
+}
+
 // mbar_wait, reading the clock only once in 64 polls: its read takes longer
 // than a tile's waits.
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity) {
@@ -410,7 +722,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     for (uint32_t i0 = 0; i0 < p.rows.n_seq; i0 += 32u) {
       uint32_t w = 0;
       const bool in = i0 + lane < p.rows.n_seq;
-      if (in) w = attn_seq_work(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
+      if (in && p.seq_run == 0) w = attn_seq_work(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
       uint32_t c = w;
 #pragma unroll
       for (uint32_t o = 1; o < 32u; o <<= 1) {
@@ -423,6 +735,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     if (lane == 0) cum[p.rows.n_seq] = carry;
     __syncwarp();
     pl.prefix = prefix_len < p.max_prefix ? prefix_len : p.max_prefix;
+    if (p.prefix_run > 0) pl.prefix = 0;
     pl.rows_p = rows_end;
     pl.tp = attn_ceil(pl.prefix, kKvPage);
     pl.rgp = attn_ceil(pl.rows_p * p.group, RT);
@@ -630,24 +943,15 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
             for (uint32_t pn = 0; pn < G::kPanels; ++pn) {
               v[pn] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               if (HD >= 128u || lane < HD / 4u) v[pn] = *reinterpret_cast<const float4*>(raw + r * HD + pn * 128u + lane * 4u);
-              amax = max(max(amax, __float_as_uint(v[pn].x) & 0x7fffffffu), __float_as_uint(v[pn].y) & 0x7fffffffu);
-              amax = max(max(amax, __float_as_uint(v[pn].z) & 0x7fffffffu), __float_as_uint(v[pn].w) & 0x7fffffffu);
+              amax = attn_absmax(amax, v[pn]);
             }
             amax = __reduce_max_sync(0xffffffffu, amax);
-            const bool finite = amax < 0x7f800000u;
-            const float top = fmaxf(__uint_as_float(amax), 1e-30f);
-            // a negative scale turns the integers' sign: larger products are larger scores
-            const float inv = finite ? __fdiv_rn(p.scale_log2 < 0.0f ? -kAttnQMax : kAttnQMax, top) : 0.0f;
-            // (above 0, so that a hidden token's -infinity stays one when the softmax scale is 0)
-            scale = finite ? fmaxf(__fdiv_rn(top, kAttnQMax) * (256.0f * fabsf(p.scale_log2)), 1e-37f) : NAN;
+            const AttnQScale q = attn_query_scale(amax, p.scale_log2);
+            scale = q.scale;
 #pragma unroll
             for (uint32_t pn = 0; pn < G::kPanels; ++pn) {
-              const float f[4] = {v[pn].x, v[pn].y, v[pn].z, v[pn].w};
-              uint32_t b[4], d[3];
-#pragma unroll
-              for (uint32_t e = 0; e < 4u; ++e)  // balanced digits: bytes of (x + 0x808080) ^ 0x808080
-                b[e] = (uint32_t)((finite ? __float2int_rn(f[e] * inv) : 0) + 0x808080) ^ 0x808080u;
-              attn_digits(b, d);
+              uint32_t d[3];
+              attn_query_digits(v[pn], q, d);
               if (HD >= 128u || lane < HD / 4u) {
 #pragma unroll
                 for (uint32_t e = 0; e < 3u; ++e) {
@@ -865,7 +1169,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
       if (!live) break;
       // the partial of this piece and half
       const size_t id = 2u * (size_t)(s.unit + blockIdx.x) + half;
-      const uint32_t cap = s.prefix ? RT : p.seq_cap;
+      const uint32_t cap = s.prefix ? p.prefix_cap : p.seq_cap;
       float* po = (s.prefix ? p.po : p.so) + id * cap * HD;
       float* pml = (s.prefix ? p.pml : p.sml) + id * cap * kAttnMl;
 #pragma unroll
@@ -920,32 +1224,52 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
   pdl_wait();
   const uint32_t t = r - kv_row_start(p.rows, i);
   if (t >= p.max_rows) return;  // reported by the attention kernel
-  const uint32_t quantum = __ldcg(p.plan), tp = __ldcg(p.plan + 1), rgp = __ldcg(p.plan + 2), wp = __ldcg(p.plan + 3);
   // ids of the row's partials: [first, last] of the prefix and of its sequence
   struct Part {
     const float *o, *ml;
     uint32_t n, o_step, ml_step;
   } part[2] = {};
-  auto set = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t w, uint32_t tiles,
-                 uint32_t row) {
+  // on the line: the CTAs that hold tiles of the unit, two halves each
+  auto line = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t w, uint32_t tiles,
+                  uint32_t row) {
     if (tiles == 0) return;
+    const uint32_t quantum = __ldcg(p.plan);
     const uint32_t c0 = (w + kAttnStart) / quantum, c1 = (w + kAttnStart + tiles - 1u) / quantum;
-    a.n = 2u * (c1 - c0 + 1u);  // two halves each
+    a.n = 2u * (c1 - c0 + 1u);
     a.o_step = cap * HD;
     a.ml_step = cap * kAttnMl;
     a.o = o + ((size_t)2u * (unit + c0) * cap + row) * HD;
     a.ml = ml + ((size_t)2u * (unit + c0) * cap + row) * kAttnMl;
   };
-  {
-    const uint32_t fr = r * p.group + hh, rg = fr / RT, unit = g * rgp + rg;
-    set(part[0], p.po, p.pml, RT, unit, unit * attn_cost(tp), tp, fr % RT);
+  // runs of pages of the few-rows kernel
+  auto runs = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t per_unit,
+                  uint32_t run, uint32_t tiles, uint32_t row) {
+    a.n = attn_ceil(tiles, run);
+    a.o_step = cap * HD;
+    a.ml_step = cap * kAttnMl;
+    a.o = o + ((size_t)unit * per_unit * cap + row) * HD;
+    a.ml = ml + ((size_t)unit * per_unit * cap + row) * kAttnMl;
+  };
+  if (p.max_prefix > 0) {
+    const uint32_t fr = r * p.group + hh;
+    if (p.prefix_run > 0) {
+      const uint32_t len = *p.prefix_len < p.max_prefix ? *p.prefix_len : p.max_prefix;
+      runs(part[0], p.po, p.pml, p.prefix_cap, g, p.prefix_runs, p.prefix_run, attn_ceil(len, kKvPage), fr);
+    } else {
+      const uint32_t tp = __ldcg(p.plan + 1), rgp = __ldcg(p.plan + 2), rg = fr / RT, unit = g * rgp + rg;
+      line(part[0], p.po, p.pml, p.prefix_cap, unit, unit * attn_cost(tp), tp, fr % RT);
+    }
   }
   {
-    uint32_t len = p.seq_len[i];
-    len = len < p.max_len ? len : p.max_len;
-    const uint32_t fr = t * p.group + hh, rg = fr / RT, u = rg * p.n_kv_head + g, tiles = attn_ceil(len, kKvPage);
-    set(part[1], p.so, p.sml, p.seq_cap, i * p.seq_groups * p.n_kv_head + u, wp + __ldcg(p.plan + 4u + i) + u * attn_cost(tiles),
-        tiles, fr % RT);
+    const uint32_t len = p.seq_len[i] < p.max_len ? p.seq_len[i] : p.max_len;
+    const uint32_t fr = t * p.group + hh, tiles = attn_ceil(len, kKvPage);
+    if (p.seq_run > 0) {
+      runs(part[1], p.so, p.sml, p.seq_cap, i * p.n_kv_head + g, p.seq_runs, p.seq_run, tiles, fr);
+    } else {
+      const uint32_t rg = fr / RT, u = rg * p.n_kv_head + g;
+      line(part[1], p.so, p.sml, p.seq_cap, i * p.seq_groups * p.n_kv_head + u,
+           __ldcg(p.plan + 3) + __ldcg(p.plan + 4u + i) + u * attn_cost(tiles), tiles, fr % RT);
+    }
   }
   // partial k of the row; lane k looks after its weight
   const uint32_t n = part[0].n + part[1].n;
@@ -1004,43 +1328,90 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
 
 namespace {
 
-struct AttnScratch {
+// How a call runs: the prefix and the sequences each on the tensor cores' line
+// or, with at most kFewRows rows to a unit, in runs of pages (see the two
+// kernels); and where their partials sit.
+struct AttnSplit {
   size_t plan, po, pml, so, sml, bytes;
-  uint32_t seq_cap, seq_groups;
+  uint32_t prefix_cap, seq_cap, seq_groups;
+  uint32_t prefix_run, prefix_runs, seq_run, seq_runs;
+  bool line;
 };
-AttnScratch attn_scratch(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
+// Pages per CTA of `units` units of up to `pages` pages: enough CTAs for the
+// machine (about eight per SM), at most 8 pages so that a row has few partials
+// to join next to what it reads.
+uint32_t attn_run(uint64_t units, uint64_t pages) {
+  const uint64_t want = units * pages / 1184u;
+  return want < 1u ? 1u : (want > 8u ? 8u : (uint32_t)want);
+}
+AttnSplit attn_split(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
   const uint32_t group = n_head / kv.n_kv_head, rt = kAttnRows;
-  AttnScratch s{};
-  auto put = [&](size_t bytes) {
-    const size_t at = s.bytes;
-    s.bytes += (bytes + 255u) & ~(size_t)255u;
-    return at;
+  AttnSplit s{};
+  auto put = [&](uint64_t parts, uint32_t cap, size_t& o, size_t& ml) {
+    o = s.bytes;
+    s.bytes += (parts * cap * kv.head_dim * 4u + 255u) & ~(size_t)255u;
+    ml = s.bytes;
+    s.bytes += (parts * cap * kAttnMl * 4u + 255u) & ~(size_t)255u;
   };
-  s.plan = put(4u * ((size_t)b.n_seq + 5u));
-  const size_t np = b.max_prefix ? (size_t)kv.n_kv_head * (((size_t)b.n_rows * group + rt - 1u) / rt) + kAttnMaxCtas : 0u;
-  s.po = put(2u * np * rt * kv.head_dim * 4u);
-  s.pml = put(2u * np * rt * kAttnMl * 4u);
-  const size_t most = (size_t)b.max_rows * group;
-  s.seq_cap = most < rt ? (uint32_t)most : rt;
-  s.seq_groups = (uint32_t)((most + rt - 1u) / rt);
-  const size_t ns = b.max_len ? (size_t)b.n_seq * s.seq_groups * kv.n_kv_head + kAttnMaxCtas : 0u;
-  s.so = put(2u * ns * s.seq_cap * kv.head_dim * 4u);
-  s.sml = put(2u * ns * s.seq_cap * kAttnMl * 4u);
+  s.plan = 0;
+  s.bytes = (4u * ((size_t)b.n_seq + 5u) + 255u) & ~(size_t)255u;
+  const uint64_t rows = (uint64_t)b.n_rows * group, per_seq = (uint64_t)b.max_rows * group;
+  if (b.max_prefix > 0) {
+    const uint32_t pages = attn_ceil(b.max_prefix, kKvPage);
+    s.prefix_cap = rows < rt ? (uint32_t)rows : rt;
+    if (rows <= kFewRows) {
+      s.prefix_run = attn_run(kv.n_kv_head, pages);
+      s.prefix_runs = attn_ceil(pages, s.prefix_run);
+      put((uint64_t)kv.n_kv_head * s.prefix_runs, s.prefix_cap, s.po, s.pml);
+    } else {
+      s.line = true;
+      put(2u * ((uint64_t)kv.n_kv_head * ((rows + rt - 1u) / rt) + kAttnMaxCtas), s.prefix_cap, s.po, s.pml);
+    }
+  }
+  if (b.max_len > 0) {
+    const uint32_t pages = attn_ceil(b.max_len, kKvPage);
+    s.seq_cap = per_seq < rt ? (uint32_t)per_seq : rt;
+    s.seq_groups = (uint32_t)((per_seq + rt - 1u) / rt);
+    if (per_seq <= kFewRows) {
+      s.seq_run = attn_run((uint64_t)b.n_seq * kv.n_kv_head, pages);
+      s.seq_runs = attn_ceil(pages, s.seq_run);
+      put((uint64_t)b.n_seq * kv.n_kv_head * s.seq_runs, s.seq_cap, s.so, s.sml);
+    } else {
+      s.line = true;
+      put(2u * ((uint64_t)b.n_seq * s.seq_groups * kv.n_kv_head + kAttnMaxCtas), s.seq_cap, s.so, s.sml);
+    }
+  }
   return s;
 }
 
+template <uint32_t HD, uint32_t R>
+void attn_few(const KvAttnParams& p, uint32_t prefix, cudaStream_t st) {
+  const dim3 grid(prefix ? p.prefix_runs : p.seq_runs, p.n_kv_head, prefix ? 1u : p.rows.n_seq);
+  kv_attn_few_kernel<HD, R><<<grid, kFewThreads, 0, st>>>(p, prefix, prefix ? p.prefix_run : p.seq_run);
+}
 template <uint32_t HD>
-cudaError_t attn_launch(const KvAttnParams& p, int num_sms, uint64_t work, cudaStream_t st) {
+void attn_few_rows(const KvAttnParams& p, uint32_t prefix, uint32_t rows, cudaStream_t st) {
+  if (rows == 1) attn_few<HD, 1>(p, prefix, st);
+  else if (rows == 2) attn_few<HD, 2>(p, prefix, st);
+  else attn_few<HD, 4>(p, prefix, st);
+}
+
+template <uint32_t HD>
+cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t work, cudaStream_t st) {
   using G = AttnGeo<HD>;
-  static SmemAttr attr;
-  const uint32_t smem = G::smem(p.rows.n_seq);
-  cudaError_t e = ensure_smem_attr((const void*)kv_attn_kernel<HD>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
-  if (e != cudaSuccess) return e;
-  uint64_t grid = (uint64_t)G::kCtas * (uint32_t)num_sms;
-  if (grid > kAttnMaxCtas) grid = kAttnMaxCtas;
-  if (grid > work) grid = work;
-  if (grid == 0) grid = 1;
-  kv_attn_kernel<HD><<<(uint32_t)grid, kAttnThreads, smem, st>>>(p);
+  cudaError_t e = cudaSuccess;
+  if (p.seq_run > 0) attn_few_rows<HD>(p, 0, p.seq_cap, st);
+  if (p.prefix_run > 0) attn_few_rows<HD>(p, 1, p.prefix_cap, st);
+  if (line) {
+    static SmemAttr attr;
+    e = ensure_smem_attr((const void*)kv_attn_kernel<HD>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
+    if (e != cudaSuccess) return e;
+    uint64_t grid = (uint64_t)G::kCtas * (uint32_t)num_sms;
+    if (grid > kAttnMaxCtas) grid = kAttnMaxCtas;
+    if (grid > work) grid = work;
+    if (grid == 0) grid = 1;
+    kv_attn_kernel<HD><<<(uint32_t)grid, kAttnThreads, G::smem(p.rows.n_seq), st>>>(p);
+  }
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
@@ -1058,7 +1429,7 @@ cudaError_t attn_launch(const KvAttnParams& p, int num_sms, uint64_t work, cudaS
 }  // namespace
 
 size_t kv_attn_scratch_bytes(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
-  return attn_scratch(kv, b, n_head).bytes;
+  return attn_split(kv, b, n_head).bytes;
 }
 
 // The line of tiles of the largest lengths (its words are 32-bit).
@@ -1076,7 +1447,7 @@ cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* 
                            uint64_t out_stride, uint32_t n_head, float scale, void* scratch, int num_sms,
                            uint32_t* err, cudaStream_t st) {
   if (b.n_rows == 0 || b.n_seq == 0) return cudaSuccess;
-  const AttnScratch s = attn_scratch(kv, b, n_head);
+  const AttnSplit s = attn_split(kv, b, n_head);
   uint8_t* ws = static_cast<uint8_t*>(scratch);
   KvAttnParams p{};
   p.rows = KvRows{b.row0, b.n_seq, b.n_rows, b.row0 ? 0u : b.n_rows / b.n_seq};
@@ -1105,13 +1476,18 @@ cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* 
   p.pml = reinterpret_cast<float*>(ws + s.pml);
   p.so = reinterpret_cast<float*>(ws + s.so);
   p.sml = reinterpret_cast<float*>(ws + s.sml);
+  p.prefix_cap = s.prefix_cap;
   p.seq_cap = s.seq_cap;
   p.seq_groups = s.seq_groups;
+  p.prefix_run = s.prefix_run;
+  p.prefix_runs = s.prefix_runs;
+  p.seq_run = s.seq_run;
+  p.seq_runs = s.seq_runs;
   p.err = err;
   const uint64_t work = kv_attn_work_bound(kv, b, n_head);
-  if (kv.head_dim == 64) return attn_launch<64>(p, num_sms, work, st);
-  if (kv.head_dim == 128) return attn_launch<128>(p, num_sms, work, st);
-  return attn_launch<256>(p, num_sms, work, st);
+  if (kv.head_dim == 64) return attn_launch<64>(p, s.line, num_sms, work, st);
+  if (kv.head_dim == 128) return attn_launch<128>(p, s.line, num_sms, work, st);
+  return attn_launch<256>(p, s.line, num_sms, work, st);
 }
 
 }  // namespace eos
