@@ -1,5 +1,6 @@
 // kv_q8.cu -- the 8-bit paged key/value cache: rows quantised as they are
-// written, and read back (layout and quantizer: kv_q8.cuh).
+// written, and read back (layout and quantizer: kv_q8.cuh).  Both directions
+// share their kernels: one for a few rows per sequence, one for many.
 #include "eos_kernels.h"
 #include "kv_q8.cuh"
 
@@ -38,57 +39,240 @@ __device__ __forceinline__ uint8_t* kv_locate(const KvCopyParams& p, uint32_t r,
   return p.pages + ((size_t)page * p.n_kv_head + h) * kv_block_bytes(hd);
 }
 
-// One warp per (row, head): lane l holds elements l E .. l E + E - 1.
-template <uint32_t HD>
-__global__ void __launch_bounds__(256) kv_write_rows_kernel(const KvCopyParams p) {
-  constexpr uint32_t E = HD / 32u;
-  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
+// Byte e of four words as one word.
+__device__ __forceinline__ uint32_t kv_pick_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e) {
+  const uint32_t sel = e | ((e + 4u) << 4);
+  return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
+}
+__device__ __forceinline__ uint32_t kv_quant4(float4 v, const KvRowScale& s) {
+  return (uint32_t)(kv_quant(v.x, s) & 0xff) | ((uint32_t)(kv_quant(v.y, s) & 0xff) << 8) |
+         ((uint32_t)(kv_quant(v.z, s) & 0xff) << 16) | ((uint32_t)kv_quant(v.w, s) << 24);
+}
+__device__ __forceinline__ uint32_t kv_absmax4(uint32_t amax, float4 v) {
+  amax = max(max(amax, __float_as_uint(v.x) & 0x7fffffffu), __float_as_uint(v.y) & 0x7fffffffu);
+  return max(max(amax, __float_as_uint(v.z) & 0x7fffffffu), __float_as_uint(v.w) & 0x7fffffffu);
+}
+__device__ __forceinline__ float4 kv_value4(uint32_t w, float s) {
+  return make_float4(__fmul_rn((float)(int8_t)w, s), __fmul_rn((float)(int8_t)(w >> 8), s),
+                     __fmul_rn((float)(int8_t)(w >> 16), s), __fmul_rn((float)(int8_t)(w >> 24), s));
+}
+
+// ---- a few rows per sequence (a decode step) -----------------------------------
+// One warp per (row, head); lane l holds elements 4 l + 128 c .. + 3.  A row's
+// value bytes lie HD / 4 sectors apart, so this moves a sector per byte: right
+// for a token or a few, where a launch is what counts.
+template <uint32_t HD, bool READ>
+__global__ void __launch_bounds__(128) kv_rows_kernel(const KvCopyParams p) {
+  constexpr uint32_t C = HD <= 128u ? 1u : HD / 128u;
+  const uint64_t w = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 5);
   const uint32_t lane = threadIdx.x & 31u;
   if (w >= (uint64_t)p.rows.n_rows * p.n_kv_head) return;  // warp-uniform
   const uint32_t r = (uint32_t)(w / p.n_kv_head), h = (uint32_t)(w % p.n_kv_head);
+  const bool on = HD >= 128u || lane < HD / 4u;
+  const size_t at = r * p.row_stride + h * HD + lane * 4u;
+  float4 x[2][C];
+  if (!READ) {  // the loads fly while the slot is looked up
+#pragma unroll
+    for (uint32_t which = 0; which < 2; ++which)
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c)
+        x[which][c] = on ? *reinterpret_cast<const float4*>((which ? p.v : p.k) + at + c * 128u)
+                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   uint32_t slot;
   uint8_t* blk = kv_locate(p, r, h, HD, slot);
   if (blk == nullptr) return;
 #pragma unroll
   for (uint32_t which = 0; which < 2; ++which) {
-    const float* src = (which ? p.v : p.k) + r * p.row_stride + h * HD + lane * E;
-    float x[E];
-    uint32_t amax = 0;
+    float* sc = reinterpret_cast<float*>(blk + kv_scale_offset<HD>(slot, which));
+    if (READ) {
+      const float s = *sc;
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-      x[e] = src[e];
-      const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
-      amax = b > amax ? b : amax;
-    }
-    const KvRowScale s = kv_row_scale(__reduce_max_sync(0xffffffffu, amax));
+      for (uint32_t c = 0; c < C; ++c) {
+        const uint32_t d = lane * 4u + c * 128u;
+        uint32_t q = 0;
+        if (on && which == 0) q = *reinterpret_cast<const uint32_t*>(blk + kv_k_offset<HD>(slot, d));
+        if (on && which == 1)
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-      const uint32_t d = lane * E + e;
-      blk[which ? kv_v_offset<HD>(slot, d) : kv_k_offset<HD>(slot, d)] = (uint8_t)kv_quant(x[e], s);
+          for (uint32_t e = 0; e < 4u; ++e) q |= (uint32_t)blk[kv_v_offset<HD>(slot, d + e)] << (8u * e);
+        if (on) *reinterpret_cast<float4*>((which ? p.v : p.k) + at + c * 128u) = kv_value4(q, s);
+      }
+    } else {
+      uint32_t amax = 0;
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c) amax = kv_absmax4(amax, x[which][c]);
+      const KvRowScale s = kv_row_scale(__reduce_max_sync(0xffffffffu, amax));
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c) {
+        const uint32_t d = lane * 4u + c * 128u, q = kv_quant4(x[which][c], s);
+        if (on && which == 0) *reinterpret_cast<uint32_t*>(blk + kv_k_offset<HD>(slot, d)) = q;
+        if (on && which == 1)
+#pragma unroll
+          for (uint32_t e = 0; e < 4u; ++e) blk[kv_v_offset<HD>(slot, d + e)] = (uint8_t)(q >> (8u * e));
+      }
+      if (lane == 0) *sc = s.scale;
     }
-    if (lane == 0) *reinterpret_cast<float*>(blk + kv_scale_offset<HD>(slot, which)) = s.scale;
   }
 }
 
-template <uint32_t HD>
-__global__ void __launch_bounds__(256) kv_read_rows_kernel(const KvCopyParams p) {
-  constexpr uint32_t E = HD / 32u;
-  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
-  const uint32_t lane = threadIdx.x & 31u;
-  if (w >= (uint64_t)p.rows.n_rows * p.n_kv_head) return;  // warp-uniform
-  const uint32_t r = (uint32_t)(w / p.n_kv_head), h = (uint32_t)(w % p.n_kv_head);
-  uint32_t slot;
-  const uint8_t* blk = kv_locate(p, r, h, HD, slot);
-  if (blk == nullptr) return;
+// ---- many rows: a quarter of a page per CTA --------------------------------------
+// One CTA of 256 threads per (32-token quarter, head).  Warp g has tokens g, g +
+// 8, g + 16, g + 24 -- the four that are neighbours in a value row -- and a
+// lane four neighbouring elements of each, so both layouts are whole words:
+// a key row's word is a token's four elements, a value row's word an element's
+// four tokens (a 4 x 4 byte transpose in registers).  The words of the 32
+// tokens meet in shared memory (rows of nine words: the lanes' accesses then
+// collide four ways at most) and value rows move as 16 bytes a thread.  Every
+// byte moves once; reading and writing f32 rows is what bounds it.
+//
+// Quarters of a ragged batch: sequence i's blocks start at row0[i] / 32 + 2 i,
+// which leaves room for the two broken ends; a CTA searches its sequence.
+template <uint32_t HD, bool READ>
+__global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
+  constexpr uint32_t C = HD <= 128u ? 1u : HD / 128u;
+  constexpr uint32_t PITCH = 9u;  // words per value row in shared memory
+  __shared__ uint32_t vt[HD * PITCH];
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, g = tid >> 5, h = blockIdx.y;
+  uint32_t i = 0;
+  {
+    uint32_t lo = 0, hi = p.rows.n_seq;
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (kv_row_start(p.rows, mid) / 32u + 2u * mid <= blockIdx.x) lo = mid;
+      else hi = mid;
+    }
+    i = lo;
+  }
+  const uint32_t r0 = kv_row_start(p.rows, i), r1 = kv_row_start(p.rows, i + 1u), n = r1 > r0 ? r1 - r0 : 0u;
+  const uint64_t pos = p.pos[i];
+  const uint32_t b0 = r0 / 32u + 2u * i;
+  if (blockIdx.x < b0) return;  // (rows before the first sequence)
+  const uint64_t t0 = (pos & ~(uint64_t)31u) + 32ull * (blockIdx.x - b0);  // the quarter's first position
+  if (n == 0 || t0 >= pos + n) return;
+  uint32_t page = 0xffffffffu;
+  if (t0 < (uint64_t)p.table_stride * kKvPage) page = p.table[(size_t)i * p.table_stride + (uint32_t)(t0 / kKvPage)];
+  if (page >= p.n_pages) {
+    if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
+    return;
+  }
+  uint8_t* blk = p.pages + ((size_t)page * p.n_kv_head + h) * kv_block_bytes(HD);
+  const uint32_t s0 = (uint32_t)(t0 % kKvPage);
+  const bool whole = t0 >= pos && t0 + 32u <= pos + n;
+  uint8_t* vq = blk + kKvPage * HD + (s0 / kKvQuarter) * (HD * kKvQuarter);
+  const bool on = HD >= 128u || lane < HD / 4u;
+  // value rows of the quarter as 16-byte chunks: chunk x is element x / 2, half x % 2
+  auto chunk = [&](uint32_t x) { return vq + (x >> 1) * 32u + (((x & 1u) ^ ((x >> 1) >> 2)) & 1u) * 16u; };
+  if (READ) {
 #pragma unroll
-  for (uint32_t which = 0; which < 2; ++which) {
-    float* dst = (which ? p.v : p.k) + r * p.row_stride + h * HD + lane * E;
-    const float s = *reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(slot, which));
+    for (uint32_t x = tid; x < 2u * HD; x += 256u) {
+      const uint4 v = *reinterpret_cast<const uint4*>(chunk(x));
+      uint32_t* dst = vt + (x >> 1) * PITCH + (x & 1u) * 4u;
+      dst[0] = v.x;
+      dst[1] = v.y;
+      dst[2] = v.z;
+      dst[3] = v.w;
+    }
+  }
+  uint32_t kw[4][C], vw[4][C];
+  float ks[4], vs[4];
+  bool in[4];
+  size_t at[4];
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-      const uint32_t d = lane * E + e;
-      const int8_t q = (int8_t)blk[which ? kv_v_offset<HD>(slot, d) : kv_k_offset<HD>(slot, d)];
-      dst[e] = __fmul_rn((float)q, s);
+  for (uint32_t j = 0; j < 4u; ++j) {
+    const uint64_t t = t0 + g + 8u * j;
+    in[j] = t >= pos && t < pos + n;
+    at[j] = in[j] ? (size_t)(r0 + (uint32_t)(t - pos)) * p.row_stride + h * HD + lane * 4u : 0u;
+  }
+  if (!READ) {
+    float4 x[2][4][C];
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j)
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c) {
+        x[0][j][c] = x[1][j][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (in[j] && on) {
+          x[0][j][c] = __ldcs(reinterpret_cast<const float4*>(p.k + at[j] + c * 128u));
+          x[1][j][c] = __ldcs(reinterpret_cast<const float4*>(p.v + at[j] + c * 128u));
+        }
+      }
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) {
+      uint32_t ka = 0, va = 0;
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c) {
+        ka = kv_absmax4(ka, x[0][j][c]);
+        va = kv_absmax4(va, x[1][j][c]);
+      }
+      const KvRowScale sk = kv_row_scale(__reduce_max_sync(0xffffffffu, ka));
+      const KvRowScale sv = kv_row_scale(__reduce_max_sync(0xffffffffu, va));
+      ks[j] = sk.scale;
+      vs[j] = sv.scale;
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c) {
+        kw[j][c] = kv_quant4(x[0][j][c], sk);
+        vw[j][c] = kv_quant4(x[1][j][c], sv);
+      }
+      if (!in[j]) continue;  // warp-uniform
+      const uint32_t slot = s0 + g + 8u * j;
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c)
+        if (on) *reinterpret_cast<uint32_t*>(blk + kv_k_offset<HD>(slot, lane * 4u + c * 128u)) = kw[j][c];
+      if (lane < 2u) *reinterpret_cast<float*>(blk + kv_scale_offset<HD>(slot, lane)) = lane ? vs[j] : ks[j];
+    }
+    if (whole) {
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c)
+        if (on)
+#pragma unroll
+          for (uint32_t e = 0; e < 4u; ++e)
+            vt[(lane * 4u + c * 128u + e) * PITCH + g] = kv_pick_bytes(vw[0][c], vw[1][c], vw[2][c], vw[3][c], e);
+    } else {  // a broken end: the neighbours' bytes stay as they are
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j)
+        if (in[j] && on)
+#pragma unroll
+          for (uint32_t c = 0; c < C; ++c)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e)
+              blk[kv_v_offset<HD>(s0 + g + 8u * j, lane * 4u + c * 128u + e)] = (uint8_t)(vw[j][c] >> (8u * e));
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) {
+      const uint32_t slot = s0 + g + 8u * j;
+      ks[j] = vs[j] = 0.0f;
+      if (!in[j]) continue;  // warp-uniform
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c)
+        kw[j][c] = on ? *reinterpret_cast<const uint32_t*>(blk + kv_k_offset<HD>(slot, lane * 4u + c * 128u)) : 0u;
+      ks[j] = *reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(slot, 0));
+      vs[j] = *reinterpret_cast<const float*>(blk + kv_scale_offset<HD>(slot, 1));
+    }
+  }
+  __syncthreads();
+  if (!READ) {
+    if (whole) {
+#pragma unroll
+      for (uint32_t x = tid; x < 2u * HD; x += 256u) {
+        const uint32_t* src = vt + (x >> 1) * PITCH + (x & 1u) * 4u;
+        *reinterpret_cast<uint4*>(chunk(x)) = make_uint4(src[0], src[1], src[2], src[3]);
+      }
+    }
+    return;
+  }
+  uint32_t w[C][4];
+#pragma unroll
+  for (uint32_t c = 0; c < C; ++c)
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e) w[c][e] = on ? vt[(lane * 4u + c * 128u + e) * PITCH + g] : 0u;
+#pragma unroll
+  for (uint32_t j = 0; j < 4u; ++j) {
+    if (!in[j] || !on) continue;
+#pragma unroll
+    for (uint32_t c = 0; c < C; ++c) {
+      __stcs(reinterpret_cast<float4*>(p.k + at[j] + c * 128u), kv_value4(kw[j][c], ks[j]));
+      __stcs(reinterpret_cast<float4*>(p.v + at[j] + c * 128u),
+             kv_value4(kv_pick_bytes(w[c][0], w[c][1], w[c][2], w[c][3], j), vs[j]));
     }
   }
 }
@@ -110,28 +294,38 @@ KvCopyParams copy_params(const KvPool& kv, const KvRowSet& rs, const float* k, c
   p.err = err;
   return p;
 }
+
+// Rows or quarters: a quarter's CTA pays off from about four rows of a sequence
+// on (its launch covers up to two broken quarters per sequence).
+template <bool READ>
+cudaError_t copy_launch(const KvPool& kv, const KvCopyParams& p, cudaStream_t st) {
+  const KvRows& r = p.rows;
+  const uint64_t blocks = (uint64_t)r.n_rows / 32u + 2ull * r.n_seq;
+  if (r.n_rows >= 4ull * r.n_seq && kv.n_kv_head <= 65535u) {
+    const dim3 grid((uint32_t)blocks, kv.n_kv_head);
+    if (kv.head_dim == 64) kv_quarter_kernel<64, READ><<<grid, 256, 0, st>>>(p);
+    else if (kv.head_dim == 128) kv_quarter_kernel<128, READ><<<grid, 256, 0, st>>>(p);
+    else kv_quarter_kernel<256, READ><<<grid, 256, 0, st>>>(p);
+  } else {
+    const uint32_t grid = (uint32_t)(((uint64_t)r.n_rows * kv.n_kv_head + 3u) / 4u);
+    if (kv.head_dim == 64) kv_rows_kernel<64, READ><<<grid, 128, 0, st>>>(p);
+    else if (kv.head_dim == 128) kv_rows_kernel<128, READ><<<grid, 128, 0, st>>>(p);
+    else kv_rows_kernel<256, READ><<<grid, 128, 0, st>>>(p);
+  }
+  return cudaGetLastError();
+}
 }  // namespace
 
 cudaError_t launch_kv_write(const KvPool& kv, const KvRowSet& rs, const float* k, const float* v, uint64_t row_stride,
                             uint32_t* err, cudaStream_t st) {
   if (rs.n_rows == 0 || rs.n_seq == 0) return cudaSuccess;
-  const KvCopyParams p = copy_params(kv, rs, k, v, row_stride, err);
-  const uint32_t grid = (uint32_t)(((uint64_t)rs.n_rows * kv.n_kv_head + 7u) / 8u);
-  if (kv.head_dim == 64) kv_write_rows_kernel<64><<<grid, 256, 0, st>>>(p);
-  else if (kv.head_dim == 128) kv_write_rows_kernel<128><<<grid, 256, 0, st>>>(p);
-  else kv_write_rows_kernel<256><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  return copy_launch<false>(kv, copy_params(kv, rs, k, v, row_stride, err), st);
 }
 
 cudaError_t launch_kv_read(const KvPool& kv, const KvRowSet& rs, float* k, float* v, uint64_t row_stride,
                            uint32_t* err, cudaStream_t st) {
   if (rs.n_rows == 0 || rs.n_seq == 0) return cudaSuccess;
-  const KvCopyParams p = copy_params(kv, rs, k, v, row_stride, err);
-  const uint32_t grid = (uint32_t)(((uint64_t)rs.n_rows * kv.n_kv_head + 7u) / 8u);
-  if (kv.head_dim == 64) kv_read_rows_kernel<64><<<grid, 256, 0, st>>>(p);
-  else if (kv.head_dim == 128) kv_read_rows_kernel<128><<<grid, 256, 0, st>>>(p);
-  else kv_read_rows_kernel<256><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  return copy_launch<true>(kv, copy_params(kv, rs, k, v, row_stride, err), st);
 }
 
 }  // namespace eos

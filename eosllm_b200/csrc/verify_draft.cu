@@ -34,46 +34,109 @@ __device__ __forceinline__ double vd_weight(float p, float q, bool residual) {
   return (p > 0.0f && p < INFINITY) ? (double)p : 0.0;
 }
 
-constexpr uint32_t kVdThreads = 1024, kVdWarps = kVdThreads / 32;
+// Four neighbouring weights v .. v + 3 of [.., hi) (0 beyond).
+template <bool VEC>
+__device__ __forceinline__ void vd_weights4(const float* p, const float* q, uint32_t v, uint32_t hi, bool residual,
+                                            double* w) {
+  float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (VEC && v + 4u <= hi) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(p + v));
+    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+    if (residual) {
+      const float4 y = __ldg(reinterpret_cast<const float4*>(q + v));
+      b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e)
+      if (v + e < hi) {
+        a[e] = __ldg(p + v + e);
+        if (residual) b[e] = __ldg(q + v + e);
+      }
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 4u; ++e) w[e] = vd_weight(a[e], b[e], residual);
+}
 
-// One CTA per sequence; warp w owns the w-th contiguous slice of the row.
-__global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyParams a) {
+constexpr uint32_t kVdThreads = 512, kVdWarps = kVdThreads / 32, kVdMaxCluster = 8;
+
+__device__ __forceinline__ void vd_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// Address of a shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t vd_map(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(a)
+      : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return a;
+}
+
+// One cluster of CTAs per sequence; CTA c and in it warp w own the row's
+// contiguous slices in order.  A first pass sums the slices and tells every CTA
+// the others' sums; the warp whose slice crosses the cut goes over it once
+// more (from L1 or L2).  Reading one or two rows once is what bounds it for
+// many sequences, the chain of three reads (draft, its probabilities, the
+// row) for few: so few sequences get eight CTAs each.
+template <bool VEC>
+__global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyParams a, uint32_t n_cta) {
   __shared__ uint32_t s_taken;
   __shared__ double s_sum[kVdWarps];
   __shared__ uint32_t s_last[kVdWarps];
-  const uint32_t i = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  __shared__ double c_sum[kVdMaxCluster];
+  __shared__ uint32_t c_last[kVdMaxCluster];
+  const uint32_t i = blockIdx.x / n_cta, cta = blockIdx.x % n_cta;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t kk = a.max_draft;
   uint32_t k = a.n_draft != nullptr ? a.n_draft[i] : kk;
   if (k > kk) k = kk;
   const float* prow = a.p + (size_t)i * (kk + 1u) * a.stride;
   const float* qrow = a.q + (size_t)i * kk * a.stride;
-  if (tid == 0) {
-    uint32_t t = 0;
-    for (; t < k; ++t) {
-      const uint32_t x = a.drafts[(size_t)i * kk + t];
-      if (x >= a.n_vocab) break;
-      const double lhs = (double)a.u[(size_t)i * (kk + 1u) + t] * (double)qrow[t * a.stride + x];
-      if (!(lhs < (double)prow[t * a.stride + x])) break;
+  const float* urow = a.u + (size_t)i * (kk + 1u);
+  const double u = (double)urow[kk];
+  if (warp == 0) {  // 32 drafts at a time: the first that is not accepted
+    uint32_t taken = k;
+    for (uint32_t t0 = 0; t0 < k; t0 += 32u) {
+      const uint32_t t = t0 + lane;
+      bool good = t >= k;
+      if (t < k) {
+        const uint32_t x = a.drafts[(size_t)i * kk + t];
+        if (x < a.n_vocab)
+          good = (double)urow[t] * (double)qrow[t * a.stride + x] < (double)prow[t * a.stride + x];
+      }
+      const uint32_t bad = __ballot_sync(0xffffffffu, !good);
+      if (bad) {
+        taken = t0 + (uint32_t)__ffs((int)bad) - 1u;
+        break;
+      }
     }
-    s_taken = t;
+    if (lane == 0) s_taken = taken;
   }
   __syncthreads();
   const uint32_t taken = s_taken;
   const float* pr = prow + taken * a.stride;
   const float* qr = qrow + taken * a.stride;
-  const double u = (double)a.u[(size_t)i * (kk + 1u) + kk];
-  const uint32_t per = ((a.n_vocab + kVdThreads - 1u) / kVdThreads) * 32u;  // a warp's slice
-  const uint32_t lo = warp * per < a.n_vocab ? warp * per : a.n_vocab;
-  const uint32_t hi = lo + per < a.n_vocab ? lo + per : a.n_vocab;
+  // slices in steps of 128 elements (four per lane)
+  const uint32_t steps = (a.n_vocab + 127u) / 128u, per = (steps + n_cta * kVdWarps - 1u) / (n_cta * kVdWarps);
+  const uint32_t s_lo = (cta * kVdWarps + warp) * per;
+  const uint32_t lo = s_lo < steps ? s_lo * 128u : a.n_vocab;
+  const uint32_t hi = lo + per * 128u < a.n_vocab ? lo + per * 128u : a.n_vocab;
   bool residual = taken < k;
-  for (;;) {
+  for (;;) {  // (a second time where p_a <= q_a everywhere: draw from p_a)
     double sum = 0.0;
     uint32_t last = 0;  // 1 + the last index with weight
-    for (uint32_t v = lo + lane; v < hi; v += 32u) {
-      const double w = vd_weight(pr[v], residual ? qr[v] : 0.0f, residual);
-      sum += w;
-      if (w > 0.0) last = v + 1u;
+#pragma unroll 4
+    for (uint32_t v0 = lo; v0 < hi; v0 += 128u) {
+      const uint32_t v = v0 + lane * 4u;
+      double w[4];
+      vd_weights4<VEC>(pr, qr, v, hi, residual, w);
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e) {
+        sum += w[e];
+        if (w[e] > 0.0) last = v + e + 1u;
+      }
     }
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     last = __reduce_max_sync(0xffffffffu, last);
     if (lane == 0) {
@@ -81,59 +144,88 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
       s_last[warp] = last;
     }
     __syncthreads();
-    double total = 0.0;
-    uint32_t end = 0;
-    for (uint32_t w = 0; w < kVdWarps; ++w) {
-      total += s_sum[w];
-      end = s_last[w] > end ? s_last[w] : end;
+    if (tid < n_cta) {  // this CTA's sum into every CTA
+      double t = 0.0;
+      uint32_t e = 0;
+#pragma unroll
+      for (uint32_t w = 0; w < kVdWarps; ++w) {
+        t += s_sum[w];
+        e = s_last[w] > e ? s_last[w] : e;
+      }
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(vd_map(&c_sum[cta], tid)), "d"(t) : "memory");
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(vd_map(&c_last[cta], tid)), "r"(e) : "memory");
     }
-    if (end == 0 && residual) {  // p_a <= q_a everywhere: draw from p_a
+    vd_cluster_sync();
+    double total = 0.0, base = 0.0;
+    uint32_t end = 0;
+    for (uint32_t c = 0; c < n_cta; ++c) {
+      if (c == cta) base = total;
+      total += c_sum[c];
+      end = c_last[c] > end ? c_last[c] : end;
+    }
+    if (end == 0 && residual) {
       residual = false;
-      __syncthreads();
+      vd_cluster_sync();  // every CTA has read the sums
       continue;
     }
     const double cut = u * total;
-    // the warp whose slice crosses the cut, or, past every rounding, the last one with weight
-    double before = 0.0;
+    // the first slice that crosses the cut or, past every rounding, holds the last weight
+    bool before = false;
+    double run = 0.0;
+    for (uint32_t c = 0; c < cta; ++c) {
+      if (c_last[c] != 0 && (run + c_sum[c] > cut || c_last[c] == end)) before = true;
+      run += c_sum[c];
+    }
     uint32_t pick = kVdWarps;
-    double base = 0.0;
-    for (uint32_t w = 0; w < kVdWarps; ++w) {
-      if (s_last[w] != 0 && (before + s_sum[w] > cut || s_last[w] == end)) {
-        pick = w;
-        base = before;
-        break;
+    if (!before)
+      for (uint32_t w = 0; w < kVdWarps; ++w) {
+        if (s_last[w] != 0 && (base + s_sum[w] > cut || s_last[w] == end)) {
+          pick = w;
+          break;
+        }
+        base += s_sum[w];
       }
-      before += s_sum[w];
-    }
-    if (tid == 0) {
-      if (pick == kVdWarps) a.tokens[(size_t)i * (kk + 1u) + taken] = 0xffffffffu;  // no weight at all
-      a.n_token[i] = taken + (pick < kVdWarps ? 1u : 0u);
-    }
     if (warp == pick) {
-      double run = base;
       uint32_t tok = s_last[pick] - 1u;
-      for (uint32_t v0 = lo; v0 < hi; v0 += 32u) {
-        const uint32_t v = v0 + lane;
-        double w = v < hi ? vd_weight(pr[v], residual ? qr[v] : 0.0f, residual) : 0.0;
-        double c = w;
+      double at = base;
+      for (uint32_t v0 = lo; v0 < hi; v0 += 128u) {
+        const uint32_t v = v0 + lane * 4u;
+        double w[4];
+        vd_weights4<VEC>(pr, qr, v, hi, residual, w);
+        const double mine = (w[0] + w[1]) + (w[2] + w[3]);
+        double c = mine;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const double t = __shfl_up_sync(0xffffffffu, c, o);
           if ((int)lane >= o) c += t;
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && run + c > cut);
-        if (hit) {
-          tok = v0 + (uint32_t)__ffs((int)hit) - 1u;
+        double s = at + (c - mine);
+        uint32_t hit = 4u;
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+          s += w[e];
+          if (hit == 4u && w[e] > 0.0 && s > cut) hit = e;
+        }
+        const uint32_t any = __ballot_sync(0xffffffffu, hit < 4u);
+        if (any) {
+          const uint32_t src = (uint32_t)__ffs((int)any) - 1u;
+          tok = v0 + src * 4u + __shfl_sync(0xffffffffu, hit, (int)src);
           break;
         }
-        run += __shfl_sync(0xffffffffu, c, 31);
+        at += __shfl_sync(0xffffffffu, c, 31);
       }
       if (lane == 0) a.tokens[(size_t)i * (kk + 1u) + taken] = tok;
     }
+    if (cta == 0 && tid == 0) {
+      if (end == 0) a.tokens[(size_t)i * (kk + 1u) + taken] = 0xffffffffu;  // no weight at all
+      a.n_token[i] = taken + (end != 0 ? 1u : 0u);
+    }
     break;
   }
-  for (uint32_t t = tid; t <= kk; t += kVdThreads)
-    if (t != taken) a.tokens[(size_t)i * (kk + 1u) + t] = t < taken ? a.drafts[(size_t)i * kk + t] : 0xffffffffu;
-  
+  if (cta == 0)
+    for (uint32_t t = tid; t <= kk; t += kVdThreads)
+      if (t != taken) a.tokens[(size_t)i * (kk + 1u) + t] = t < taken ? a.drafts[(size_t)i * kk + t] : 0xffffffffu;
+  vd_cluster_sync();  // no CTA leaves while another may still write into it
 }
 
 cudaError_t launch_verify_draft(const float* p, const float* q, uint64_t stride, const uint32_t* drafts,
@@ -141,8 +233,23 @@ cudaError_t launch_verify_draft(const float* p, const float* q, uint64_t stride,
                                 uint32_t n_vocab, uint32_t* tokens, uint32_t* n_token, cudaStream_t st) {
   if (n_seq == 0) return cudaSuccess;
   const VerifyParams a{p, q, stride, drafts, n_draft, u, max_draft, n_vocab, tokens, n_token};
-  verify_draft_kernel<<<n_seq, kVdThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  // as many CTAs per sequence (1, 2, 4 or 8) as keep two per SM, each warp with a step to do
+  uint32_t n_cta = 1;
+  while (n_cta < kVdMaxCluster && 2ull * n_cta * n_seq <= 296u && 2u * n_cta * kVdWarps * 128u <= n_vocab) n_cta *= 2u;
+  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0 && stride % 4u == 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n_seq * n_cta);
+  cfg.blockDim = dim3(kVdThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = n_cta;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return vec ? cudaLaunchKernelEx(&cfg, verify_draft_kernel<true>, a, n_cta)
+             : cudaLaunchKernelEx(&cfg, verify_draft_kernel<false>, a, n_cta);
 }
 
 }  // namespace eos
