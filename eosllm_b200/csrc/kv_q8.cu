@@ -44,10 +44,6 @@ __device__ __forceinline__ uint32_t kv_pick_bytes(uint32_t a, uint32_t b, uint32
   const uint32_t sel = e | ((e + 4u) << 4);
   return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
-__device__ __forceinline__ uint32_t kv_quant4(float4 v, const KvRowScale& s) {
-  return (uint32_t)(kv_quant(v.x, s) & 0xff) | ((uint32_t)(kv_quant(v.y, s) & 0xff) << 8) |
-         ((uint32_t)(kv_quant(v.z, s) & 0xff) << 16) | ((uint32_t)kv_quant(v.w, s) << 24);
-}
 __device__ __forceinline__ uint32_t kv_absmax4(uint32_t amax, float4 v) {
   amax = max(max(amax, __float_as_uint(v.x) & 0x7fffffffu), __float_as_uint(v.y) & 0x7fffffffu);
   return max(max(amax, __float_as_uint(v.z) & 0x7fffffffu), __float_as_uint(v.w) & 0x7fffffffu);
@@ -162,8 +158,14 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
   const bool on = HD >= 128u || lane < HD / 4u;
   // value rows of the quarter as 16-byte chunks: chunk x is element x / 2, half x % 2
   auto chunk = [&](uint32_t x) { return vq + (x >> 1) * 32u + (((x & 1u) ^ ((x >> 1) >> 2)) & 1u) * 16u; };
-  if (READ) {
+  // the bytes of word w of a value row (tokens w, w + 8, w + 16, w + 24) that this call writes
+  auto keep = [&](uint32_t w) {
+    uint32_t m = 0;
 #pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) m |= (t0 + w + 8u * j >= pos && t0 + w + 8u * j < pos + n) ? 0xffu << (8u * j) : 0u;
+    return m;
+  };
+  if (READ) {
     for (uint32_t x = tid; x < 2u * HD; x += 256u) {
       const uint4 v = *reinterpret_cast<const uint4*>(chunk(x));
       uint32_t* dst = vt + (x >> 1) * PITCH + (x & 1u) * 4u;
@@ -219,23 +221,12 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
         if (on) *reinterpret_cast<uint32_t*>(blk + kv_k_offset<HD>(slot, lane * 4u + c * 128u)) = kw[j][c];
       if (lane < 2u) *reinterpret_cast<float*>(blk + kv_scale_offset<HD>(slot, lane)) = lane ? vs[j] : ks[j];
     }
-    if (whole) {
 #pragma unroll
-      for (uint32_t c = 0; c < C; ++c)
-        if (on)
+    for (uint32_t c = 0; c < C; ++c)
+      if (on)
 #pragma unroll
-          for (uint32_t e = 0; e < 4u; ++e)
-            vt[(lane * 4u + c * 128u + e) * PITCH + g] = kv_pick_bytes(vw[0][c], vw[1][c], vw[2][c], vw[3][c], e);
-    } else {  // a broken end: the neighbours' bytes stay as they are
-#pragma unroll
-      for (uint32_t j = 0; j < 4u; ++j)
-        if (in[j] && on)
-#pragma unroll
-          for (uint32_t c = 0; c < C; ++c)
-#pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e)
-              blk[kv_v_offset<HD>(s0 + g + 8u * j, lane * 4u + c * 128u + e)] = (uint8_t)(vw[j][c] >> (8u * e));
-    }
+        for (uint32_t e = 0; e < 4u; ++e)
+          vt[(lane * 4u + c * 128u + e) * PITCH + g] = kv_pick_bytes(vw[0][c], vw[1][c], vw[2][c], vw[3][c], e);
   } else {
 #pragma unroll
     for (uint32_t j = 0; j < 4u; ++j) {
@@ -250,29 +241,34 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
     }
   }
   __syncthreads();
-  if (!READ) {
-    if (whole) {
-#pragma unroll
-      for (uint32_t x = tid; x < 2u * HD; x += 256u) {
-        const uint32_t* src = vt + (x >> 1) * PITCH + (x & 1u) * 4u;
-        *reinterpret_cast<uint4*>(chunk(x)) = make_uint4(src[0], src[1], src[2], src[3]);
+  if constexpr (!READ) {
+    for (uint32_t x = tid; x < 2u * HD; x += 256u) {
+      const uint32_t* src = vt + (x >> 1) * PITCH + (x & 1u) * 4u;
+      uint4 v = make_uint4(src[0], src[1], src[2], src[3]);
+      if (!whole) {  // a broken end: the neighbours' bytes stay as they are
+        const uint4 old = *reinterpret_cast<const uint4*>(chunk(x));
+        v.x = (v.x & keep(4u * (x & 1u))) | (old.x & ~keep(4u * (x & 1u)));
+        v.y = (v.y & keep(4u * (x & 1u) + 1u)) | (old.y & ~keep(4u * (x & 1u) + 1u));
+        v.z = (v.z & keep(4u * (x & 1u) + 2u)) | (old.z & ~keep(4u * (x & 1u) + 2u));
+        v.w = (v.w & keep(4u * (x & 1u) + 3u)) | (old.w & ~keep(4u * (x & 1u) + 3u));
       }
+      *reinterpret_cast<uint4*>(chunk(x)) = v;
     }
-    return;
-  }
-  uint32_t w[C][4];
+  } else {
+    uint32_t w[C][4];
 #pragma unroll
-  for (uint32_t c = 0; c < C; ++c)
+    for (uint32_t c = 0; c < C; ++c)
 #pragma unroll
-    for (uint32_t e = 0; e < 4u; ++e) w[c][e] = on ? vt[(lane * 4u + c * 128u + e) * PITCH + g] : 0u;
+      for (uint32_t e = 0; e < 4u; ++e) w[c][e] = on ? vt[(lane * 4u + c * 128u + e) * PITCH + g] : 0u;
 #pragma unroll
-  for (uint32_t j = 0; j < 4u; ++j) {
-    if (!in[j] || !on) continue;
+    for (uint32_t j = 0; j < 4u; ++j) {
+      if (!in[j] || !on) continue;
 #pragma unroll
-    for (uint32_t c = 0; c < C; ++c) {
-      __stcs(reinterpret_cast<float4*>(p.k + at[j] + c * 128u), kv_value4(kw[j][c], ks[j]));
-      __stcs(reinterpret_cast<float4*>(p.v + at[j] + c * 128u),
-             kv_value4(kv_pick_bytes(w[c][0], w[c][1], w[c][2], w[c][3], j), vs[j]));
+      for (uint32_t c = 0; c < C; ++c) {
+        __stcs(reinterpret_cast<float4*>(p.k + at[j] + c * 128u), kv_value4(kw[j][c], ks[j]));
+        __stcs(reinterpret_cast<float4*>(p.v + at[j] + c * 128u),
+               kv_value4(kv_pick_bytes(w[c][0], w[c][1], w[c][2], w[c][3], j), vs[j]));
+      }
     }
   }
 }

@@ -77,14 +77,15 @@ __device__ __forceinline__ uint32_t kv_row_seq(const KvRows& b, uint32_t r) {
 }
 
 // ---- the row quantizer ----------------------------------------------------
-// scale = max|x| * fl32(1 / 127) in f32; q = the integer nearest to 127 x / max|x| (ties
-// to even) of the real quotient: the f32 estimate is off by at most 127 *
-// 2^-23 < 1e-4, so wherever it lies 1e-4 away from a half it decides, and
-// otherwise (about one element in 5000) the f64 quotient does, whose rounding
-// cannot move it across a half (127 x is exact, and a quotient of two floats
-// that is not a half differs from it by more than 2^-33 relative).  A row that
-// holds a NaN or an infinity gets that as its scale and q = 0: it reads back
-// as NaN.
+// scale = max|x| * fl32(1 / 127) in f32; q = the integer nearest to 127 x / max|x|
+// (ties to even) of the real quotient.  The f32 estimate x * fl32(127 / max|x|)
+// is off by at most 127 * 2^-24 < 1e-5, so wherever it lies 1e-4 away from a
+// half it decides: it is rounded by adding 1.5 * 2^23, which leaves q in the
+// sum's low byte, and its distance from q is exact.  Otherwise (about one
+// element in 5000) the f64 quotient decides, whose rounding cannot move it
+// across a half (127 x is exact, and a quotient of two floats that is not a
+// half differs from it by more than 2^-33 relative).  A row that holds a NaN
+// or an infinity gets that as its scale and q = 0: it reads back as NaN.
 struct KvRowScale {
   float scale, amax, inv;
   bool finite, tiny;
@@ -98,12 +99,29 @@ __device__ __forceinline__ KvRowScale kv_row_scale(uint32_t amax_bits) {
   s.inv = (s.finite && !s.tiny) ? __fdiv_rn(127.0f, s.amax) : 0.0f;
   return s;
 }
-__device__ __forceinline__ int32_t kv_quant(float x, const KvRowScale& s) {
-  const float y = __fmul_rn(x, s.inv);
-  const float r = rintf(y);
-  if (fabsf(__fsub_rn(y, r)) <= 0.4999f && !s.tiny) return (int32_t)r;
-  if (!s.finite || s.amax == 0.0f) return 0;
-  return (int32_t)rint(__ddiv_rn(127.0 * (double)x, (double)s.amax));
+static __device__ __noinline__ uint32_t kv_quant4_exact(float4 v, float amax) {
+  const double d = (double)amax;
+  return amax == 0.0f ? 0u
+                      : ((uint32_t)((int32_t)rint(127.0 * (double)v.x / d) & 0xff) |
+                         ((uint32_t)((int32_t)rint(127.0 * (double)v.y / d) & 0xff) << 8) |
+                         ((uint32_t)((int32_t)rint(127.0 * (double)v.z / d) & 0xff) << 16) |
+                         ((uint32_t)((int32_t)rint(127.0 * (double)v.w / d) & 0xff) << 24));
+}
+// Four elements as the bytes of a word.
+__device__ __forceinline__ uint32_t kv_quant4(float4 v, const KvRowScale& s) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+  const float x[4] = {v.x, v.y, v.z, v.w};
+  uint32_t b[4];
+  float off = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float r = __fmaf_rn(x[e], s.inv, kMagic);
+    b[e] = __float_as_uint(r);
+    off = fmaxf(off, fabsf(__fmaf_rn(x[e], s.inv, -__fsub_rn(r, kMagic))));
+  }
+  if (!s.finite) return 0u;
+  if (off > 0.4999f || s.tiny) return kv_quant4_exact(v, s.amax);
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
 }  // namespace eos

@@ -255,8 +255,8 @@ EOSLLM_CUDA_API size_t eosi_cuda_kv_q8_page_bytes(uint32_t n_kv_head, uint32_t h
  * n_rows / n_seq each), which sit at positions pos[i], pos[i] + 1, ... ;
  * position j of sequence i lives in page table[i * table_stride + j / 128].
  * Rows behind the last sequence, and every token not written, stay as they
- * were.  Two rows of one call must not share a (page, slot): distinct
- * sequences write distinct pages. */
+ * were.  Sequences of one call write distinct pages, and calls that write to
+ * the same page do not overlap. */
 EOSLLM_CUDA_API int eosi_cuda_kv_q8_write_dev(const eosi_cuda_kv_q8_t *kv, const float *k, const float *v,
                                               uint64_t row_stride, uint32_t n_rows, const uint32_t *row0,
                                               const uint32_t *table, uint32_t table_stride, const uint32_t *pos,
