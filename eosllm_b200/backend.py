@@ -122,6 +122,12 @@ _SIGNATURES = {
     "eosi_cuda_text_attach_local": (C.c_int, [_vp, C.c_int]),
     "eosi_cuda_text_set_wait_limit": (C.c_int, [_vp, _u32]),
     "eosi_cuda_text_partition": (C.c_int, [_vp, C.c_int, C.c_int, _vp]),
+    "eosi_cuda_text_set_cache": (C.c_int, [_vp, C.c_int]),
+    "eosi_cuda_text_cache": (C.c_int, [_vp]),
+    "eosi_cuda_text_fork": (C.c_int, [_vp, _u32, _u32, _u32]),
+    "eosi_cuda_text_branch_step": (C.c_int, [_vp, _vp, _u32, _vp, _vp, C.c_float, _vp, _vp]),
+    "eosi_cuda_text_branch_adopt": (C.c_int, [_vp, _u32]),
+    "eosi_cuda_text_branch_close": (C.c_int, [_vp]),
     "eosi_cuda_text_close": (None, [_vp]),
 }
 

@@ -60,6 +60,7 @@
 #include "eos_common.cuh"
 #include "eos_kernels.h"
 #include "eosllm_cuda.h"
+#include "kv_q8.cuh"
 
 namespace eos {
 
@@ -734,6 +735,44 @@ struct TextDecoder {
   std::vector<void*> pf_wres;
   bool pf_resident = true;  // allow pf_wres (eosi_cuda_text_set_prefill_resident)
   uint32_t prefill_min = 16;
+  // 8-bit cache mode (eosi_cuda_text_set_cache; one GPU, per-op step): per
+  // layer a pool of q8_pages pages, position j in page j / 128, instead of
+  // kc / vc
+  bool q8 = false;
+  uint32_t q8_pages = 0;
+  size_t q8_layer = 0;           // bytes of a layer's pool
+  uint8_t* q8_pool = nullptr;
+  uint32_t* q8_table = nullptr;  // 0, 1, 2, ...
+  uint32_t* q8_words = nullptr;  // {position, length} of the pass
+  float* q8_attn = nullptr;      // attention outputs of a pass
+  void* q8_scratch = nullptr;
+  // branches (eosi_cuda_text_fork): sequences that continue the tokens fed so
+  // far.  The shared prefix is the whole pages of the main cache; each
+  // sequence's own pages (per layer, br.pages of them per sequence) start with
+  // a copy of the main cache's last, partly filled page.
+  struct Branches {
+    uint32_t n = 0, max_new = 0, max_draft = 0, pages = 0;
+    uint32_t full = 0, rem = 0;      // shared tokens (whole pages); tokens copied behind them
+    size_t layer = 0;                // bytes of a layer's own pages
+    uint8_t* pool = nullptr;
+    uint32_t* words = nullptr;       // device words, see branch_step
+    float *probs = nullptr, *q = nullptr, *u = nullptr;
+    void* scratch = nullptr;
+    std::vector<uint32_t> len;       // tokens of each sequence behind the shared ones
+    std::vector<uint32_t> host;      // the words' host copy
+  } br;
+  void* wout_pf = nullptr;  // LM head in the GEMM layout (prepared by the first fork)
+
+  template <typename T>
+  void release(T*& p) {
+    for (size_t i = 0; i < allocs.size(); ++i)
+      if (allocs[i] == (void*)p) {
+        allocs.erase(allocs.begin() + i);
+        break;
+      }
+    if (p) cudaFree((void*)p);
+    p = nullptr;
+  }
 
   template <typename T>
   cudaError_t alloc(T** p, size_t bytes) {
@@ -775,6 +814,44 @@ struct TextDecoder {
   cudaError_t record_step_persistent(cudaStream_t s);
   int capture();
   int set_step_mode(int mode);
+  KvPool q8_at(uint32_t L) const { return KvPool{q8_pool + (size_t)L * q8_layer, q8_pages, kvl, hd}; }
+  KvPool br_at(uint32_t L) const { return KvPool{br.pool + (size_t)L * br.layer, br.n * br.pages, kvl, hd}; }
+  uint32_t pass_rows() const { return m.max_ctx < kPrefillRows ? m.max_ctx : kPrefillRows; }
+  cudaError_t prefill_buffers();
+  void prefill_matrix(uint32_t L, int i, uint32_t& n, uint32_t& k, const uint8_t** w) const;
+  void prefill_weights();
+  cudaError_t prefill_gemm(uint32_t L, int i, const void* act, float* c, uint32_t mm, bool acc, uint32_t ldc = 0,
+                           float* const* extra = nullptr, uint32_t n_extra = 0);
+  int set_cache(int mode);
+  int fork(uint32_t n, uint32_t max_new, uint32_t max_draft);
+  void close_branches();
+  cudaError_t branch_pass(uint32_t per_seq, float temperature);
+  // attention of a pass over the 8-bit cache
+  KvAttnBatch q8_batch(uint32_t rows) const {
+    KvAttnBatch b{};
+    b.table = q8_table;
+    b.seq_len = q8_words + 1;
+    b.table_stride = q8_pages;
+    b.max_len = m.max_ctx;
+    b.n_seq = 1;
+    b.n_rows = b.max_rows = rows;
+    return b;
+  }
+  KvAttnBatch br_batch(uint32_t per_seq, const KvPool* shared) const {
+    KvAttnBatch b{};
+    b.prefix_table = br.full ? q8_table : nullptr;
+    b.prefix_len = br.full ? br.words : nullptr;
+    b.max_prefix = br.full;
+    b.prefix_pool = shared;
+    b.table = br.words + 1u + 3u * br.n;
+    b.table_stride = br.pages;
+    b.seq_len = br.words + 1u + 2u * br.n;
+    b.max_len = br.rem + br.max_new;
+    b.n_seq = br.n;
+    b.n_rows = br.n * per_seq;
+    b.max_rows = per_seq;
+    return b;
+  }
 };
 
 // The slice of the model rank rk of ws owns: heads [h0, h0 + hl) (and their
@@ -1086,7 +1163,18 @@ cudaError_t TextDecoder::record_step(cudaStream_t s) {
     e = norm_pack(L == 0 ? nullptr : x0, L == 0 ? nullptr : d_full, x1, d.attn_norm, wdt, xoff_d,
                   L == 0 ? 0u : 4u * L - 1u);
     if (e == cudaSuccess) e = gemv(wdt, d.wqkv, act_e, actf_e, qkv, nqkv, E);
-    if (e == cudaSuccess) {
+    if (q8) {  // rotate, append to the 8-bit cache, attend, pack for the O projection
+      const KvPool pool = q8_at(L);
+      const KvRowSet row{nullptr, q8_table, &state->pos, 1u, 1u, q8_pages};
+      float* out = wdt == EOS_DT_Q4_K ? q8_attn : actf_o;
+      if (e == cudaSuccess) e = launch_rope_rows(qkv, 1, 1, hl, kvl, hd, &state->pos, m.rope_base, q8_words + 1, s);
+      if (e == cudaSuccess)
+        e = launch_kv_write(pool, row, qkv + hl * hd, qkv + (hl + kvl) * hd, nqkv, gemv_err, s);
+      if (e == cudaSuccess)
+        e = launch_kv_attn(pool, q8_batch(1), qkv, nqkv, out, E, m.n_head, 1.0f / sqrtf((float)hd), q8_scratch,
+                           num_sms, gemv_err, s);
+      if (e == cudaSuccess && wdt == EOS_DT_Q4_K) e = launch_act_pack(out, 1, E, act_o, EOS_ACT_LAYOUT_GEMV, s);
+    } else if (e == cudaSuccess) {
       AttnParams a{};
       a.qkv = qkv;
       a.kc = kc + (size_t)L * m.max_ctx * kvl * hd;
@@ -1236,6 +1324,10 @@ int TextDecoder::set_step_mode(int mode) {
     set_error_message("cuda text: unknown step mode");
     return EOS_E_INVALID_ARG;
   }
+  if (mode == EOSI_CUDA_STEP_PERSISTENT && q8) {
+    set_error_message("cuda text: the persistent step reads the f32 cache");
+    return EOS_E_UNSUPPORTED;
+  }
   if (mode == EOSI_CUDA_STEP_PERSISTENT && !persistent_ok) {
     set_error_message("cuda text: the persistent step needs Q4_K linears and LM head, head_dim 64 or 128 and "
                       "n_embd <= 4096, with its shared memory on this device");
@@ -1261,23 +1353,67 @@ int TextDecoder::set_step_mode(int mode) {
   return capture();
 }
 
-// Batched prefill of the n tokens at prompt[host_pos ...]: per block of up to
-// pf_rows tokens and per layer, the block's rows go through the GEMMs and
-// the prefill kernels, which write their K/V rows into the cache; the next
-// block attends to them.  Only the cache matters afterwards (the next step
-// reads it), so the last layer stops after its K/V rows and no block computes
-// logits.  Tensor parallel, the matrices are split by output rows as in the
-// step: each rank packs its heads' attention output and its FFN units'
-// SiLU output into every rank's copy of the next GEMM's operand, and pushes
-// its O / down output rows into every rank's row buffer, which the exchange
-// kernel then adds to the residual rows -- so every rank holds the one-GPU
-// residual stream bit for bit.  Leaves state->pos = host_pos + n (not
-// host_pos itself: the caller commits it after its synchronisation).
-cudaError_t TextDecoder::prefill(uint32_t n) {
+// Matrix i of a layer -- qkv, O, gate | up, down -- its shape and rows.
+void TextDecoder::prefill_matrix(uint32_t L, int i, uint32_t& n, uint32_t& k, const uint8_t** w) const {
+  const DecLayer& d = layers[L];
+  n = i == 0 ? hl * hd + 2u * kvl * hd : (i == 2 ? 2u * ffl : el);
+  k = i == 3 ? m.n_ff : m.n_embd;
+  *w = i == 0 ? d.wqkv : (i == 1 ? d.wo : (i == 2 ? d.wgu : d.wd));
+}
+
+// Every layer's matrices in the GEMM layout, where they fit (pf_wres).
+void TextDecoder::prefill_weights() {
+  if (!pf_wres.empty() || !pf_resident) return;
+  uint32_t n = 0, k = 0;
+  const uint8_t* w = nullptr;
+  size_t need = 0;
+  for (int i = 0; i < 4 && m.n_layer > 0; ++i) {
+    prefill_matrix(0, i, n, k, &w);
+    need += prefill_operand_bytes(n, k);
+  }
+  need *= m.n_layer;
+  size_t free_b = 0, total_b = 0;
+  if (cudaMemGetInfo(&free_b, &total_b) != cudaSuccess || need > free_b / 2) return;
+  std::vector<void*> res(4u * m.n_layer, nullptr);
+  cudaError_t r = cudaSuccess;
+  for (uint32_t L = 0; L < m.n_layer && r == cudaSuccess; ++L)
+    for (int i = 0; i < 4 && r == cudaSuccess; ++i) {
+      prefill_matrix(L, i, n, k, &w);
+      r = cudaMalloc(&res[4u * L + i], prefill_operand_bytes(n, k));
+      if (r == cudaSuccess) r = launch_prefill_w_prep(w, n, k, res[4u * L + i], st);
+    }
+  if (r == cudaSuccess) {
+    pf_wres = res;
+    for (void* q : res) allocs.push_back(q);
+  } else {
+    for (void* q : res)
+      if (q) cudaFree(q);
+    cudaGetLastError();  // not fatal: prepare per layer instead
+  }
+}
+
+// C (+)= act . deq(W)^T with W resident in the GEMM layout, or prepared on the
+// fly; rows of C ldc floats apart, pushed into `extra` too.
+cudaError_t TextDecoder::prefill_gemm(uint32_t L, int i, const void* act, float* c, uint32_t mm, bool acc,
+                                      uint32_t ldc, float* const* extra, uint32_t n_extra) {
+  uint32_t n = 0, k = 0;
+  const uint8_t* w = nullptr;
+  prefill_matrix(L, i, n, k, &w);
+  const bool res = pf_resident && !pf_wres.empty();
+  const void* wp = res ? pf_wres[4u * L + i] : pf_w;
+  cudaError_t e = res ? cudaSuccess : launch_prefill_w_prep(w, n, k, pf_w, st);
+  int status = EOS_OK;
+  if (e == cudaSuccess)
+    e = launch_prefill_gemm(act, wp, c, mm, n, k, gemv_err, st, &status, acc, extra, n_extra, ldc);
+  return e == cudaSuccess && status != EOS_OK ? cudaErrorNotSupported : e;
+}
+
+// Scratch of a batched pass, allocated at first use.
+cudaError_t TextDecoder::prefill_buffers() {
   const uint32_t E = m.n_embd, F = m.n_ff, nqkv = hl * hd + 2u * kvl * hd;
   cudaError_t e = cudaSuccess;
   if (pf_rows == 0) {
-    const uint32_t rows = m.max_ctx < kPrefillRows ? m.max_ctx : kPrefillRows;
+    const uint32_t rows = pass_rows();
     // the operand size grows with the row count: `rows` bounds every block
     size_t amax = 0;
     for (const uint32_t kk : {E, F})
@@ -1294,46 +1430,29 @@ cudaError_t TextDecoder::prefill(uint32_t n) {
     if (e != cudaSuccess) return e;
     pf_rows = rows;
   }
-  int status = EOS_OK;
-  const uint32_t mat_n[4] = {nqkv, el, 2u * ffl, el}, mat_k[4] = {E, E, E, F};  // qkv, o, gate|up, down
-  auto mat_w = [&](uint32_t L, int i) -> const uint8_t* {
-    const DecLayer& d = layers[L];
-    return i == 0 ? d.wqkv : (i == 1 ? d.wo : (i == 2 ? d.wgu : d.wd));
-  };
-  if (pf_wres.empty() && pf_resident) {
-    size_t need = 0;
-    for (int i = 0; i < 4; ++i) need += prefill_operand_bytes(mat_n[i], mat_k[i]);
-    need *= m.n_layer;
-    size_t free_b = 0, total_b = 0;
-    if (cudaMemGetInfo(&free_b, &total_b) == cudaSuccess && need <= free_b / 2) {
-      std::vector<void*> res(4u * m.n_layer, nullptr);
-      cudaError_t r = cudaSuccess;
-      for (uint32_t L = 0; L < m.n_layer && r == cudaSuccess; ++L)
-        for (int i = 0; i < 4 && r == cudaSuccess; ++i) {
-          r = cudaMalloc(&res[4u * L + i], prefill_operand_bytes(mat_n[i], mat_k[i]));
-          if (r == cudaSuccess) r = launch_prefill_w_prep(mat_w(L, i), mat_n[i], mat_k[i], res[4u * L + i], st);
-        }
-      if (r == cudaSuccess) {
-        pf_wres = res;
-        for (void* q : res) allocs.push_back(q);
-      } else {
-        for (void* q : res)
-          if (q) cudaFree(q);
-        cudaGetLastError();  // not fatal: prepare per layer instead
-      }
-    }
-  }
-  // C (+)= act . deq(W)^T with W resident in the GEMM layout, or prepared on
-  // the fly; rows of C ldc floats apart, pushed into `extra` too
+  return e;
+}
+
+// Batched prefill of the n tokens at prompt[host_pos ...]: per block of up to
+// pf_rows tokens and per layer, the block's rows go through the GEMMs and
+// the prefill kernels, which write their K/V rows into the cache; the next
+// block attends to them.  Only the cache matters afterwards (the next step
+// reads it), so the last layer stops after its K/V rows and no block computes
+// logits.  Tensor parallel, the matrices are split by output rows as in the
+// step: each rank packs its heads' attention output and its FFN units'
+// SiLU output into every rank's copy of the next GEMM's operand, and pushes
+// its O / down output rows into every rank's row buffer, which the exchange
+// kernel then adds to the residual rows -- so every rank holds the one-GPU
+// residual stream bit for bit.  Leaves state->pos = host_pos + n (not
+// host_pos itself: the caller commits it after its synchronisation).
+cudaError_t TextDecoder::prefill(uint32_t n) {
+  const uint32_t E = m.n_embd, F = m.n_ff, nqkv = hl * hd + 2u * kvl * hd;
+  cudaError_t e = prefill_buffers();
+  if (e != cudaSuccess) return e;
+  prefill_weights();
   auto gemm = [&](uint32_t L, int i, const void* act, float* c, uint32_t mm, bool acc, uint32_t ldc = 0,
                   float* const* extra = nullptr, uint32_t n_extra = 0) {
-    const uint32_t nn = mat_n[i], kk = mat_k[i];
-    const bool res = pf_resident && !pf_wres.empty();
-    const void* wp = res ? pf_wres[4u * L + i] : pf_w;
-    if (e == cudaSuccess && !res) e = launch_prefill_w_prep(mat_w(L, i), nn, kk, pf_w, st);
-    if (e == cudaSuccess)
-      e = launch_prefill_gemm(act, wp, c, mm, nn, kk, gemv_err, st, &status, acc, extra, n_extra, ldc);
-    if (e == cudaSuccess && status != EOS_OK) e = cudaErrorNotSupported;
+    if (e == cudaSuccess) e = prefill_gemm(L, i, act, c, mm, acc, ldc, extra, n_extra);
   };
   // tensor parallel: the other ranks' copies of the O / down output rows and
   // of the O / down operands
@@ -1370,16 +1489,34 @@ cudaError_t TextDecoder::prefill(uint32_t n) {
   for (uint32_t b0 = 0; b0 < n && e == cudaSuccess; b0 += pf_rows) {
     const uint32_t mm = (n - b0) < pf_rows ? (n - b0) : pf_rows;
     const uint32_t pos0 = host_pos + b0;
+    if (q8) {  // {position of the block's first row, tokens with it}
+      const uint32_t words[2] = {pos0, pos0 + mm};
+      e = cudaMemcpyAsync(q8_words, words, sizeof(words), cudaMemcpyHostToDevice, st);
+    }
     for (uint32_t L = 0; L < m.n_layer && e == cudaSuccess; ++L) {
       const DecLayer& d = layers[L];
-      float* kcl = kc + (size_t)L * m.max_ctx * kvl * hd;
-      float* vcl = vc + (size_t)L * m.max_ctx * kvl * hd;
-      e = launch_pf_norm_pack(pf_x, L == 0 ? prompt + pos0 : nullptr, tok_embd, d.attn_norm, m.rms_eps, mm, E,
+      float* kcl = q8 ? nullptr : kc + (size_t)L * m.max_ctx * kvl * hd;
+      float* vcl = q8 ? nullptr : vc + (size_t)L * m.max_ctx * kvl * hd;
+      if (e == cudaSuccess)
+        e = launch_pf_norm_pack(pf_x, L == 0 ? prompt + pos0 : nullptr, tok_embd, d.attn_norm, m.rms_eps, mm, E,
                               pf_act, st);
       gemm(L, 0, pf_act, pf_qkv, mm, false);
-      if (e == cudaSuccess) e = launch_pf_rope_kv(pf_qkv, kcl, vcl, mm, hl, kvl, hd, pos0, m.rope_base, st);
+      if (q8) {
+        const KvRowSet set{nullptr, q8_table, q8_words, mm, 1u, q8_pages};
+        if (e == cudaSuccess)
+          e = launch_rope_rows(pf_qkv, mm, mm, hl, kvl, hd, q8_words, m.rope_base, nullptr, st);
+        if (e == cudaSuccess)
+          e = launch_kv_write(q8_at(L), set, pf_qkv + hl * hd, pf_qkv + (hl + kvl) * hd, nqkv, gemv_err, st);
+      } else if (e == cudaSuccess) {
+        e = launch_pf_rope_kv(pf_qkv, kcl, vcl, mm, hl, kvl, hd, pos0, m.rope_base, st);
+      }
       if (L + 1u == m.n_layer) break;  // the cache needs nothing more of the last layer
-      if (e == cudaSuccess)
+      if (q8) {
+        if (e == cudaSuccess)
+          e = launch_kv_attn(q8_at(L), q8_batch(mm), pf_qkv, nqkv, q8_attn, E, m.n_head, scale, q8_scratch, num_sms,
+                             gemv_err, st);
+        if (e == cudaSuccess) e = launch_prefill_act_pack(q8_attn, mm, E, op_o, st);
+      } else if (e == cudaSuccess)
         e = launch_pf_attn(pf_qkv, kcl, vcl, op_o, mm, hl, kvl, h0, kv0, m.n_head, m.n_kv_head, hd, pos0, scale,
                            E, push_op[0], np, st);
       if (world == 1) {
@@ -1402,6 +1539,201 @@ cudaError_t TextDecoder::prefill(uint32_t n) {
       }
     }
   }
+  return e;
+}
+
+// f32 or 8-bit cache, at position 0 (nothing cached yet); re-records the step.
+int TextDecoder::set_cache(int mode) {
+  if (mode != EOSI_CUDA_CACHE_F32 && mode != EOSI_CUDA_CACHE_Q8) {
+    set_error_message("cuda text: unknown cache mode");
+    return EOS_E_INVALID_ARG;
+  }
+  if (host_pos != 0 || br.n != 0) {
+    set_error_message("cuda text: the cache can only be changed at position 0");
+    return EOS_E_INVALID_ARG;
+  }
+  const bool want = mode == EOSI_CUDA_CACHE_Q8;
+  if (want && world > 1) {
+    set_error_message("cuda text: the 8-bit cache needs the whole model on one GPU");
+    return EOS_E_UNSUPPORTED;
+  }
+  if (want && persistent) {
+    set_error_message("cuda text: the persistent step reads the f32 cache");
+    return EOS_E_UNSUPPORTED;
+  }
+  if (want == q8) return EOS_OK;
+  if (cudaSetDevice(device) != cudaSuccess) return EOS_E_INTERNAL;
+  cudaError_t e = cudaStreamSynchronize(st);
+  const uint32_t pages = (m.max_ctx + kKvPage - 1u) / kKvPage;
+  const size_t layer = (size_t)pages * kvl * kv_block_bytes(hd);
+  const size_t kv_bytes = 4ull * m.n_layer * m.max_ctx * kvl * hd;
+  if (want) {  // the new cache first: a failure leaves the decoder as it was
+    q8_pages = pages;
+    q8_layer = layer;
+    size_t scratch = 0;  // of a step and of every prefill block (few rows are split otherwise than many)
+    for (uint32_t rows : {1u, 2u, 3u, 4u, 5u, pass_rows()}) {
+      const size_t b = kv_attn_scratch_bytes(q8_at(0), q8_batch(rows), m.n_head);
+      scratch = b > scratch ? b : scratch;
+    }
+    if (e == cudaSuccess) e = alloc(&q8_pool, layer * m.n_layer);
+    if (e == cudaSuccess) e = alloc(&q8_table, 4ull * pages);
+    if (e == cudaSuccess) e = alloc(&q8_words, 16);
+    if (e == cudaSuccess) e = alloc(&q8_attn, 4ull * m.n_embd * (prefill_ok() ? pass_rows() : 1u));
+    if (e == cudaSuccess) e = alloc(&q8_scratch, scratch);
+    std::vector<uint32_t> id(pages);
+    for (uint32_t i = 0; i < pages; ++i) id[i] = i;
+    if (e == cudaSuccess) e = cudaMemcpyAsync(q8_table, id.data(), 4ull * pages, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  } else {
+    if (e == cudaSuccess) e = alloc(&kc, kv_bytes);
+    if (e == cudaSuccess) e = alloc(&vc, kv_bytes);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  // the cache no longer wanted, or the one that could not be set up
+  if ((e == cudaSuccess) == want) {
+    release(kc);
+    release(vc);
+  } else {
+    release(q8_pool);
+    release(q8_table);
+    release(q8_words);
+    release(q8_attn);
+    release(q8_scratch);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error_message(cudaGetErrorString(e));
+    return e == cudaErrorMemoryAllocation ? EOS_E_OUT_OF_MEMORY : EOS_E_INTERNAL;
+  }
+  q8 = want;
+  if (graph) cudaGraphExecDestroy(graph);
+  graph = nullptr;
+  return capture();
+}
+
+void TextDecoder::close_branches() {
+  if (br.n == 0) return;
+  cudaStreamSynchronize(st);
+  release(br.pool);
+  release(br.words);
+  release(br.probs);
+  release(br.q);
+  release(br.u);
+  release(br.scratch);
+  br = Branches();
+}
+
+// Words of the branches in device memory, n sequences, k = per_seq rows each:
+//   [0] shared tokens; [1, n] position of each sequence's first row; [1 + n, 2n]
+//   the same within its own pages; [1 + 2n, 3n] its own tokens with the new
+//   rows; then the page table [n][pages], the rows' tokens [n k], the drafts
+//   [n (k - 1)], and, written by the verification, the tokens [n k] and their
+//   number [n].
+int TextDecoder::fork(uint32_t n, uint32_t max_new, uint32_t max_draft) {
+  if (!q8) {
+    set_error_message("cuda text: branches need the 8-bit cache (eosi_cuda_text_set_cache)");
+    return EOS_E_UNSUPPORTED;
+  }
+  if (!prefill_ok() || m.out_dtype != EOS_DT_Q4_K) {
+    set_error_message("cuda text: branches need Q4_K linears and LM head");
+    return EOS_E_UNSUPPORTED;
+  }
+  if (br.n != 0) {
+    set_error_message("cuda text: branches are open already");
+    return EOS_E_INVALID_ARG;
+  }
+  if (n == 0 || n > EOS_ATTN_MAX_SEQ || max_new == 0 || max_draft >= pass_rows() ||
+      (uint64_t)n * (max_draft + 1u) > pass_rows()) {
+    set_error_message("cuda text: a pass holds at most min(max_ctx, 1024) rows, n_seq * (max_draft + 1) of them");
+    return EOS_E_INVALID_ARG;
+  }
+  if ((uint64_t)host_pos + max_new > m.max_ctx) {
+    set_error_message("cuda text: branches exceed the context");
+    return EOS_E_OUT_OF_MEMORY;
+  }
+  if (cudaSetDevice(device) != cudaSuccess) return EOS_E_INTERNAL;
+  const uint32_t E = m.n_embd, V = m.n_vocab, k = max_draft + 1u;
+  br.n = n;
+  br.max_new = max_new;
+  br.max_draft = max_draft;
+  br.full = host_pos / kKvPage * kKvPage;
+  br.rem = host_pos - br.full;
+  br.pages = (br.rem + max_new + kKvPage - 1u) / kKvPage;
+  const size_t page = (size_t)kvl * kv_block_bytes(hd);
+  br.layer = page * br.pages * n;
+  br.len.assign(n, br.rem);
+  const size_t words = 1u + 3ull * n + (size_t)n * br.pages + 3ull * n * k + n;
+  br.host.assign(words, 0u);
+  const KvPool shared = q8_at(0);
+  cudaError_t e = prefill_buffers();
+  if (e == cudaSuccess) prefill_weights();
+  if (e == cudaSuccess) e = alloc(&br.pool, br.layer * m.n_layer);
+  if (e == cudaSuccess) e = alloc(&br.words, 4u * words);
+  if (e == cudaSuccess) e = alloc(&br.probs, 4ull * n * k * V);
+  if (e == cudaSuccess) e = alloc(&br.q, 4ull * n * max_draft * V);
+  if (e == cudaSuccess) e = alloc(&br.u, 4ull * n * k);
+  if (e == cudaSuccess) {
+    // the scratch of the widest pass (its size does not shrink with the rows' number in every split)
+    size_t need = 0;
+    for (uint32_t r = 1; r <= k; ++r) {
+      const size_t b = kv_attn_scratch_bytes(br_at(0), br_batch(r, &shared), m.n_head);
+      need = b > need ? b : need;
+    }
+    e = alloc(&br.scratch, need);
+  }
+  if (e == cudaSuccess && wout_pf == nullptr) {
+    e = alloc(&wout_pf, prefill_operand_bytes(V, E));
+    if (e == cudaSuccess) e = launch_prefill_w_prep(wout, V, E, wout_pf, st);
+  }
+  // the last, partly filled page of the main cache into every sequence
+  for (uint32_t L = 0; L < m.n_layer && br.rem > 0 && e == cudaSuccess; ++L)
+    for (uint32_t i = 0; i < n && e == cudaSuccess; ++i)
+      e = cudaMemcpyAsync(br_at(L).pages + page * br.pages * i, q8_at(L).pages + page * (br.full / kKvPage), page,
+                          cudaMemcpyDeviceToDevice, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    close_branches();
+    set_error_message(cudaGetErrorString(e));
+    return e == cudaErrorMemoryAllocation ? EOS_E_OUT_OF_MEMORY : EOS_E_INTERNAL;
+  }
+  return EOS_OK;
+}
+
+// One pass of per_seq rows of every branch: their keys and values into the own
+// pages, and the probabilities of every row into br.probs.
+cudaError_t TextDecoder::branch_pass(uint32_t per_seq, float temperature) {
+  const uint32_t E = m.n_embd, V = m.n_vocab, n = br.n, mm = n * per_seq, nqkv = hl * hd + 2u * kvl * hd;
+  const uint32_t* tokens = br.words + 1u + 3u * n + (size_t)n * br.pages;
+  const float scale = 1.0f / sqrtf((float)hd);  // text.c:365
+  cudaError_t e = cudaSuccess;
+  auto run = [&](cudaError_t r) {
+    if (e == cudaSuccess) e = r;
+  };
+  for (uint32_t L = 0; L < m.n_layer && e == cudaSuccess; ++L) {
+    const DecLayer& d = layers[L];
+    const KvPool own = br_at(L), shared = q8_at(L);
+    const KvRowSet set{nullptr, br.words + 1u + 3u * n, br.words + 1u + n, mm, n, br.pages};
+    run(launch_pf_norm_pack(pf_x, L == 0 ? tokens : nullptr, tok_embd, d.attn_norm, m.rms_eps, mm, E, pf_act, st));
+    if (e == cudaSuccess) run(prefill_gemm(L, 0, pf_act, pf_qkv, mm, false));
+    if (e == cudaSuccess) run(launch_rope_rows(pf_qkv, mm, per_seq, hl, kvl, hd, br.words + 1, m.rope_base, nullptr, st));
+    if (e == cudaSuccess)
+      run(launch_kv_write(own, set, pf_qkv + hl * hd, pf_qkv + (hl + kvl) * hd, nqkv, gemv_err, st));
+    if (e == cudaSuccess)
+      run(launch_kv_attn(own, br_batch(per_seq, &shared), pf_qkv, nqkv, q8_attn, E, m.n_head, scale, br.scratch,
+                         num_sms, gemv_err, st));
+    if (e == cudaSuccess) run(launch_prefill_act_pack(q8_attn, mm, E, pf_act, st));
+    if (e == cudaSuccess) run(prefill_gemm(L, 1, pf_act, pf_x, mm, true));
+    if (e == cudaSuccess) run(launch_pf_norm_pack(pf_x, nullptr, tok_embd, d.ffn_norm, m.rms_eps, mm, E, pf_act, st));
+    if (e == cudaSuccess) run(prefill_gemm(L, 2, pf_act, pf_gu, mm, false));
+    if (e == cudaSuccess) run(launch_pf_silu_pack(pf_gu, mm, ffl, pf_act, ff0, m.n_ff, nullptr, 0, st));
+    if (e == cudaSuccess) run(prefill_gemm(L, 3, pf_act, pf_x, mm, true));
+  }
+  int status = EOS_OK;
+  if (e == cudaSuccess) run(launch_pf_norm_pack(pf_x, nullptr, tok_embd, out_norm, m.rms_eps, mm, E, pf_act, st));
+  if (e == cudaSuccess) run(eos::launch_prefill_gemm(pf_act, wout_pf, br.probs, mm, V, E, gemv_err, st, &status));
+  if (e == cudaSuccess && status != EOS_OK) e = cudaErrorNotSupported;
+  if (e == cudaSuccess) run(launch_logit_probs(br.probs, mm, V, temperature, st));
   return e;
 }
 
@@ -1512,6 +1844,10 @@ EOSLLM_CUDA_API int eosi_cuda_text_open(const eosi_cuda_llama_t* m, int device, 
 EOSLLM_CUDA_API int eosi_cuda_text_step(eosi_cuda_text_t* t, uint32_t token, float* logits) {
   if (t == nullptr || logits == nullptr) return EOS_E_INVALID_ARG;
   TextDecoder& d = t->d;
+  if (d.br.n != 0) {
+    eos::set_error_message("cuda text: branches are open (adopt or close them first)");
+    return EOS_E_INVALID_ARG;
+  }
   if (token >= d.m.n_vocab) {  // text.c:277
     eos::set_error_message("cuda text: token id out of range");
     return EOS_E_INVALID_ARG;
@@ -1551,6 +1887,10 @@ EOSLLM_CUDA_API int eosi_cuda_text_generate(eosi_cuda_text_t* t, const uint32_t*
   if (t == nullptr || prompt == nullptr || n_prompt == 0 || (n_gen > 0 && out_tokens == nullptr))
     return EOS_E_INVALID_ARG;
   TextDecoder& d = t->d;
+  if (d.br.n != 0) {
+    eos::set_error_message("cuda text: branches are open (adopt or close them first)");
+    return EOS_E_INVALID_ARG;
+  }
   if (d.graph == nullptr) {
     eos::set_error_message("cuda text: tensor-parallel decoder not attached to its peers");
     return EOS_E_INVALID_ARG;
@@ -1592,6 +1932,10 @@ EOSLLM_CUDA_API int eosi_cuda_text_generate(eosi_cuda_text_t* t, const uint32_t*
 EOSLLM_CUDA_API int eosi_cuda_text_prefill(eosi_cuda_text_t* t, const uint32_t* tokens, uint32_t n) {
   if (t == nullptr || (tokens == nullptr && n > 0)) return EOS_E_INVALID_ARG;
   TextDecoder& d = t->d;
+  if (d.br.n != 0) {
+    eos::set_error_message("cuda text: branches are open (adopt or close them first)");
+    return EOS_E_INVALID_ARG;
+  }
   if (!d.prefill_ok()) {
     eos::set_error_message("cuda text: batched prefill needs Q4_K linears");
     return EOS_E_UNSUPPORTED;
@@ -1637,6 +1981,7 @@ EOSLLM_CUDA_API int eosi_cuda_text_reset(eosi_cuda_text_t* t) {
   if (t == nullptr) return EOS_E_INVALID_ARG;
   TextDecoder& d = t->d;
   if (cudaSetDevice(d.device) != cudaSuccess) return EOS_E_INTERNAL;
+  d.close_branches();
   // position, prompt length, pick, argmax count and error word; the exchange
   // epoch keeps counting (the peers' flags hold earlier epochs)
   cudaError_t e = cudaMemsetAsync(d.state, 0, offsetof(eos::DecState, epoch), d.st);
@@ -1729,6 +2074,115 @@ EOSLLM_CUDA_API int eosi_cuda_text_set_step_mode(eosi_cuda_text_t* t, int mode) 
 EOSLLM_CUDA_API int eosi_cuda_text_step_mode(const eosi_cuda_text_t* t) {
   if (t == nullptr) return 0;
   return t->d.persistent ? EOSI_CUDA_STEP_PERSISTENT : EOSI_CUDA_STEP_PER_OP;
+}
+
+EOSLLM_CUDA_API int eosi_cuda_text_set_cache(eosi_cuda_text_t* t, int mode) {
+  return t ? t->d.set_cache(mode) : EOS_E_INVALID_ARG;
+}
+
+EOSLLM_CUDA_API int eosi_cuda_text_cache(const eosi_cuda_text_t* t) {
+  return t && t->d.q8 ? EOSI_CUDA_CACHE_Q8 : EOSI_CUDA_CACHE_F32;
+}
+
+EOSLLM_CUDA_API int eosi_cuda_text_fork(eosi_cuda_text_t* t, uint32_t n_seq, uint32_t max_new, uint32_t max_draft) {
+  return t ? t->d.fork(n_seq, max_new, max_draft) : EOS_E_INVALID_ARG;
+}
+
+EOSLLM_CUDA_API int eosi_cuda_text_branch_step(eosi_cuda_text_t* t, const uint32_t* tokens, uint32_t n_draft,
+                                               const float* draft_probs, const float* u, float temperature,
+                                               uint32_t* out_tokens, uint32_t* n_out) {
+  if (t == nullptr || tokens == nullptr || u == nullptr || out_tokens == nullptr || n_out == nullptr)
+    return EOS_E_INVALID_ARG;
+  TextDecoder& d = t->d;
+  auto& b = d.br;
+  const uint32_t n = b.n, k = n_draft + 1u, V = d.m.n_vocab;
+  if (n == 0 || n_draft > b.max_draft) {
+    eos::set_error_message(n == 0 ? "cuda text: no branches are open" : "cuda text: more drafts than the fork allows");
+    return EOS_E_INVALID_ARG;
+  }
+  if (!(temperature >= 0.0f) || !std::isfinite(temperature)) {
+    eos::set_error_message("cuda text: temperature must be finite and not negative");
+    return EOS_E_INVALID_ARG;
+  }
+  for (uint32_t i = 0; i < n * k; ++i)
+    if (tokens[i] >= V || !(u[i] >= 0.0f && u[i] < 1.0f)) {
+      eos::set_error_message(tokens[i] >= V ? "cuda text: token id out of range" : "cuda text: random numbers must be in [0, 1)");
+      return EOS_E_INVALID_ARG;
+    }
+  for (uint32_t i = 0; i < n; ++i)
+    if (b.len[i] + k > b.rem + b.max_new) {
+      eos::set_error_message("cuda text: a branch is full");
+      return EOS_E_OUT_OF_MEMORY;
+    }
+  if (cudaSetDevice(d.device) != cudaSuccess) return EOS_E_INTERNAL;
+  uint32_t* w = b.host.data();
+  const size_t at_table = 1u + 3ull * n, at_tokens = at_table + (size_t)n * b.pages, at_drafts = at_tokens + (size_t)n * k,
+               at_out = at_drafts + (size_t)n * n_draft, at_count = at_out + (size_t)n * k;
+  w[0] = b.full;
+  for (uint32_t i = 0; i < n; ++i) {
+    w[1u + i] = b.full + b.len[i];
+    w[1u + n + i] = b.len[i];
+    w[1u + 2u * n + i] = b.len[i] + k;
+    for (uint32_t p = 0; p < b.pages; ++p) w[at_table + (size_t)i * b.pages + p] = i * b.pages + p;
+    memcpy(w + at_tokens + (size_t)i * k, tokens + (size_t)i * k, 4ull * k);
+    memcpy(w + at_drafts + (size_t)i * n_draft, tokens + (size_t)i * k + 1u, 4ull * n_draft);
+  }
+  cudaError_t e = cudaMemcpyAsync(b.words, w, 4ull * at_out, cudaMemcpyHostToDevice, d.st);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(b.u, u, 4ull * n * k, cudaMemcpyHostToDevice, d.st);
+  if (e == cudaSuccess && n_draft > 0) {
+    if (draft_probs != nullptr)
+      e = cudaMemcpyAsync(b.q, draft_probs, 4ull * n * n_draft * V, cudaMemcpyHostToDevice, d.st);
+    else
+      e = eos::launch_one_hot(b.q, b.words + at_drafts, n * n_draft, V, d.st);
+  }
+  if (e == cudaSuccess) e = d.branch_pass(k, temperature);
+  if (e == cudaSuccess)
+    e = eos::launch_verify_draft(b.probs, b.q, V, b.words + at_drafts, nullptr, n_draft, b.u, n, V, b.words + at_out,
+                                 b.words + at_count, d.st);
+  if (e == cudaSuccess)
+    e = cudaMemcpyAsync(w + at_out, b.words + at_out, 4ull * n * (k + 1u), cudaMemcpyDeviceToHost, d.st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(d.st);
+  if (e != cudaSuccess) return dec_fail(e);
+  const int rc = dec_check_device_errors(t);
+  if (rc != EOS_OK) return rc;
+  for (uint32_t i = 0; i < n; ++i)
+    if (w[at_count + i] == 0 || w[at_out + (size_t)i * k + w[at_count + i] - 1u] >= V) {
+      eos::set_error_message("cuda text: a row's probabilities hold no token (NaN logits)");
+      return EOS_E_INTERNAL;
+    }
+  memcpy(out_tokens, w + at_out, 4ull * n * k);
+  memcpy(n_out, w + at_count, 4ull * n);
+  for (uint32_t i = 0; i < n; ++i) b.len[i] += n_out[i];  // the fed token and the accepted drafts are cached
+  return EOS_OK;
+}
+
+EOSLLM_CUDA_API int eosi_cuda_text_branch_adopt(eosi_cuda_text_t* t, uint32_t seq) {
+  if (t == nullptr) return EOS_E_INVALID_ARG;
+  TextDecoder& d = t->d;
+  if (seq >= d.br.n) {
+    eos::set_error_message("cuda text: no such branch");
+    return EOS_E_INVALID_ARG;
+  }
+  if (cudaSetDevice(d.device) != cudaSuccess) return EOS_E_INTERNAL;
+  const size_t page = (size_t)d.kvl * eos::kv_block_bytes(d.hd);
+  const uint32_t used = (d.br.len[seq] + eos::kKvPage - 1u) / eos::kKvPage, pos = d.br.full + d.br.len[seq];
+  cudaError_t e = cudaSuccess;
+  for (uint32_t L = 0; L < d.m.n_layer && used > 0 && e == cudaSuccess; ++L)
+    e = cudaMemcpyAsync(d.q8_at(L).pages + page * (d.br.full / eos::kKvPage),
+                        d.br_at(L).pages + page * d.br.pages * seq, page * used, cudaMemcpyDeviceToDevice, d.st);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&d.state->pos, &pos, 4, cudaMemcpyHostToDevice, d.st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(d.st);
+  if (e != cudaSuccess) return dec_fail(e);
+  d.host_pos = pos;
+  d.close_branches();
+  return EOS_OK;
+}
+
+EOSLLM_CUDA_API int eosi_cuda_text_branch_close(eosi_cuda_text_t* t) {
+  if (t == nullptr) return EOS_E_INVALID_ARG;
+  if (cudaSetDevice(t->d.device) != cudaSuccess) return EOS_E_INTERNAL;
+  t->d.close_branches();
+  return EOS_OK;
 }
 
 EOSLLM_CUDA_API void eosi_cuda_text_close(eosi_cuda_text_t* t) {

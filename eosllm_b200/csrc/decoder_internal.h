@@ -170,4 +170,15 @@ cudaError_t launch_pf_silu_pack(const float* gu, uint32_t m, uint32_t ffl, void*
 // x[i] += src[i] over m rows of n (the rows every rank pushed into src).
 cudaError_t launch_pf_xchg(const XchgSync& xs, float* x, const float* src, uint32_t m, uint32_t n, cudaStream_t st);
 
+// 8-bit cache mode and branches (decoder_branch.cu).  RoPE on the q and k heads
+// of m rows of qkv, in place; row r of sequence r / per_seq sits at position
+// pos[r / per_seq] + r % per_seq (device memory); len_out (optional) receives
+// pos[0] + 1.
+cudaError_t launch_rope_rows(float* qkv, uint32_t m, uint32_t per_seq, uint32_t hl, uint32_t kvl, uint32_t hd,
+                             const uint32_t* pos, float base, uint32_t* len_out, cudaStream_t st);
+// rows of n logits -> softmax(logits / temperature) in place (0: all on the largest).
+cudaError_t launch_logit_probs(float* logits, uint32_t rows, uint32_t n, float temperature, cudaStream_t st);
+// q[r][i] = (i == tokens[r]).
+cudaError_t launch_one_hot(float* q, const uint32_t* tokens, uint32_t rows, uint32_t n, cudaStream_t st);
+
 }  // namespace eos

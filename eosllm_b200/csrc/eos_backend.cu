@@ -637,7 +637,7 @@ int attn_batch_args(const eosi_cuda_attn_batch_t* b, const eos::KvPool& pool, ui
     return fail(EOS_E_INVALID_ARG, "kv attention: lengths above 2^30 tokens");
   out = eos::KvAttnBatch{b->max_prefix ? b->prefix_table : nullptr, b->max_prefix ? b->prefix_len : nullptr,
                          b->table, b->seq_len, b->row0, b->max_prefix, b->table_stride, b->max_len,
-                         b->n_seq, b->n_rows, b->max_rows};
+                         b->n_seq, b->n_rows, b->max_rows, nullptr};
   if (eos::kv_attn_work_bound(pool, out, n_head) >= (1ull << 31))
     return fail(EOS_E_INVALID_ARG, "kv attention: too many pages times heads times row groups (2^31)");
   return EOS_OK;

@@ -115,6 +115,7 @@ struct KvAttnBatch {
   const uint32_t* seq_len;
   const uint32_t* row0;
   uint32_t max_prefix, table_stride, max_len, n_seq, n_rows, max_rows;
+  const KvPool* prefix_pool;  // where the prefix's pages are, when not in the sequences' pool (host pointer)
 };
 constexpr uint32_t EOS_ATTN_MAX_SEQ = 1024;  // EOSI_CUDA_ATTN_MAX_SEQ
 size_t kv_attn_scratch_bytes(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head);

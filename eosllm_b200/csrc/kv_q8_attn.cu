@@ -71,13 +71,14 @@ inline AttnDiv attn_divisor(uint32_t d) {  // mul = ceil(2^(32 + s) / d), 2^(s -
 
 struct KvAttnParams {
   KvRows rows;
-  const uint8_t* pages;
+  const uint8_t* pages;         // the sequences' pool
+  const uint8_t* prefix_pages;  // the prefix's (the same, or another of the same geometry)
   const uint32_t* prefix_table;
   const uint32_t* prefix_len;
   const uint32_t* table;
   const uint32_t* seq_len;
   uint32_t max_prefix, table_stride, max_len, max_rows;
-  uint32_t n_pages, n_head, n_kv_head, group;
+  uint32_t n_pages, prefix_n_pages, n_head, n_kv_head, group;
   AttnDiv by_group, by_kv_head;
   const float* q;
   float* out;
@@ -453,11 +454,12 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
   }
   for (uint32_t pg = first; pg < last; ++pg) {
     const uint32_t page = table[pg];
-    if (page >= p.n_pages) {  // hidden
+    if (page >= (prefix ? p.prefix_n_pages : p.n_pages)) {  // hidden
       if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
       continue;
     }
-    const uint8_t* blk = p.pages + ((size_t)page * p.n_kv_head + g) * kv_block_bytes(HD);
+    const uint8_t* blk =
+        (prefix ? p.prefix_pages : p.pages) + ((size_t)page * p.n_kv_head + g) * kv_block_bytes(HD);
     const uint32_t avail = s.len - pg * kKvPage;  // tokens (may exceed a page)
     uint4 kw[CL], vw[DT][QT][2];
 #pragma unroll
@@ -764,7 +766,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
         if (s.tiles > 0) break;
       }
       more = s.tiles > 0;
-      const uint32_t* table = s.seq == p.rows.n_seq ? p.prefix_table : p.table + (size_t)s.seq * p.table_stride;
+      const bool is_prefix = s.seq == p.rows.n_seq;
+      const uint32_t* table = is_prefix ? p.prefix_table : p.table + (size_t)s.seq * p.table_stride;
+      const uint8_t* pool = is_prefix ? p.prefix_pages : p.pages;
+      const uint32_t pool_pages = is_prefix ? p.prefix_n_pages : p.n_pages;
       uint32_t mine = lane < s.tiles ? table[s.tile0 + lane] : 0u;
       if (lane == 0) {
         live = stage_free();
@@ -773,7 +778,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
           live = false;
         }
         if (live) {
-          bar.job[nj & 1u] = AttnJob{s.tiles, s.tile0, s.rows, s.row0, s.len, s.n, s.unit, s.seq == p.rows.n_seq ? 1u : 0u};
+          bar.job[nj & 1u] = AttnJob{s.tiles, s.tile0, s.rows, s.row0, s.len, s.n, s.unit, is_prefix ? 1u : 0u};
           if (more) mbar_arrive_expect_tx(&bar.full[x % S], s.rows * HD * 4u);
           else mbar_arrive(&bar.full[x % S]);
         }
@@ -794,13 +799,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
           const uint32_t st = x % S;
           live = stage_free();
           if (!live) {
-          } else if (page >= p.n_pages) {
+          } else if (page >= pool_pages) {
             report(p.err, EOS_DEVERR_RANGE);
             bar.ok[st] = 0u;
             mbar_arrive(&bar.full[st]);
           } else {
             bar.ok[st] = 1u;
-            const uint8_t* src = p.pages + ((size_t)page * p.n_kv_head + s.head) * G::kBlock;
+            const uint8_t* src = pool + ((size_t)page * p.n_kv_head + s.head) * G::kBlock;
             const uint32_t dst = smem_u32(stages + st * G::kBlock);
             const uint32_t left = s.len - (s.tile0 + j) * kKvPage;
             if (left >= kKvPage) {
@@ -1452,6 +1457,8 @@ cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* 
   KvAttnParams p{};
   p.rows = KvRows{b.row0, b.n_seq, b.n_rows, b.row0 ? 0u : b.n_rows / b.n_seq};
   p.pages = kv.pages;
+  p.prefix_pages = b.prefix_pool ? b.prefix_pool->pages : kv.pages;
+  p.prefix_n_pages = b.prefix_pool ? b.prefix_pool->n_pages : kv.n_pages;
   p.prefix_table = b.prefix_table;
   p.prefix_len = b.prefix_len;
   p.table = b.table;

@@ -165,6 +165,53 @@ class TextDecoder:
         B.check(self.lib.eosi_cuda_text_set_prefill_resident(self.handle, int(bool(resident))),
                 "eosi_cuda_text_set_prefill_resident")
 
+    # eosi_cuda_text_set_cache: how keys and values are held
+    CACHE_F32, CACHE_Q8 = 0, 1
+
+    def set_cache(self, mode: int) -> None:
+        """CACHE_F32 (default) or CACHE_Q8 (8-bit integers with a scale per
+        token and head), at position 0."""
+        B.check(self.lib.eosi_cuda_text_set_cache(self.handle, int(mode)), "eosi_cuda_text_set_cache")
+
+    @property
+    def cache(self) -> int:
+        return int(self.lib.eosi_cuda_text_cache(self.handle))
+
+    def fork(self, n_seq: int, max_new: int, max_draft: int = 0) -> None:
+        """Open n_seq branches that continue the tokens fed so far (8-bit
+        cache), each by up to max_new tokens."""
+        B.check(self.lib.eosi_cuda_text_fork(self.handle, n_seq, max_new, max_draft), "eosi_cuda_text_fork")
+        self._branches = n_seq
+
+    def branch_step(self, tokens, u, draft_probs=None, temperature: float = 1.0) -> list:
+        """Feed every branch tokens[i] = [next token, drafts...]; returns each
+        branch's accepted drafts plus one drawn token.  u: uniform numbers of
+        the same shape; draft_probs [n_seq][drafts][n_vocab] or None for drafts
+        that were not drawn; temperature 0 picks the most likely token."""
+        tok = np.ascontiguousarray(tokens, dtype=np.uint32)
+        un = np.ascontiguousarray(u, dtype=np.float32)
+        if tok.ndim != 2 or tok.shape[0] != getattr(self, "_branches", 0) or un.shape != tok.shape:
+            raise ValueError("tokens and u must be [n_seq][1 + drafts]")
+        n, k = tok.shape
+        q = None
+        if draft_probs is not None:
+            q = np.ascontiguousarray(draft_probs, dtype=np.float32)
+            if q.shape != (n, k - 1, self.n_vocab):
+                raise ValueError("draft_probs must be [n_seq][drafts][n_vocab]")
+        out, cnt = np.empty((n, k), np.uint32), np.empty(n, np.uint32)
+        B.check(self.lib.eosi_cuda_text_branch_step(self.handle, tok.ctypes.data, k - 1,
+                                                    None if q is None or q.size == 0 else q.ctypes.data,
+                                                    un.ctypes.data, float(temperature), out.ctypes.data,
+                                                    cnt.ctypes.data), "eosi_cuda_text_branch_step")
+        return [out[i, :cnt[i]] for i in range(n)]
+
+    def adopt(self, seq: int) -> None:
+        """Go on as branch `seq`; all branches close."""
+        B.check(self.lib.eosi_cuda_text_branch_adopt(self.handle, seq), "eosi_cuda_text_branch_adopt")
+
+    def close_branches(self) -> None:
+        B.check(self.lib.eosi_cuda_text_branch_close(self.handle), "eosi_cuda_text_branch_close")
+
     def reset(self) -> None:
         B.check(self.lib.eosi_cuda_text_reset(self.handle), "eosi_cuda_text_reset")
 

@@ -409,6 +409,42 @@ EOSLLM_CUDA_API int eosi_cuda_text_set_prefill_min(eosi_cuda_text_t *t, uint32_t
  * prefill, when that fits in half of the free device memory, and kept;
  * 0: each matrix is prepared into a scratch buffer just before its GEMM. */
 EOSLLM_CUDA_API int eosi_cuda_text_set_prefill_resident(eosi_cuda_text_t *t, int resident);
+/* The key/value cache.  F32 (the default): as the reference's.  Q8: rows held as
+ * 8-bit integers with one scale per token and head (eosi_cuda_kv_q8_write_dev's
+ * format), about a quarter of the memory and of the attention's reads; steps,
+ * prefill and generation run as before, with every token attending to its
+ * context as stored.  Only at position 0, without open branches
+ * (EOS_E_INVALID_ARG otherwise); Q8 needs world == 1 and the PER_OP step
+ * (EOS_E_UNSUPPORTED). */
+#define EOSI_CUDA_CACHE_F32 0
+#define EOSI_CUDA_CACHE_Q8 1
+EOSLLM_CUDA_API int eosi_cuda_text_set_cache(eosi_cuda_text_t *t, int mode);
+EOSLLM_CUDA_API int eosi_cuda_text_cache(const eosi_cuda_text_t *t);
+/* Branches: n_seq sequences that continue the tokens fed so far, each by up to
+ * max_new tokens, with up to max_draft drafted tokens per pass
+ * (n_seq * (max_draft + 1) <= min(max_ctx, 1024)).  They share the cache of the
+ * tokens so far, which every pass reads once for all of them.  Needs the Q8
+ * cache and Q4_K linears and LM head (EOS_E_UNSUPPORTED); while branches are
+ * open, step, prefill and generate are EOS_E_INVALID_ARG, and reset closes
+ * them. */
+EOSLLM_CUDA_API int eosi_cuda_text_fork(eosi_cuda_text_t *t, uint32_t n_seq, uint32_t max_new, uint32_t max_draft);
+/* One pass over all branches: branch i is fed tokens[i * (n_draft + 1) ...]: its
+ * next token, then n_draft <= max_draft drafted continuations.  The drafts are
+ * verified as by eosi_cuda_verify_draft_dev against softmax(logits /
+ * temperature) (temperature 0: the most likely token has probability 1) with
+ * the uniform numbers u[i * (n_draft + 1) ...] in [0, 1); draft_probs: host
+ * memory [n_seq][n_draft][n_vocab], the probabilities the drafts were drawn
+ * from, or NULL for drafts that were not drawn (probability 1 each).
+ * out_tokens[i * (n_draft + 1) ...] gets n_out[i] tokens: the accepted drafts and
+ * one drawn token, to be fed next.  With n_draft = 0 this draws one token per
+ * branch.  Host pointers; synchronous. */
+EOSLLM_CUDA_API int eosi_cuda_text_branch_step(eosi_cuda_text_t *t, const uint32_t *tokens, uint32_t n_draft,
+                                               const float *draft_probs, const float *u, float temperature,
+                                               uint32_t *out_tokens, uint32_t *n_out);
+/* The decoder goes on as branch `seq`: its tokens fed so far become the
+ * decoder's, the position moves behind them, and all branches close. */
+EOSLLM_CUDA_API int eosi_cuda_text_branch_adopt(eosi_cuda_text_t *t, uint32_t seq);
+EOSLLM_CUDA_API int eosi_cuda_text_branch_close(eosi_cuda_text_t *t);
 /* Position back to 0 (the KV cache is overwritten as steps proceed). */
 EOSLLM_CUDA_API int eosi_cuda_text_reset(eosi_cuda_text_t *t);
 EOSLLM_CUDA_API uint32_t eosi_cuda_text_pos(const eosi_cuda_text_t *t);
