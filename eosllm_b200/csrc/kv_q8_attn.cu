@@ -337,12 +337,14 @@ __device__ __forceinline__ float attn_warp_max(float x) {
 // memory's time.  No barrier or tensor memory to set up and several CTAs per
 // SM, each with a page's loads in flight: units of a page or two (a
 // sequence's own tokens, a decode step) take one round trip to memory.
-// Same digits and sums as the tensor-core kernel: s32 sums over 16 dimensions
-// (scores) and over a page (values) are exact.
+// Queries as in the tensor-core kernel, probabilities with 8 bits more; s32 sums
+// over 16 dimensions (scores) and over a page (values) are exact.
 constexpr uint32_t kFewRows = 4;
 constexpr uint32_t kFewThreads = 128;
 
-__device__ __forceinline__ int32_t attn_dp4a_su(uint32_t a, uint32_t b, int32_t c) {  // s8 x u8
+// s8 x u8 (or s8 x s8) dot product of four.
+__device__ __forceinline__ int32_t attn_dp4a(bool b_unsigned, uint32_t a, uint32_t b, int32_t c) {
+  if (!b_unsigned) return __dp4a((int)a, (int)b, c);
   int32_t d;
   asm("dp4a.s32.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
   constexpr uint32_t QT = HD == 64u ? 2u : 4u;         // quarters of the values per thread
   __shared__ __align__(16) uint32_t qd[R][3][HD / 4u]; // query digits
   __shared__ float qscale[R];
-  __shared__ __align__(16) uint8_t pd[R][3][kKvPage];  // probability digits by position
+  __shared__ __align__(16) uint8_t pd[R][4][kKvPage];  // probability digits by position
   __shared__ float red[2][4][R + 1u];                  // per warp: maxima, largest value scale
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t g = blockIdx.y;
@@ -543,21 +545,24 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
       m[r] = nm;
       const float e = attn_ex2(fmaf(z[r], qsc[r], neg));
       l[r] = fmaf(l[r], f[r], e);  // this token's share
-      const uint32_t w = __float_as_uint(fmaf(e, vs * up, 8388608.0f));
+      // e vs as 23 bits (the low bytes of 2^23 + ..) and a signed byte of what is left, in 1 / 256
+      const float y = vs * up, b = fmaf(e, y, 8388608.0f), rest = fmaf(e, y, 8388608.0f - b);
+      const uint32_t w = __float_as_uint(b);
       uint8_t* at = &pd[r][0][warp * 32u + kv_v_position(own)];
       at[0] = (uint8_t)w;
       at[kKvPage] = (uint8_t)(w >> 8);
       at[2u * kKvPage] = (uint8_t)(w >> 16);
+      at[3u * kKvPage] = (uint8_t)__float2int_rn(fminf(rest * 256.0f, 127.0f));
     }
     __syncthreads();
     // values
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
-      int32_t a[DT][3];
+      int32_t a[DT][4];
 #pragma unroll
-      for (uint32_t d = 0; d < DT; ++d) a[d][0] = a[d][1] = a[d][2] = 0;
+      for (uint32_t d = 0; d < DT; ++d) a[d][0] = a[d][1] = a[d][2] = a[d][3] = 0;
 #pragma unroll
-      for (uint32_t e = 0; e < 3u; ++e)
+      for (uint32_t e = 0; e < 4u; ++e)
 #pragma unroll
         for (uint32_t q = 0; q < QT; ++q)
 #pragma unroll
@@ -565,15 +570,16 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
             const uint4 w = *reinterpret_cast<const uint4*>(&pd[r][e][(q0 + q) * kKvQuarter + c * 16u]);
 #pragma unroll
             for (uint32_t d = 0; d < DT; ++d) {
-              a[d][e] = attn_dp4a_su(vw[d][q][c].x, w.x, a[d][e]);
-              a[d][e] = attn_dp4a_su(vw[d][q][c].y, w.y, a[d][e]);
-              a[d][e] = attn_dp4a_su(vw[d][q][c].z, w.z, a[d][e]);
-              a[d][e] = attn_dp4a_su(vw[d][q][c].w, w.w, a[d][e]);
+              a[d][e] = attn_dp4a(e < 3u, vw[d][q][c].x, w.x, a[d][e]);
+              a[d][e] = attn_dp4a(e < 3u, vw[d][q][c].y, w.y, a[d][e]);
+              a[d][e] = attn_dp4a(e < 3u, vw[d][q][c].z, w.z, a[d][e]);
+              a[d][e] = attn_dp4a(e < 3u, vw[d][q][c].w, w.w, a[d][e]);
             }
           }
 #pragma unroll
       for (uint32_t d = 0; d < DT; ++d) {
-        const float v = fmaf((float)a[d][2], 65536.0f, fmaf((float)a[d][1], 256.0f, (float)a[d][0]));
+        const float low = fmaf((float)a[d][1], 256.0f, fmaf((float)a[d][3], 1.0f / 256.0f, (float)a[d][0]));
+        const float v = fmaf((float)a[d][2], 65536.0f, low);
         o[r][d] = fmaf(v, unit, o[r][d] * f[r]);
       }
     }
@@ -810,7 +816,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
             const uint32_t left = s.len - (s.tile0 + j) * kKvPage;
             if (left >= kKvPage) {
               mbar_arrive_expect_tx(&bar.full[st], G::kBlock);
-              attn_bulk(dst, src, G::kBlock, &bar.full[st]);
             } else {  // the rows, quarters and scales that hold tokens
               const uint32_t kr = (left + 7u) / 8u * 8u * G::kQRow, nq = attn_ceil(left, kKvQuarter);
               const uint32_t vb = nq * HD * kKvQuarter, sb = nq * 256u;
@@ -824,6 +829,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
         }
         live = agree(live);
         if (!live) break;
+        // a whole page as eight copies side by side
+        if (page < pool_pages && s.len - (s.tile0 + j) * kKvPage >= kKvPage && lane < 8u)
+          attn_bulk(smem_u32(stages + (x % S) * G::kBlock) + lane * (G::kBlock / 8u),
+                    pool + ((size_t)page * p.n_kv_head + s.head) * G::kBlock + lane * (G::kBlock / 8u), G::kBlock / 8u,
+                    &bar.full[x % S]);
         ++x;
       }
     }
@@ -1006,14 +1016,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
         return seen <= 0 ? 0u : (seen < (int64_t)s.len ? (uint32_t)seen : s.len);
       };
       const uint32_t common = limit(0);
-      float fold = 0.0f;       // the last tile's probability unit
+      float2 fold[NC];         // the last tile's probability unit, relative to the running reference
       uint32_t it = n_own;     // tiles of this half so far
-      // o = o f + unit * (value product of the tile before)
+      // o = o f + fold * (value product of the tile before)
       auto fold_tile = [&]() {
         if (!__all_sync(0xffffffffu, attn_wait(&bar.o_full[half], (it - 1u) & 1u))) return false;
         attn_fence_after();
         if (HD >= 128u || quad * 32u < HD) {
-          const float2 unit = attn_two(fold);
 #pragma unroll
           for (uint32_t y = 0; y < NC; ++y) {
             if (y >= nact) break;  // warp-uniform
@@ -1029,7 +1038,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
               attn_ld_wait();
 #pragma unroll
               for (uint32_t j = 0; j < 4u; ++j)
-                o[y][mh][j] = attn_fma2(attn_join_value(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), unit,
+                o[y][mh][j] = attn_fma2(attn_join_value(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), fold[y],
                                         attn_mul2(o[y][mh][j], f[y]));
             }
           }
@@ -1123,12 +1132,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
                        m1 = *reinterpret_cast<const float2*>(xmt + RT + 8u * y),
                        m2 = *reinterpret_cast<const float2*>(xmt + 2u * RT + 8u * y),
                        m3 = *reinterpret_cast<const float2*>(xmt + 3u * RT + 8u * y);
-          // the reference is rounded up, so that no probability exceeds 1
+          // the tile's own reference, rounded up so that no probability exceeds 1
+          // (its integers are relative to it: their rounding fades with the tile)
           const float t0 = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x)), t1 = fmaxf(fmaxf(m0.y, m1.y), fmaxf(m2.y, m3.y));
-          const float2 nm = make_float2(fmaxf(t0 == -INFINITY ? t0 : __fmul_ru(t0, qsc[y].x), m[y].x),
-                                        fmaxf(t1 == -INFINITY ? t1 : __fmul_ru(t1, qsc[y].y), m[y].y));
-          const float2 neg = make_float2(nm.x == -INFINITY ? 0.0f : -nm.x, nm.y == -INFINITY ? 0.0f : -nm.y);
-          f[y] = make_float2(attn_ex2(m[y].x + neg.x), attn_ex2(m[y].y + neg.y));
+          const float2 ref = make_float2(t0 == -INFINITY ? t0 : __fmul_ru(t0, qsc[y].x),
+                                         t1 == -INFINITY ? t1 : __fmul_ru(t1, qsc[y].y));
+          const float2 neg = make_float2(ref.x == -INFINITY ? 0.0f : -ref.x, ref.y == -INFINITY ? 0.0f : -ref.y);
+          const float2 nm = make_float2(fmaxf(ref.x, m[y].x), fmaxf(ref.y, m[y].y));
+          const float2 run = make_float2(nm.x == -INFINITY ? 0.0f : nm.x, nm.y == -INFINITY ? 0.0f : nm.y);
+          f[y] = make_float2(attn_ex2(m[y].x - run.x), attn_ex2(m[y].y - run.y));
+          const float2 share = make_float2(attn_ex2(ref.x - run.x), attn_ex2(ref.y - run.y));
+          fold[y] = attn_mul2(share, attn_two(unit));
           m[y] = nm;
           uint32_t b0[4], b1[4], d[3];
           float2 ls = attn_two(0.0f);
@@ -1141,7 +1155,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
             b0[j] = __float_as_uint(w.x);
             b1[j] = __float_as_uint(w.y);
           }
-          l[y] = attn_fma2(l[y], f[y], ls);
+          l[y] = attn_fma2(l[y], f[y], attn_mul2(ls, share));
           // row e RT + col of digit e, this thread's four tokens: one word
           uint8_t* at = pop + (g & 3u) * 4u;
           const uint32_t chunk = 2u * quad + (g >> 2);
@@ -1154,7 +1168,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
           for (uint32_t e = 0; e < 3u; ++e)
             *reinterpret_cast<uint32_t*>(at + (e * RT + col + 1u) * kKvPage + ((chunk ^ ((col + 1u) & 7u)) << 4)) = d[e];
         }
-        fold = unit;
         ++it;
         attn_fence_async();
         __syncwarp();

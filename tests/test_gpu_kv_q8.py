@@ -248,6 +248,12 @@ def test_attention_long(gpu, prefix, lens, counts):
     Batch(gpu, 4, 2, 128, prefix, lens, counts, seed=1).check()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_units(gpu, hd):
+    """More units (a head of a sequence) than CTAs: each takes several in turn."""
+    Batch(gpu, 16, 16, hd, 200, [20, 5, 130] * 14, [5, 5, 6] * 14, seed=hd).check()
+
+
 def test_rows_without_any_key(gpu):
     """Sequences with no visible token give 0, with and without neighbours."""
     b = Batch(gpu, 4, 2, 64, 0, [0, 1, 2], [1, 3, 2], seed=4)  # row 0 none; rows 1, 2 of sequence 1 none
