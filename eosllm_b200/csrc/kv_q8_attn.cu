@@ -274,17 +274,10 @@ __device__ __forceinline__ float2 attn_float(uint32_t a, uint32_t b) {
   return attn_add2(make_float2(__uint_as_float(a + 0x4B400000u), __uint_as_float(b + 0x4B400000u)),
                    attn_two(-kAttnMagic));
 }
-// Value sums: D2 65536 + D1 256 + D0, every bit (a bias of the low digit
-// would add up over the tiles).
-__device__ __forceinline__ float2 attn_join_value(const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
-  return attn_fma2(attn_float(d2[0], d2[1]), attn_two(65536.0f),
-                   attn_fma2(attn_float(d1[0], d1[1]), attn_two(256.0f), attn_float(d0[0], d0[1])));
-}
-// Score sums: D2 256 + D1 + floor(D0 / 256), in units of 256 (less than one
-// unit off, of about 2^22 for a typical score).
-__device__ __forceinline__ float2 attn_join_score(const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
-  const uint32_t y0 = d1[0] + (uint32_t)((int32_t)d0[0] >> 8), y1 = d1[1] + (uint32_t)((int32_t)d0[1] >> 8);
-  return attn_fma2(attn_float(d2[0], d2[1]), attn_two(256.0f), attn_float(y0, y1));
+// D2 256 + D1 + D0 / 256 of three s32 sums, rounded once or twice.
+__device__ __forceinline__ float2 attn_join(const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
+  return attn_fma2(attn_float(d2[0], d2[1]), attn_two(256.0f),
+                   attn_fma2(attn_float(d0[0], d0[1]), attn_two(1.0f / 256.0f), attn_float(d1[0], d1[1])));
 }
 // Bytes 0, 1 and 2 of four words as three words.
 __device__ __forceinline__ void attn_digits(const uint32_t* b, uint32_t* w) {
@@ -1038,7 +1031,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
               attn_ld_wait();
 #pragma unroll
               for (uint32_t j = 0; j < 4u; ++j)
-                o[y][mh][j] = attn_fma2(attn_join_value(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), fold[y],
+                o[y][mh][j] = attn_fma2(attn_join(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), fold[y],
                                         attn_mul2(o[y][mh][j], f[y]));
             }
           }
@@ -1066,7 +1059,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
         top = __reduce_max_sync(0xffffffffu, top) >> 23;
         top = top < 23u ? 23u : top;
         const float up = __uint_as_float((276u - top) << 23);           // 2^(22 - exponent)
-        const float unit = __uint_as_float((top - 22u) << 23);          // 2^(exponent - 22)
+        const float unit = __uint_as_float((top - 14u) << 23);          // 256 * 2^(exponent - 22)
         // this thread's four tokens: quarter quad, g + 8 j
         float ks[4], vw[4];
 #pragma unroll
@@ -1094,7 +1087,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
           attn_ld_wait();
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j)
-            sv[y][j] = attn_mul2(attn_join_score(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), attn_two(ks[j]));
+            sv[y][j] = attn_mul2(attn_join(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), attn_two(ks[j]));
           if (!whole) {
             const uint32_t col = 8u * y + 2u * cq;
             const uint32_t lim0 = limit(col), lim1 = limit(col + 1u);
