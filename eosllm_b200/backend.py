@@ -332,7 +332,12 @@ NO_TOKEN = 0xFFFFFFFF
 
 
 def _optr(x):
-    return None if x is None else (_ptr(x) or None)
+    if x is None:
+        return None
+    try:
+        return x.data_ptr() or None
+    except AttributeError:
+        return _ptr(x) or None
 
 
 def kv_q8_page_bytes(n_kv_head: int, head_dim: int) -> int:

@@ -89,8 +89,9 @@ struct KvAttnParams {
   float *so, *sml;   // the sequences' partials, with seq_cap rows
   uint32_t prefix_cap, seq_cap;  // rows of a partial
   uint32_t seq_groups;           // row groups reserved per sequence
-  // pages per CTA where the few-rows kernel has the prefix (the sequences), else 0: the line has them
-  uint32_t prefix_run, prefix_runs, seq_run, seq_runs;
+  // clusters per unit and CTAs per cluster where the few-rows kernel has the prefix (the sequences), else 0: the
+  // line has them
+  uint32_t prefix_few, prefix_ctas, seq_few, seq_ctas;
   uint32_t* err;
 };
 
@@ -323,9 +324,11 @@ __device__ __forceinline__ float attn_warp_max(float x) {
 }
 
 // ---- few rows: integer dot products on the CUDA cores -------------------------
-// Up to kFewRows rows (query rows times heads of the kv head) against the pages
-// [first, first + pages_per_cta) of a unit, one CTA of 128 threads per (unit,
-// run of pages).  Reading the cache is what bounds it: 2 HD + 8 bytes per token
+// Up to kFewRows rows (query rows times heads of the kv head) against a unit's
+// pages, dealt out to the CTAs (128 threads) of one or more clusters: whatever
+// the length turns out to be, all of them have their share.  A cluster joins
+// its CTAs' sums through shared memory, so a unit on one cluster is done with
+// one launch.  Reading the cache is what bounds it: 2 HD + 8 bytes per token
 // against 6 HD / 4 dp4a per token and row, so up to four rows stay below the
 // memory's time.  No barrier or tensor memory to set up and several CTAs per
 // SM, each with a page's loads in flight: units of a page or two (a
@@ -350,11 +353,23 @@ __device__ __forceinline__ uint4 attn_ld_stream(const void* src) {
   return v;
 }
 
-// Grid (pages / pages_per_cta, kv heads, sequences); prefix: one "sequence" of
-// all rows.
+__device__ __forceinline__ void attn_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A float of this CTA's shared memory as CTA `rank` of the cluster holds it.
+__device__ __forceinline__ float attn_peer(const float* x, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(x)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// Grid (clusters x CTAs, kv heads, sequences); prefix: one "sequence" of all
+// rows.  direct: there is nothing to join the rows with, write them out.
 template <uint32_t HD, uint32_t R>
 __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnParams p, uint32_t prefix,
-                                                                  uint32_t pages_per_cta) {
+                                                                  uint32_t n_cta, uint32_t direct) {
   constexpr uint32_t CL = HD / 16u;                    // 16-byte chunks of a key row = lanes per token
   constexpr uint32_t DT = HD <= 128u ? 1u : HD / 128u; // dimensions per thread
   constexpr uint32_t QT = HD == 64u ? 2u : 4u;         // quarters of the values per thread
@@ -362,6 +377,7 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
   __shared__ float qscale[R];
   __shared__ __align__(16) uint8_t pd[R][4][kKvPage];  // probability digits by position
   __shared__ float red[2][4][R + 1u];                  // per warp: maxima, largest value scale
+  __shared__ float cl_o[R][HD], cl_ml[R][2];           // this CTA's sums, for the cluster
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t g = blockIdx.y;
   AttnSeq s{0, 0, 0};
@@ -371,21 +387,19 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
     s.n = kv_row_start(p.rows, p.rows.n_seq);
     if (s.len > p.max_prefix) {
       s.len = p.max_prefix;
-      if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
+      if (blockIdx.x == 0 && g == 0 && tid == 0) report(p.err, EOS_DEVERR_RANGE);
     }
   } else {
     s = attn_seq(p, blockIdx.z);
     table = p.table + (size_t)blockIdx.z * p.table_stride;
-    if (blockIdx.x == 0 && tid == 0 && (p.seq_len[blockIdx.z] > p.max_len || s.n > p.max_rows))
+    if (blockIdx.x == 0 && g == 0 && tid == 0 && (p.seq_len[blockIdx.z] > p.max_len || s.n > p.max_rows))
       report(p.err, EOS_DEVERR_RANGE);
   }
-  const uint32_t first = blockIdx.x * pages_per_cta;
   const uint32_t pages = attn_ceil(s.len, kKvPage);
   uint32_t rows = (prefix || s.n < p.max_rows ? s.n : p.max_rows) * p.group;
   if (rows > R) rows = R;  // (the host chose R >= rows)
   pdl_trigger();
-  if (first >= pages || rows == 0) return;  // the joining kernel knows which runs exist
-  const uint32_t last = first + pages_per_cta < pages ? first + pages_per_cta : pages;
+  if (rows == 0) return;  // the whole cluster
   const int32_t seen0 = (int32_t)s.len - (int32_t)s.n + 1;  // tokens a sequence's first row sees (may be negative)
   // warp r: row r's digits
   if (warp < R) {
@@ -447,7 +461,8 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
 #pragma unroll
     for (uint32_t d = 0; d < DT; ++d) o[r][d] = 0.0f;
   }
-  for (uint32_t pg = first; pg < last; ++pg) {
+  uint32_t par = 0;  // which red[]
+  for (uint32_t pg = blockIdx.x; pg < pages; pg += gridDim.x, par ^= 1u) {
     const uint32_t page = table[pg];
     if (page >= (prefix ? p.prefix_n_pages : p.n_pages)) {  // hidden
       if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
@@ -517,14 +532,14 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
       const int32_t tok = (int32_t)(pg * kKvPage + own);
       z[r] = own < avail && tok < seen ? part[0] * ks : -INFINITY;
       const float mx = attn_warp_max(z[r]);
-      if (lane == 0) red[pg & 1u][warp][r] = mx;
+      if (lane == 0) red[par][warp][r] = mx;
     }
     {
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs));
-      if (lane == 0) red[pg & 1u][warp][R] = __uint_as_float(top);
+      if (lane == 0) red[par][warp][R] = __uint_as_float(top);
     }
     __syncthreads();
-    const float(*rd)[R + 1u] = red[pg & 1u];
+    const float(*rd)[R + 1u] = red[par];
     uint32_t top = __float_as_uint(fmaxf(fmaxf(rd[0][R], rd[1][R]), fmaxf(rd[2][R], rd[3][R]))) >> 23;
     top = top < 23u ? 23u : top;
     const float up = __uint_as_float((276u - top) << 23), unit = __uint_as_float((top - 22u) << 23);
@@ -578,29 +593,80 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
     }
     // (the next page's red[] is the other buffer, and its pd[] follows a barrier that every warp reaches after these reads)
   }
-  // partial: all l shares, one maximum, the outputs
-  const uint32_t cap = prefix ? p.prefix_cap : p.seq_cap;
-  const size_t id = ((size_t)(prefix ? 0u : blockIdx.z) * p.n_kv_head + g) * gridDim.x + blockIdx.x;
-  float* po = (prefix ? p.po : p.so) + id * cap * HD;
-  float* pml = (prefix ? p.pml : p.sml) + id * cap * kAttnMl;
+  // this CTA's sums, then the cluster's: CTA 0 joins and writes them
 #pragma unroll
   for (uint32_t r = 0; r < R; ++r) {
     float ls = l[r];
 #pragma unroll
     for (uint32_t b = 16; b > 0; b >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, b);
-    if (r >= rows) continue;
-    if (lane == 0) pml[r * kAttnMl + 4u + warp] = ls;
-    if (tid == 0) pml[r * kAttnMl] = m[r];
+    if (lane == 0) red[0][warp][r] = ls;
     if constexpr (HD == 64) {  // two threads hold the halves of a dimension's sum
-      __shared__ float oh[R][64];
-      if (tid >= 64u) oh[r][tid & 63u] = o[r][0];
-      __syncthreads();
-      if (tid < 64u) po[(size_t)r * HD + tid] = o[r][0] + oh[r][tid];
+      if (tid >= 64u) cl_o[r][tid & 63u] = o[r][0];
     } else {
 #pragma unroll
-      for (uint32_t d = 0; d < DT; ++d) po[(size_t)r * HD + d * 128u + tid] = o[r][d];
+      for (uint32_t d = 0; d < DT; ++d) cl_o[r][d * 128u + tid] = o[r][d];
     }
   }
+  __syncthreads();
+  if (tid < R) {
+    cl_ml[tid][1] = (red[0][0][tid] + red[0][1][tid]) + (red[0][2][tid] + red[0][3][tid]);
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r)
+      if (tid == r) cl_ml[r][0] = m[r];
+  }
+  if constexpr (HD == 64) {
+    if (tid < 64u)
+#pragma unroll
+      for (uint32_t r = 0; r < R; ++r) cl_o[r][tid] += o[r][0];
+  }
+  attn_cluster_sync();
+  const uint32_t rank = blockIdx.x % n_cta;
+  if (rank == 0) {
+    const uint32_t cap = prefix ? p.prefix_cap : p.seq_cap;
+    const size_t id = ((size_t)(prefix ? 0u : blockIdx.z) * p.n_kv_head + g) * (gridDim.x / n_cta) + blockIdx.x / n_cta;
+    float* po = (prefix ? p.po : p.so) + id * cap * HD;
+    float* pml = (prefix ? p.pml : p.sml) + id * cap * kAttnMl;
+    for (uint32_t r = 0; r < rows; ++r) {
+      float mc[8], lc2[8], oc[8][DT], top = -INFINITY;
+#pragma unroll
+      for (uint32_t c = 0; c < 8u; ++c)
+        if (c < n_cta) {
+          mc[c] = attn_peer(&cl_ml[r][0], c);
+          lc2[c] = attn_peer(&cl_ml[r][1], c);
+#pragma unroll
+          for (uint32_t d = 0; d < DT; ++d) oc[c][d] = attn_peer(&cl_o[r][(d * 128u + tid) % HD], c);
+          top = fmaxf(top, mc[c]);
+        }
+      const float mu = top == -INFINITY ? 0.0f : top;
+      float ls = 0.0f, acc[DT];
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d) acc[d] = 0.0f;
+#pragma unroll
+      for (uint32_t c = 0; c < 8u; ++c)
+        if (c < n_cta) {
+          const float f = attn_ex2(mc[c] - mu);
+          ls = fmaf(f, lc2[c], ls);
+#pragma unroll
+          for (uint32_t d = 0; d < DT; ++d) acc[d] = fmaf(f, oc[c][d], acc[d]);
+        }
+      if (tid >= HD) continue;
+      if (direct) {
+        const float inv = ls == 0.0f ? 0.0f : __fdiv_rn(1.0f, ls);
+        const uint32_t xr = attn_div(r, p.by_group);
+        float* dst = p.out + (size_t)(s.r0 + xr) * p.out_stride + (size_t)(g * p.group + r - xr * p.group) * HD;
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d) dst[d * 128u + tid] = acc[d] * inv;
+      } else {
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d) po[(size_t)r * HD + d * 128u + tid] = acc[d];
+        if (tid == 0) {
+          pml[r * kAttnMl] = top;
+          *reinterpret_cast<float4*>(pml + r * kAttnMl + 4u) = make_float4(ls, 0.0f, 0.0f, 0.0f);
+        }
+      }
+    }
+  }
+  attn_cluster_sync();  // no CTA leaves while its sums are read
 }
 
 // mbar_wait, reading the clock only once in 64 polls: its read takes longer
@@ -723,7 +789,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     for (uint32_t i0 = 0; i0 < p.rows.n_seq; i0 += 32u) {
       uint32_t w = 0;
       const bool in = i0 + lane < p.rows.n_seq;
-      if (in && p.seq_run == 0) w = attn_seq_work(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
+      if (in && p.seq_few == 0) w = attn_seq_work(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
       uint32_t c = w;
 #pragma unroll
       for (uint32_t o = 1; o < 32u; o <<= 1) {
@@ -736,7 +802,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     if (lane == 0) cum[p.rows.n_seq] = carry;
     __syncwarp();
     pl.prefix = prefix_len < p.max_prefix ? prefix_len : p.max_prefix;
-    if (p.prefix_run > 0) pl.prefix = 0;
+    if (p.prefix_few > 0) pl.prefix = 0;
     pl.rows_p = rows_end;
     pl.tp = attn_ceil(pl.prefix, kKvPage);
     pl.rgp = attn_ceil(pl.rows_p * p.group, RT);
@@ -1230,11 +1296,24 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
   const uint32_t hw = attn_div((uint32_t)x, p.by_group);  // row * n_kv_head + kv head
   const uint32_t r = attn_div(hw, p.by_kv_head), g = hw - r * p.n_kv_head, hh = (uint32_t)x - hw * p.group;
   const uint32_t h = g * p.group + hh;
-  const uint32_t i = kv_row_seq(p.rows, r);
-  if (i >= p.rows.n_seq) return;
-  pdl_wait();
+  // the row's sequence and the inputs' words: read while the attention still runs
+  uint32_t i = 0;
+  if (p.rows.row0 == nullptr) {
+    i = r / p.rows.per_seq;
+  } else {  // sequences that start at or before the row, 32 at a time
+    uint32_t n = 0;
+    for (;; n += 32u) {
+      const uint32_t c = __popc(__ballot_sync(0xffffffffu, n + lane <= p.rows.n_seq && kv_row_start(p.rows, n + lane) <= r));
+      i = n + c;
+      if (c < 32u) break;
+    }
+    if (i == 0 || i > p.rows.n_seq) return;  // before the first sequence or behind the last
+    --i;
+  }
   const uint32_t t = r - kv_row_start(p.rows, i);
   if (t >= p.max_rows) return;  // reported by the attention kernel
+  const uint32_t seq_len = p.seq_len[i];
+  pdl_wait();
   // ids of the row's partials: [first, last] of the prefix and of its sequence
   struct Part {
     const float *o, *ml;
@@ -1252,30 +1331,28 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
     a.o = o + ((size_t)2u * (unit + c0) * cap + row) * HD;
     a.ml = ml + ((size_t)2u * (unit + c0) * cap + row) * kAttnMl;
   };
-  // runs of pages of the few-rows kernel
-  auto runs = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t per_unit,
-                  uint32_t run, uint32_t tiles, uint32_t row) {
-    a.n = attn_ceil(tiles, run);
+  // the few-rows kernel's clusters
+  auto few = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t n, uint32_t row) {
+    a.n = n;
     a.o_step = cap * HD;
     a.ml_step = cap * kAttnMl;
-    a.o = o + ((size_t)unit * per_unit * cap + row) * HD;
-    a.ml = ml + ((size_t)unit * per_unit * cap + row) * kAttnMl;
+    a.o = o + ((size_t)unit * n * cap + row) * HD;
+    a.ml = ml + ((size_t)unit * n * cap + row) * kAttnMl;
   };
   if (p.max_prefix > 0) {
     const uint32_t fr = r * p.group + hh;
-    if (p.prefix_run > 0) {
-      const uint32_t len = *p.prefix_len < p.max_prefix ? *p.prefix_len : p.max_prefix;
-      runs(part[0], p.po, p.pml, p.prefix_cap, g, p.prefix_runs, p.prefix_run, attn_ceil(len, kKvPage), fr);
+    if (p.prefix_few > 0) {
+      few(part[0], p.po, p.pml, p.prefix_cap, g, p.prefix_few, fr);
     } else {
       const uint32_t tp = __ldcg(p.plan + 1), rgp = __ldcg(p.plan + 2), rg = fr / RT, unit = g * rgp + rg;
       line(part[0], p.po, p.pml, p.prefix_cap, unit, unit * attn_cost(tp), tp, fr % RT);
     }
   }
   {
-    const uint32_t len = p.seq_len[i] < p.max_len ? p.seq_len[i] : p.max_len;
+    const uint32_t len = seq_len < p.max_len ? seq_len : p.max_len;
     const uint32_t fr = t * p.group + hh, tiles = attn_ceil(len, kKvPage);
-    if (p.seq_run > 0) {
-      runs(part[1], p.so, p.sml, p.seq_cap, i * p.n_kv_head + g, p.seq_runs, p.seq_run, tiles, fr);
+    if (p.seq_few > 0) {
+      few(part[1], p.so, p.sml, p.seq_cap, i * p.n_kv_head + g, p.seq_few, fr);
     } else {
       const uint32_t rg = fr / RT, u = rg * p.n_kv_head + g;
       line(part[1], p.so, p.sml, p.seq_cap, i * p.seq_groups * p.n_kv_head + u,
@@ -1340,20 +1417,26 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
 namespace {
 
 // How a call runs: the prefix and the sequences each on the tensor cores' line
-// or, with at most kFewRows rows to a unit, in runs of pages (see the two
+// or, with at most kFewRows rows to a unit, on clusters of CTAs (see the two
 // kernels); and where their partials sit.
 struct AttnSplit {
   size_t plan, po, pml, so, sml, bytes;
   uint32_t prefix_cap, seq_cap, seq_groups;
-  uint32_t prefix_run, prefix_runs, seq_run, seq_runs;
+  uint32_t prefix_few, prefix_ctas, seq_few, seq_ctas;
   bool line;
 };
-// Pages per CTA of `units` units of up to `pages` pages: enough CTAs for the
-// machine (about eight per SM), at most 8 pages so that a row has few partials
-// to join next to what it reads.
-uint32_t attn_run(uint64_t units, uint64_t pages) {
-  const uint64_t want = units * pages / 1184u;
-  return want < 1u ? 1u : (want > 8u ? 8u : (uint32_t)want);
+// Clusters of up to eight CTAs for each of `units` units of up to `pages` pages.
+// CTAs: as many as give the machine about five an SM (many units: one CTA
+// each; 512 units of 3 pages on three CTAs each took 6 us longer).  Clusters:
+// one, which needs no joining kernel, unless the units leave SMs idle (below
+// about four CTAs each) and a CTA would still have four pages to read.
+void attn_clusters(uint64_t units, uint32_t pages, uint32_t& clusters, uint32_t& ctas) {
+  const uint64_t want = 740u / units;
+  ctas = (uint32_t)(want < 1u ? 1u : (want > 8u ? 8u : want));
+  if (ctas > pages) ctas = pages;
+  const uint64_t most = 592u / (units * ctas), by_pages = pages / (ctas * 4u);
+  clusters = (uint32_t)(most < by_pages ? most : by_pages);
+  if (clusters < 1u) clusters = 1u;
 }
 AttnSplit attn_split(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
   const uint32_t group = n_head / kv.n_kv_head, rt = kAttnRows;
@@ -1371,9 +1454,8 @@ AttnSplit attn_split(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
     const uint32_t pages = attn_ceil(b.max_prefix, kKvPage);
     s.prefix_cap = rows < rt ? (uint32_t)rows : rt;
     if (rows <= kFewRows) {
-      s.prefix_run = attn_run(kv.n_kv_head, pages);
-      s.prefix_runs = attn_ceil(pages, s.prefix_run);
-      put((uint64_t)kv.n_kv_head * s.prefix_runs, s.prefix_cap, s.po, s.pml);
+      attn_clusters(kv.n_kv_head, pages, s.prefix_few, s.prefix_ctas);
+      put((uint64_t)kv.n_kv_head * s.prefix_few, s.prefix_cap, s.po, s.pml);
     } else {
       s.line = true;
       put(2u * ((uint64_t)kv.n_kv_head * ((rows + rt - 1u) / rt) + kAttnMaxCtas), s.prefix_cap, s.po, s.pml);
@@ -1384,9 +1466,8 @@ AttnSplit attn_split(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
     s.seq_cap = per_seq < rt ? (uint32_t)per_seq : rt;
     s.seq_groups = (uint32_t)((per_seq + rt - 1u) / rt);
     if (per_seq <= kFewRows) {
-      s.seq_run = attn_run((uint64_t)b.n_seq * kv.n_kv_head, pages);
-      s.seq_runs = attn_ceil(pages, s.seq_run);
-      put((uint64_t)b.n_seq * kv.n_kv_head * s.seq_runs, s.seq_cap, s.so, s.sml);
+      attn_clusters((uint64_t)b.n_seq * kv.n_kv_head, pages, s.seq_few, s.seq_ctas);
+      put((uint64_t)b.n_seq * kv.n_kv_head * s.seq_few, s.seq_cap, s.so, s.sml);
     } else {
       s.line = true;
       put(2u * ((uint64_t)b.n_seq * s.seq_groups * kv.n_kv_head + kAttnMaxCtas), s.seq_cap, s.so, s.sml);
@@ -1396,23 +1477,37 @@ AttnSplit attn_split(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
 }
 
 template <uint32_t HD, uint32_t R>
-void attn_few(const KvAttnParams& p, uint32_t prefix, cudaStream_t st) {
-  const dim3 grid(prefix ? p.prefix_runs : p.seq_runs, p.n_kv_head, prefix ? 1u : p.rows.n_seq);
-  kv_attn_few_kernel<HD, R><<<grid, kFewThreads, 0, st>>>(p, prefix, prefix ? p.prefix_run : p.seq_run);
+cudaError_t attn_few(const KvAttnParams& p, uint32_t prefix, uint32_t direct, cudaStream_t st) {
+  const uint32_t n = prefix ? p.prefix_few : p.seq_few, ctas = prefix ? p.prefix_ctas : p.seq_ctas;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n * ctas, p.n_kv_head, prefix ? 1u : p.rows.n_seq);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_attn_few_kernel<HD, R>, p, prefix, ctas, direct);
 }
 template <uint32_t HD>
-void attn_few_rows(const KvAttnParams& p, uint32_t prefix, uint32_t rows, cudaStream_t st) {
-  if (rows == 1) attn_few<HD, 1>(p, prefix, st);
-  else if (rows == 2) attn_few<HD, 2>(p, prefix, st);
-  else attn_few<HD, 4>(p, prefix, st);
+cudaError_t attn_few_rows(const KvAttnParams& p, uint32_t prefix, uint32_t rows, uint32_t direct, cudaStream_t st) {
+  if (rows == 1) return attn_few<HD, 1>(p, prefix, direct, st);
+  if (rows == 2) return attn_few<HD, 2>(p, prefix, direct, st);
+  return attn_few<HD, 4>(p, prefix, direct, st);
 }
 
 template <uint32_t HD>
 cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t work, cudaStream_t st) {
   using G = AttnGeo<HD>;
   cudaError_t e = cudaSuccess;
-  if (p.seq_run > 0) attn_few_rows<HD>(p, 0, p.seq_cap, st);
-  if (p.prefix_run > 0) attn_few_rows<HD>(p, 1, p.prefix_cap, st);
+  const bool alone = p.max_prefix == 0 && p.seq_few == 1u;  // nothing to join
+  if (p.seq_few > 0) e = attn_few_rows<HD>(p, 0, p.seq_cap, alone ? 1u : 0u, st);
+  if (alone || e != cudaSuccess) return e;
+  if (p.prefix_few > 0) e = attn_few_rows<HD>(p, 1, p.prefix_cap, 0u, st);
+  if (e != cudaSuccess) return e;
   if (line) {
     static SmemAttr attr;
     e = ensure_smem_attr((const void*)kv_attn_kernel<HD>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
@@ -1492,10 +1587,10 @@ cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* 
   p.prefix_cap = s.prefix_cap;
   p.seq_cap = s.seq_cap;
   p.seq_groups = s.seq_groups;
-  p.prefix_run = s.prefix_run;
-  p.prefix_runs = s.prefix_runs;
-  p.seq_run = s.seq_run;
-  p.seq_runs = s.seq_runs;
+  p.prefix_few = s.prefix_few;
+  p.prefix_ctas = s.prefix_ctas;
+  p.seq_few = s.seq_few;
+  p.seq_ctas = s.seq_ctas;
   p.err = err;
   const uint64_t work = kv_attn_work_bound(kv, b, n_head);
   if (kv.head_dim == 64) return attn_launch<64>(p, s.line, num_sms, work, st);
