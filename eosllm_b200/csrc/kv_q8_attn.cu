@@ -48,7 +48,6 @@ namespace eos {
 
 constexpr uint32_t kAttnMaxCtas = 320;    // bound on the grid (scratch is sized with it)
 constexpr uint32_t kAttnThreads = 320;    // 8 softmax warps, a copy warp, a product warp
-constexpr uint32_t kAttnRows = 16;        // rows of a group: three digits of each are the columns of a product
 constexpr uint32_t kAttnMl = 8;           // floats per partial row: maximum, 3 unused, 4 partial sums
 constexpr float kAttnQMax = 8300000.0f;   // largest query integer (three balanced digits hold 127 * 65793)
 constexpr float kAttnMagic = 12582912.0f; // 1.5 * 2^23
@@ -87,6 +86,7 @@ struct KvAttnParams {
   uint32_t* plan;    // quantum, prefix tiles, prefix row groups, prefix work, then the sequences' running work
   float *po, *pml;   // prefix partials: [unit + CTA][half][row][HD], [unit + CTA][half][row][kAttnMl]
   float *so, *sml;   // the sequences' partials, with seq_cap rows
+  uint32_t rt;                   // rows of the line's groups
   uint32_t prefix_cap, seq_cap;  // rows of a partial
   uint32_t seq_groups;           // row groups reserved per sequence
   // clusters per unit and CTAs per cluster where the few-rows kernel has the prefix (the sequences), else 0: the
@@ -115,9 +115,10 @@ __device__ __forceinline__ AttnSeq attn_seq(const KvAttnParams& p, uint32_t i) {
   return s;
 }
 // Places of a sequence on the line (rows beyond max_rows are left out).
+template <uint32_t RT>
 __device__ __forceinline__ uint32_t attn_seq_work(const KvAttnParams& p, const AttnSeq& s) {
   const uint32_t n = s.n < p.max_rows ? s.n : p.max_rows;
-  return p.n_kv_head * attn_ceil(n * p.group, kAttnRows) * attn_cost(attn_ceil(s.len, kKvPage));
+  return p.n_kv_head * attn_ceil(n * p.group, RT) * attn_cost(attn_ceil(s.len, kKvPage));
 }
 
 struct AttnPlan {
@@ -137,6 +138,7 @@ struct AttnSeg {
   uint32_t unit;            // partial index without the CTA
 };
 
+template <uint32_t RT>
 __device__ __forceinline__ AttnSeg attn_segment(const KvAttnParams& p, const AttnPlan& pl, const uint32_t* cum,
                                                 uint32_t w, uint32_t w1) {
   AttnSeg s;
@@ -152,7 +154,7 @@ __device__ __forceinline__ AttnSeg attn_segment(const KvAttnParams& p, const Att
     s.base_row = 0;
     s.len = pl.prefix;
     s.n = 0;
-    s.row0 = s.rg * kAttnRows;
+    s.row0 = s.rg * RT;
     s.rows = pl.rows_p * p.group - s.row0;
     s.unit = u;
   } else {
@@ -183,11 +185,11 @@ __device__ __forceinline__ AttnSeg attn_segment(const KvAttnParams& p, const Att
     s.base_row = q.r0;
     s.len = q.len;
     s.n = q.n;
-    s.row0 = s.rg * kAttnRows;
+    s.row0 = s.rg * RT;
     s.rows = n * p.group - s.row0;
     s.unit = lo * p.seq_groups * p.n_kv_head + u;
   }
-  if (s.rows > kAttnRows) s.rows = kAttnRows;
+  if (s.rows > RT) s.rows = RT;
   s.step = attn_cost(tiles) - at;
   if (s.step > w1 - w) s.step = w1 - w;
   s.tile0 = at > kAttnStart ? at - kAttnStart : 0u;
@@ -696,19 +698,25 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 }
 
 // ---- geometry of a CTA ------------------------------------------------------
-template <uint32_t HD>
+// Row groups of 16 (three digits each: N = 48), two CTAs per SM, for few rows: the
+// page copies of four tiles in flight hide each other's latency.  Groups of 32,
+// one CTA per SM, read a page half as often and share a tile's fixed work: 192
+// rows over 65537 tokens 360 -> @@ us, 16 rows would only leave columns empty.
+// (Two CTAs of 32 do not fit the registers; 64 dimensions leave no room for 96
+// rows of probabilities, 256 none for the value sums.)
+template <uint32_t HD, uint32_t RT>
 struct AttnGeo {
   static constexpr uint32_t kBlock = kv_block_bytes(HD);
   static constexpr uint32_t kQRow = HD < 128u ? HD : 128u;      // bytes of an operand row of K and Q
   static constexpr uint32_t kPanels = HD <= 128u ? 1u : HD / 128u;
-  static constexpr uint32_t kQBytes = 3u * kAttnRows * HD;      // a job's query digits
-  static constexpr uint32_t kCtas = HD <= 128u ? 2u : 1u;       // per SM
-  static constexpr uint32_t kStages = HD == 64u ? 5u : 3u;      // as many blocks as shared memory holds
-  static constexpr uint32_t kAcc = 64u;                         // TMEM columns between accumulators (48 used)
-  static constexpr uint32_t kTmem = HD <= 128u ? 256u : 512u;   // scores of two tiles, values of two tiles
-  static constexpr uint32_t kControl = 2048u;  // barriers, scales, maxima; also what a 64-dimension value operand reads past its end
-  static_assert(3u * kAttnRows * kKvPage <= kKvPage * HD, "a tile's probabilities take the place of its keys");
-  static_assert(kAttnRows * HD * 4u <= kBlock, "a job's queries fit a stage");
+  static constexpr uint32_t kQBytes = 3u * RT * HD;      // a job's query digits
+  static constexpr uint32_t kCtas = HD <= 128u && RT == 16u ? 2u : 1u;  // per SM
+  static constexpr uint32_t kStages = HD == 64u || RT == 32u ? 5u : 3u;  // blocks that shared memory holds
+  static constexpr uint32_t kAcc = RT == 16u ? 64u : 128u;      // TMEM columns between accumulators (3 RT used)
+  static constexpr uint32_t kTmem = HD <= 128u ? 4u * kAcc : 512u;  // scores of two tiles, values of two tiles
+  static constexpr uint32_t kControl = RT == 16u ? 2048u : 4096u;  // barriers, scales, maxima; also what a 64-dimension value operand reads past its end
+  static_assert(3u * RT * kKvPage <= kKvPage * HD, "a tile's probabilities take the place of its keys");
+  static_assert(RT * HD * 4u <= kBlock, "a job's queries fit a stage");
   static constexpr uint32_t smem(uint32_t n_seq) {
     return kQBytes + kStages * kBlock + kControl + ((n_seq + 1u) * 4u + 15u) / 16u * 16u + 1024u;
   }
@@ -727,10 +735,10 @@ struct AttnBars {
   AttnJob job[2];
 };
 
-template <uint32_t HD>
-__global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kernel(const KvAttnParams p) {
-  using G = AttnGeo<HD>;
-  constexpr uint32_t RT = kAttnRows, S = G::kStages;
+template <uint32_t HD, uint32_t RT>
+__global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_attn_kernel(const KvAttnParams p) {
+  using G = AttnGeo<HD, RT>;
+  constexpr uint32_t S = G::kStages;
   constexpr uint32_t NC = RT / 8u;                           // column chunks of 8
   constexpr uint32_t MH = HD <= 128u ? 1u : HD / 128u;       // value products of 128 dimensions
   extern __shared__ uint8_t attn_smem_raw[];
@@ -789,7 +797,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     for (uint32_t i0 = 0; i0 < p.rows.n_seq; i0 += 32u) {
       uint32_t w = 0;
       const bool in = i0 + lane < p.rows.n_seq;
-      if (in && p.seq_few == 0) w = attn_seq_work(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
+      if (in && p.seq_few == 0) w = attn_seq_work<RT>(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
       uint32_t c = w;
 #pragma unroll
       for (uint32_t o = 1; o < 32u; o <<= 1) {
@@ -826,7 +834,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     for (bool more = true; more && live; ++nj) {
       AttnSeg s{};
       while (w < w1) {  // the next piece that holds a tile
-        s = attn_segment(p, pl, cum, w, w1);
+        s = attn_segment<RT>(p, pl, cum, w, w1);
         w += s.step;
         if (s.tiles > 0) break;
       }
@@ -1001,7 +1009,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
     const uint32_t quad = warp & 3u, half = warp >> 2, g = lane >> 2, cq = lane & 3u;
     uint32_t x = 0;               // stages used before the job
     uint32_t n_own = 0, n_other = 0;  // tiles of this half and of the other before the job
-    // job n's queries (in stage y) as three signed digits each, rows warp, warp + 8
+    // job n's queries (in stage y) as three signed digits each, rows warp, warp + 8, ...
     auto prepare = [&](uint32_t n, uint32_t y) {
       if (!__all_sync(0xffffffffu, attn_wait(&bar.full[y % S], (y / S) & 1u))) return false;
       const uint32_t rows = bar.job[n & 1u].rows;
@@ -1054,7 +1062,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
       if (!live) break;
       const AttnJob s = bar.job[nj & 1u];
       if (s.tiles == 0) break;
-      const uint32_t nact = s.rows > 8u ? 2u : 1u;  // chunks of 8 columns in use
+      const uint32_t nact = (s.rows + 7u) / 8u;  // chunks of 8 columns in use
       // this thread's columns 8 y + 2 cq + {0, 1}
       float2 qsc[NC], m[NC], l[NC], f[NC], o[NC][MH][4];
 #pragma unroll
@@ -1280,6 +1288,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
   }
   attn_fence_before();
   __syncthreads();
+  pdl_wait();  // the few-rows kernels before this one, see attn_line
   if (warp == 9)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kTmem) : "memory");
 }
@@ -1289,7 +1298,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnGeo<HD>::kCtas) kv_attn_kern
 // order of the sums is the line's, so results do not depend on timing.
 template <uint32_t HD>
 __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) {
-  constexpr uint32_t E = HD / 32u, RT = kAttnRows;
+  constexpr uint32_t E = HD / 32u;
+  const uint32_t RT = p.rt;
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t x = (uint64_t)blockIdx.x * 2u + (threadIdx.x >> 5);
   if (x >= (uint64_t)p.rows.n_rows * p.n_head) return;  // warp-uniform
@@ -1421,7 +1431,7 @@ namespace {
 // kernels); and where their partials sit.
 struct AttnSplit {
   size_t plan, po, pml, so, sml, bytes;
-  uint32_t prefix_cap, seq_cap, seq_groups;
+  uint32_t rt, prefix_cap, seq_cap, seq_groups;
   uint32_t prefix_few, prefix_ctas, seq_few, seq_ctas;
   bool line;
 };
@@ -1438,9 +1448,15 @@ void attn_clusters(uint64_t units, uint32_t pages, uint32_t& clusters, uint32_t&
   clusters = (uint32_t)(most < by_pages ? most : by_pages);
   if (clusters < 1u) clusters = 1u;
 }
+// Rows of the line's groups: 32 where a unit has more than 16 (128 dimensions).
+uint32_t attn_rt(const KvPool& kv, const KvAttnBatch& b, uint32_t group) {
+  const uint64_t rows = (uint64_t)(b.max_prefix > 0 ? b.n_rows : b.max_rows) * group;
+  return kv.head_dim == 128u && rows > 16u ? 32u : 16u;
+}
 AttnSplit attn_split(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
-  const uint32_t group = n_head / kv.n_kv_head, rt = kAttnRows;
+  const uint32_t group = n_head / kv.n_kv_head, rt = attn_rt(kv, b, group);
   AttnSplit s{};
+  s.rt = rt;
   auto put = [&](uint64_t parts, uint32_t cap, size_t& o, size_t& ml) {
     o = s.bytes;
     s.bytes += (parts * cap * kv.head_dim * 4u + 255u) & ~(size_t)255u;
@@ -1499,9 +1515,34 @@ cudaError_t attn_few_rows(const KvAttnParams& p, uint32_t prefix, uint32_t rows,
   return attn_few<HD, 4>(p, prefix, direct, st);
 }
 
+template <uint32_t HD, uint32_t RT>
+cudaError_t attn_line(const KvAttnParams& p, int num_sms, uint64_t work, cudaStream_t st) {
+  using G = AttnGeo<HD, RT>;
+  static SmemAttr attr;
+  cudaError_t e = ensure_smem_attr((const void*)kv_attn_kernel<HD, RT>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
+  if (e != cudaSuccess) return e;
+  uint64_t grid = (uint64_t)G::kCtas * (uint32_t)num_sms;
+  if (grid > kAttnMaxCtas) grid = kAttnMaxCtas;
+  if (grid > work) grid = work;
+  if (grid == 0) grid = 1;
+  // may start while the few-rows kernels of this call run (it reads nothing of
+  // theirs) and waits for them at its end, so that the joining kernel, which
+  // waits for this one, waits for all
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((uint32_t)grid);
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.dynamicSmemBytes = G::smem(p.rows.n_seq);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = p.seq_few > 0 || p.prefix_few > 0 ? 1 : 0;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_attn_kernel<HD, RT>, p);
+}
+
 template <uint32_t HD>
 cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t work, cudaStream_t st) {
-  using G = AttnGeo<HD>;
   cudaError_t e = cudaSuccess;
   const bool alone = p.max_prefix == 0 && p.seq_few == 1u;  // nothing to join
   if (p.seq_few > 0) e = attn_few_rows<HD>(p, 0, p.seq_cap, alone ? 1u : 0u, st);
@@ -1509,17 +1550,13 @@ cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t 
   if (p.prefix_few > 0) e = attn_few_rows<HD>(p, 1, p.prefix_cap, 0u, st);
   if (e != cudaSuccess) return e;
   if (line) {
-    static SmemAttr attr;
-    e = ensure_smem_attr((const void*)kv_attn_kernel<HD>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
+    if constexpr (HD == 128) {
+      e = p.rt == 32u ? attn_line<HD, 32>(p, num_sms, work, st) : attn_line<HD, 16>(p, num_sms, work, st);
+    } else {
+      e = attn_line<HD, 16>(p, num_sms, work, st);
+    }
     if (e != cudaSuccess) return e;
-    uint64_t grid = (uint64_t)G::kCtas * (uint32_t)num_sms;
-    if (grid > kAttnMaxCtas) grid = kAttnMaxCtas;
-    if (grid > work) grid = work;
-    if (grid == 0) grid = 1;
-    kv_attn_kernel<HD><<<(uint32_t)grid, kAttnThreads, G::smem(p.rows.n_seq), st>>>(p);
   }
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((uint32_t)(((uint64_t)p.rows.n_rows * p.n_head + 1u) / 2u));
   cfg.blockDim = dim3(64);
@@ -1540,7 +1577,7 @@ size_t kv_attn_scratch_bytes(const KvPool& kv, const KvAttnBatch& b, uint32_t n_
 
 // The line of tiles of the largest lengths (its words are 32-bit).
 uint64_t kv_attn_work_bound(const KvPool& kv, const KvAttnBatch& b, uint32_t n_head) {
-  const uint32_t group = n_head / kv.n_kv_head, rt = kAttnRows;
+  const uint32_t group = n_head / kv.n_kv_head, rt = attn_rt(kv, b, group);
   const uint64_t tp = (b.max_prefix + kKvPage - 1u) / kKvPage, ts = (b.max_len + kKvPage - 1u) / kKvPage;
   const uint64_t rp = ((uint64_t)b.n_rows * group + rt - 1u) / rt;
   uint64_t rs = (uint64_t)b.n_seq * (((uint64_t)b.max_rows * group + rt - 1u) / rt);
@@ -1584,6 +1621,7 @@ cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* 
   p.pml = reinterpret_cast<float*>(ws + s.pml);
   p.so = reinterpret_cast<float*>(ws + s.so);
   p.sml = reinterpret_cast<float*>(ws + s.sml);
+  p.rt = s.rt;
   p.prefix_cap = s.prefix_cap;
   p.seq_cap = s.seq_cap;
   p.seq_groups = s.seq_groups;
