@@ -671,17 +671,27 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
   attn_cluster_sync();  // no CTA leaves while its sums are read
 }
 
-// mbar_wait, reading the clock only once in 64 polls: its read takes longer
-// than a tile's waits.
+// mbar_wait whose polls may sleep up to 20 us each (until the phase completes)
+// and which reads the clock only after sixteen: a warp that waits leaves the
+// issue slots to the others.
+__device__ __forceinline__ bool attn_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < 64u; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
+  for (uint32_t i = 0; i < 16u; ++i)
+    if (attn_try(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
-  for (;;) {
-    for (uint32_t i = 0; i < 64u; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+  while (!attn_try(bar, parity))
     if (global_timer_ns() - t0 > EOS_WAIT_LIMIT_NS) return false;
-  }
+  return true;
 }
 
 // One look at a barrier, without waiting.
@@ -988,7 +998,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
           if (moved) {
             polls = 0;
             t0 = 0;
-          } else if (++polls % 256u == 0) {  // bounded, like every wait
+          } else if (__nanosleep(20), ++polls % 256u == 0) {  // bounded, like every wait
             const uint64_t now = global_timer_ns();
             if (t0 == 0) t0 = now;
             if (now - t0 > EOS_WAIT_LIMIT_NS) {
