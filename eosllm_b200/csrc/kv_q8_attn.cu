@@ -6,41 +6,49 @@
 //   tokens 0 .. len_i - n_i + t;  out = sum_j softmax(S)_j v_j;  no token
 //   visible: out = 0.
 //
+// A unit is (kv head, rows that see the same pages): the prefix with the rows of
+// all sequences, and each sequence's own pages with its rows.  Units of up to
+// kFewRows rows run as integer dot products on the CUDA cores
+// (kv_attn_few_kernel), larger ones on the tensor cores (kv_attn_kernel);
+// kv_attn_join_kernel joins what they leave of a row: maximum, sum,
+// unnormalised output.  Lengths live on the device and every kernel reads them
+// there, so a captured call follows them.
+//
 // Arithmetic.  Keys and values stay the integers they are in the cache: a
 // query row is scaled to integers of 24 bits and split into three signed
-// 8-bit digits, a tile's probabilities (times the value scales) are integers
-// of 23 bits split into three unsigned ones, and both products are
-// tcgen05.mma kind::i8 with exact s32 sums -- no conversion of the cache, no
-// 16-bit rounding anywhere.  The digits are further columns of the same
-// product (N = 3 rows), so a page of keys is one M = 128 (tokens) operand and
-// a page of values one M = 128 (dimensions) operand whatever the number of
-// rows.  s32 to f32: |sum| < 2^22, so sum + (bits of 1.5 2^23) is a float 1.5
-// 2^23 + sum (an integer add and an f32 add, not the conversion pipe).  A
-// probability p times weight w becomes an integer as the mantissa of the
-// float 2^23 + p w, whose three low bytes are the digits.
+// 8-bit digits, a tile's probabilities (times the value scales) become integers
+// of 23 bits, relative to the tile's own maximum, in three unsigned digits, and
+// every product has exact s32 sums -- no conversion of the cache, no 16-bit
+// rounding anywhere.  A probability p times weight w becomes an integer as the
+// mantissa of the float 2^23 + p w, whose three low bytes are the digits.
 //
 // Scores are compared before the row's query scale and the softmax scale are
 // applied (z = sum * key scale), and the exponent is fma(z, c, -reference): a
-// rounding of c or of the reference is common to the row and cancels.
+// rounding of c or of the reference is common to the row and cancels.  One
+// pass with a running maximum and sum per row in f32; each tile's value sums
+// are folded into f32 registers.
 //
-// One pass with a running maximum and sum per row; each tile's product is
-// folded into f32 registers, so rounding does not grow with the number of
-// tokens beyond an f32 sum over tiles.
+// On the tensor cores the products are tcgen05.mma kind::i8.  The digits are
+// further columns of the same product (N = 3 rows), so a page of keys is one M
+// = 128 (tokens) operand and a page of values one M = 128 (dimensions) operand
+// whatever the number of rows, both as the cache holds them: a page is copied
+// to shared memory and multiplied.  s32 to f32: |sum| < 2^22, so sum + (bits of
+// 1.5 2^23) is a float 1.5 2^23 + sum (an integer and an f32 addition, not the
+// conversion pipe).  The units' tiles (pages) form one line, cut into equal
+// pieces, one per CTA, whatever the mixture of lengths; every CTA computes the
+// line's layout from the lengths.  Joining the digits and the softmax bound it
+// (about 35 instructions per pair of score and output; 48 rows x 4 heads over
+// 65537 tokens: 312 us, memory alone 27); for few rows over a long prefix the
+// page copies do (8 rows over 16384 tokens of 32 heads: 51 us, memory alone
+// 21), and for small calls the chain launch - lengths - table - page.
+// Widening the cache to f16 and multiplying hi and lo halves needs no joining,
+// but the widening and splitting cost as much (340 us, and 112 us for the 8
+// rows).
 //
-// Work split.  A unit is (kv head, group of up to RT rows, the pages they
-// see): the prefix with all rows of all sequences (its pages are read once
-// per row group), and each sequence's own pages with its rows.  The units'
-// tiles (pages) form one line, cut into equal pieces, one per CTA, whatever
-// the mixture of lengths; a CTA's piece of a unit leaves a partial (maximum,
-// sum, unnormalised output) per row, and a second kernel joins a row's
-// partials.  Lengths live on the device: every CTA computes the line's layout
-// from them, so a captured call follows them.
-//
-// A CTA: warps 0..7 score and fold, warp 8 copies pages (bulk copies, one for
-// a whole page), warp 9 issues the products.  The score product of a tile is
-// issued before the value product of the tile before it, so the tensor core
-// works while the softmax does.  A tile's probabilities take the place of its
-// keys in shared memory.
+// A CTA: warps 0..7 score and fold -- four on the even tiles of a piece, four on
+// the odd ones, so that one half's chain of waits is the other's work --, warp
+// 8 copies pages, warp 9 issues the products, whichever is ready first.  A
+// tile's probabilities take the place of its keys in shared memory.
 #include "eos_kernels.h"
 #include "kv_q8.cuh"
 
@@ -331,12 +339,15 @@ __device__ __forceinline__ float attn_warp_max(float x) {
 // the length turns out to be, all of them have their share.  A cluster joins
 // its CTAs' sums through shared memory, so a unit on one cluster is done with
 // one launch.  Reading the cache is what bounds it: 2 HD + 8 bytes per token
-// against 6 HD / 4 dp4a per token and row, so up to four rows stay below the
-// memory's time.  No barrier or tensor memory to set up and several CTAs per
+// against 7 HD / 4 dp4a per token and row, so a few rows stay near the
+// memory's time (one row over 16000 tokens of 32 heads: 27.5 us, 4.9 TB/s).  No barrier or tensor memory to set up and several CTAs per
 // SM, each with a page's loads in flight: units of a page or two (a
 // sequence's own tokens, a decode step) take one round trip to memory.
 // Queries as in the tensor-core kernel, probabilities with 8 bits more; s32 sums
 // over 16 dimensions (scores) and over a page (values) are exact.
+// 8 rows over 16384 tokens of 32 heads took 138 us here and 51 on the tensor
+// cores; of 1536 units of four rows, 23 here and about 17 there next to a large
+// prefix, but 5 us against 10 alone.
 constexpr uint32_t kFewRows = 4;
 constexpr uint32_t kFewThreads = 128;
 
@@ -403,16 +414,16 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
   pdl_trigger();
   if (rows == 0) return;  // the whole cluster
   const int32_t seen0 = (int32_t)s.len - (int32_t)s.n + 1;  // tokens a sequence's first row sees (may be negative)
-  // warp r: row r's digits
-  if (warp < R) {
+  // the rows' digits, warp w those of rows w, w + 4
+  for (uint32_t row = warp; row < R; row += 4u) {
     float scale = 0.0f;
     constexpr uint32_t QF = HD <= 128u ? 1u : HD / 128u;
     uint32_t d[QF][3];
 #pragma unroll
     for (uint32_t c = 0; c < QF; ++c) d[c][0] = d[c][1] = d[c][2] = 0u;
-    if (warp < rows) {
-      const uint32_t xr = attn_div(warp, p.by_group);
-      const float* src = p.q + (size_t)(s.r0 + xr) * p.q_stride + (size_t)(g * p.group + warp - xr * p.group) * HD;
+    if (row < rows) {
+      const uint32_t xr = attn_div(row, p.by_group);
+      const float* src = p.q + (size_t)(s.r0 + xr) * p.q_stride + (size_t)(g * p.group + row - xr * p.group) * HD;
       float4 v[QF];
       uint32_t amax = 0;
 #pragma unroll
@@ -431,26 +442,12 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
     for (uint32_t c = 0; c < QF; ++c)
       if (HD >= 128u || lane < HD / 4u)
 #pragma unroll
-        for (uint32_t e = 0; e < 3u; ++e) qd[warp][e][c * 32u + lane] = d[c][e];
-    if (lane == 0) qscale[warp] = scale;
+        for (uint32_t e = 0; e < 3u; ++e) qd[row][e][c * 32u + lane] = d[c][e];
+    if (lane == 0) qscale[row] = scale;
   }
   __syncthreads();
   // score side: lane's chunk of the key rows, tokens 32 warp + i (32 / CL) + lane / CL
   const uint32_t lc = lane % CL, lt = lane / CL;
-  uint32_t qw[R][3][4];
-  float qsc[R];
-#pragma unroll
-  for (uint32_t r = 0; r < R; ++r) {
-    qsc[r] = qscale[r];
-#pragma unroll
-    for (uint32_t e = 0; e < 3u; ++e) {
-      const uint4 v = *reinterpret_cast<const uint4*>(&qd[r][e][lc * 4u]);
-      qw[r][e][0] = v.x;
-      qw[r][e][1] = v.y;
-      qw[r][e][2] = v.z;
-      qw[r][e][3] = v.w;
-    }
-  }
   // after the reduction over the CL lanes of a token, this lane holds token `own`
   const uint32_t own = warp * 32u + lc * (32u / CL) + lt;
   // value side: this thread's dimension(s) and quarters
@@ -506,15 +503,18 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
       float part[CL];
+      uint4 qw[3];
+#pragma unroll
+      for (uint32_t e = 0; e < 3u; ++e) qw[e] = *reinterpret_cast<const uint4*>(&qd[r][e][lc * 4u]);
 #pragma unroll
       for (uint32_t i = 0; i < CL; ++i) {
         int32_t a[3];
 #pragma unroll
         for (uint32_t e = 0; e < 3u; ++e) {
-          a[e] = __dp4a((int)kw[i].x, (int)qw[r][e][0], 0);
-          a[e] = __dp4a((int)kw[i].y, (int)qw[r][e][1], a[e]);
-          a[e] = __dp4a((int)kw[i].z, (int)qw[r][e][2], a[e]);
-          a[e] = __dp4a((int)kw[i].w, (int)qw[r][e][3], a[e]);
+          a[e] = __dp4a((int)kw[i].x, (int)qw[e].x, 0);
+          a[e] = __dp4a((int)kw[i].y, (int)qw[e].y, a[e]);
+          a[e] = __dp4a((int)kw[i].z, (int)qw[e].z, a[e]);
+          a[e] = __dp4a((int)kw[i].w, (int)qw[e].w, a[e]);
         }
         // below 2^18 each: (a2 2^8 + a1) is exact in s32; a0 / 256 joins as a float
         part[i] = fmaf((float)a[0], 1.0f / 256.0f, (float)(a[2] * 256 + a[1]));
@@ -549,11 +549,11 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
       const float mt = fmaxf(fmaxf(rd[0][r], rd[1][r]), fmaxf(rd[2][r], rd[3][r]));
-      const float nm = fmaxf(mt == -INFINITY ? mt : __fmul_ru(mt, qsc[r]), m[r]);
+      const float nm = fmaxf(mt == -INFINITY ? mt : __fmul_ru(mt, qscale[r]), m[r]);
       const float neg = nm == -INFINITY ? 0.0f : -nm;
       f[r] = attn_ex2(m[r] + neg);
       m[r] = nm;
-      const float e = attn_ex2(fmaf(z[r], qsc[r], neg));
+      const float e = attn_ex2(fmaf(z[r], qscale[r], neg));
       l[r] = fmaf(l[r], f[r], e);  // this token's share
       // e vs as 23 bits (the low bytes of 2^23 + ..) and a signed byte of what is left, in 1 / 256
       const float y = vs * up, b = fmaf(e, y, 8388608.0f), rest = fmaf(e, y, 8388608.0f - b);
@@ -711,7 +711,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // Row groups of 16 (three digits each: N = 48), two CTAs per SM, for few rows: the
 // page copies of four tiles in flight hide each other's latency.  Groups of 32,
 // one CTA per SM, read a page half as often and share a tile's fixed work: 192
-// rows over 65537 tokens 360 -> @@ us, 16 rows would only leave columns empty.
+// rows over 65537 tokens 346 -> 314 us; with 16 rows half its columns would be empty.
 // (Two CTAs of 32 do not fit the registers; 64 dimensions leave no room for 96
 // rows of probabilities, 256 none for the value sums.)
 template <uint32_t HD, uint32_t RT>

@@ -281,9 +281,10 @@ EOSLLM_CUDA_API int eosi_cuda_kv_q8_read_dev(const eosi_cuda_kv_q8_t *kv, float 
  * and at least n_head * head_dim); rows of out behind the last sequence stay
  * as they were.  n_head is a multiple of kv->n_kv_head.
  * f32 in, f32 out: q is held as 24-bit integers (scaled by its row's
- * maximum), a row's probabilities as 23-bit integers, products and sums of
- * both with the int8 cache are exact integers, and the softmax statistics are
- * f32.  Results do not depend on timing.  A query row or a visible cache row
+ * maximum), a page's probabilities as integers of 23 bits or more (relative to
+ * the page's largest), products and sums of both with the int8 cache are exact
+ * integers, and the softmax statistics are f32.  Results do not depend on
+ * timing.  A query row or a visible cache row
  * that holds a NaN or an infinity gives a row of NaN.
  * scratch: eosi_cuda_kv_q8_attn_scratch_bytes(kv, batch, n_head) bytes, 16-byte
  * aligned, not shared by calls that may overlap. */
