@@ -345,9 +345,10 @@ __device__ __forceinline__ float attn_warp_max(float x) {
 // sequence's own tokens, a decode step) take one round trip to memory.
 // Queries as in the tensor-core kernel, probabilities with 8 bits more; s32 sums
 // over 16 dimensions (scores) and over a page (values) are exact.
-// 8 rows over 16384 tokens of 32 heads took 138 us here and 51 on the tensor
-// cores; of 1536 units of four rows, 23 here and about 17 there next to a large
-// prefix, but 5 us against 10 alone.
+// Measured both ways: 8 rows over 16384 tokens of 32 heads 138 us here, 51 on the
+// tensor cores; 384 units of four rows (up to 700 tokens) beside a prefix of
+// 65537, in all 312 us with them here, 306 with them there; one row over 640
+// tokens of 32 heads 4.9 us here (one launch), 10 there.
 constexpr uint32_t kFewRows = 4;
 constexpr uint32_t kFewThreads = 128;
 

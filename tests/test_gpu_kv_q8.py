@@ -342,6 +342,66 @@ def test_graph_replay_follows_lengths_and_tables(gpu):
     assert full_lens == [64, 200]
 
 
+def test_write_attend_verify_in_one_graph(gpu):
+    """A decode step of four sequences -- rows written, attention over the shared
+    prefix, drafts verified -- captured once and replayed as they grow."""
+    import torch
+    from kv_q8_oracle import verify
+    H, kvh, hd, V, n, k = 8, 4, 64, 96, 4, 2
+    rng = np.random.default_rng(77)
+    b = Batch(gpu, H, kvh, hd, 150, [140] * n, [k] * n, seed=31)
+    c = b.c
+    head = torch.from_numpy(rng.standard_normal((H * hd, V)).astype(np.float32)).cuda()
+    new_k = torch.zeros(n * k, kvh, hd, device="cuda")
+    new_v = torch.zeros_like(new_k)
+    pos, drafts = c.i32([0] * n), c.i32(rng.integers(0, V, n))
+    qp = torch.softmax(torch.from_numpy(rng.standard_normal((n, 1, V)).astype(np.float32)).cuda(), -1)
+    u = torch.zeros(n, k, device="cuda")
+    probs = torch.zeros(n, k, V, device="cuda")
+    tok, cnt = torch.zeros(n, k, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+
+    def step(stream):
+        gpu.kv_q8_write_dev(c.pool, new_k, new_v, kvh * hd, n * k, b.row0, b.tab, c.width, pos, n, stream=stream)
+        b.run(stream=stream)
+        probs.copy_(torch.softmax(b.out[:n * k].view(n * k, -1) @ head, -1).view(n, k, V))
+        gpu.verify_draft_dev(probs, qp, V, drafts, None, k - 1, u, n, V, tok, cnt, stream=stream)
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step(s.cuda_stream)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        step(torch.cuda.current_stream().cuda_stream)
+    lens = [100, 126, 127, 64]
+    base_k, base_v = [x.copy() for x in b.ks], [x.copy() for x in b.vs]
+    for x in base_k + base_v:
+        x[:k] = 0  # the pass before the capture wrote its zeros at position 0
+    for it in range(3):
+        kk = rng.standard_normal((n * k, kvh, hd)).astype(np.float32)
+        vv = rng.standard_normal((n * k, kvh, hd)).astype(np.float32)
+        un = rng.random((n, k)).astype(np.float32)
+        new_k.copy_(torch.from_numpy(kk))
+        new_v.copy_(torch.from_numpy(vv))
+        u.copy_(torch.from_numpy(un))
+        pos.copy_(c.i32(lens))
+        b.len_d.copy_(c.i32([x + k for x in lens]))
+        g.replay()
+        torch.cuda.synchronize()
+        for i in range(n):
+            base_k[i][lens[i]:lens[i] + k] = kk[i * k:(i + 1) * k]
+            base_v[i][lens[i]:lens[i] + k] = vv[i * k:(i + 1) * k]
+        b.ks = [base_k[i][:lens[i] + k] for i in range(n)]
+        b.vs = [base_v[i][:lens[i] + k] for i in range(n)]
+        want, tol = b.want()
+        assert np.all(np.abs(b.out[:n * k].cpu().numpy() - want) <= tol)
+        got = verify(probs.cpu().numpy(), qp.cpu().numpy(), drafts.cpu().numpy().reshape(n, 1), [k - 1] * n, un)
+        for i in range(n):
+            assert int(cnt[i]) == len(got[i]) and list(tok[i, :len(got[i])].cpu().numpy()) == got[i]
+        lens = [x + k for x in lens]
+    assert gpu.take_device_errors() == 0
+
+
 def test_two_calls_at_once_with_their_own_scratch(gpu):
     import torch
     a = Batch(gpu, 8, 4, 128, 2000, [100] * 4, [1] * 4, seed=21)

@@ -100,3 +100,11 @@ def test_verify_refusals(cuda_lib, buf):
                dict(stride=99), dict(vocab=0), dict(kk=1 << 20)):
         assert st(**kw) == B.EOS_E_INVALID_ARG, kw
     assert st(n_seq=0) == B.EOS_OK
+
+
+def test_decoder_refusals_without_a_decoder(cuda_lib):
+    for name, args in (("eosi_cuda_text_set_cache", (None, 1)), ("eosi_cuda_text_fork", (None, 2, 4, 0)),
+                       ("eosi_cuda_text_branch_step", (None, None, 0, None, None, 1.0, None, None)),
+                       ("eosi_cuda_text_branch_adopt", (None, 0)), ("eosi_cuda_text_branch_close", (None,))):
+        assert getattr(cuda_lib, name)(*args) == B.EOS_E_INVALID_ARG, name
+    assert cuda_lib.eosi_cuda_text_cache(None) == 0
