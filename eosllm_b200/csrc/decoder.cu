@@ -1567,6 +1567,8 @@ int TextDecoder::set_cache(int mode) {
   const uint32_t pages = (m.max_ctx + kKvPage - 1u) / kKvPage;
   const size_t layer = (size_t)pages * kvl * kv_block_bytes(hd);
   const size_t kv_bytes = 4ull * m.n_layer * m.max_ctx * kvl * hd;
+  std::vector<uint32_t> id(want ? pages : 0u);
+  for (uint32_t i = 0; i < id.size(); ++i) id[i] = i;
   if (want) {  // the new cache first: a failure leaves the decoder as it was
     q8_pages = pages;
     q8_layer = layer;
@@ -1580,8 +1582,6 @@ int TextDecoder::set_cache(int mode) {
     if (e == cudaSuccess) e = alloc(&q8_words, 16);
     if (e == cudaSuccess) e = alloc(&q8_attn, 4ull * m.n_embd * (prefill_ok() ? pass_rows() : 1u));
     if (e == cudaSuccess) e = alloc(&q8_scratch, scratch);
-    std::vector<uint32_t> id(pages);
-    for (uint32_t i = 0; i < pages; ++i) id[i] = i;
     if (e == cudaSuccess) e = cudaMemcpyAsync(q8_table, id.data(), 4ull * pages, cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   } else {
@@ -2077,7 +2077,13 @@ EOSLLM_CUDA_API int eosi_cuda_text_step_mode(const eosi_cuda_text_t* t) {
 }
 
 EOSLLM_CUDA_API int eosi_cuda_text_set_cache(eosi_cuda_text_t* t, int mode) {
-  return t ? t->d.set_cache(mode) : EOS_E_INVALID_ARG;
+  if (t == nullptr) return EOS_E_INVALID_ARG;
+  try {
+    return t->d.set_cache(mode);
+  } catch (const std::bad_alloc&) {
+    eos::set_error_message("cuda text: out of host memory");
+    return EOS_E_OUT_OF_MEMORY;
+  }
 }
 
 EOSLLM_CUDA_API int eosi_cuda_text_cache(const eosi_cuda_text_t* t) {
@@ -2085,7 +2091,14 @@ EOSLLM_CUDA_API int eosi_cuda_text_cache(const eosi_cuda_text_t* t) {
 }
 
 EOSLLM_CUDA_API int eosi_cuda_text_fork(eosi_cuda_text_t* t, uint32_t n_seq, uint32_t max_new, uint32_t max_draft) {
-  return t ? t->d.fork(n_seq, max_new, max_draft) : EOS_E_INVALID_ARG;
+  if (t == nullptr) return EOS_E_INVALID_ARG;
+  try {
+    return t->d.fork(n_seq, max_new, max_draft);
+  } catch (const std::bad_alloc&) {
+    t->d.close_branches();
+    eos::set_error_message("cuda text: out of host memory");
+    return EOS_E_OUT_OF_MEMORY;
+  }
 }
 
 EOSLLM_CUDA_API int eosi_cuda_text_branch_step(eosi_cuda_text_t* t, const uint32_t* tokens, uint32_t n_draft,

@@ -1039,7 +1039,7 @@ int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t* kv, const eosi_cuda_attn_b
 int eosi_cuda_verify_draft_dev(const float* p, const float* q, uint64_t stride, const uint32_t* drafts,
                                const uint32_t* n_draft, uint32_t max_draft, const float* u, uint32_t n_seq,
                                uint32_t n_vocab, uint32_t* tokens, uint32_t* n_tokens, void* stream) {
-  if (n_vocab == 0 || stride < n_vocab || max_draft > 65535u)
+  if (n_vocab == 0 || n_vocab > INT32_MAX || stride < n_vocab || max_draft > 65535u)
     return fail(EOS_E_INVALID_ARG, "verify: n_vocab=%u stride=%llu max_draft=%u", n_vocab, (unsigned long long)stride,
                 max_draft);
   if (n_seq == 0) return EOS_OK;

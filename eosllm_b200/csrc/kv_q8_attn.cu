@@ -1555,6 +1555,7 @@ cudaError_t attn_line(const KvAttnParams& p, int num_sms, uint64_t work, cudaStr
 template <uint32_t HD>
 cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t work, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
+  const bool first = !line && p.seq_few == 0 && p.prefix_few == 0;
   const bool alone = p.max_prefix == 0 && p.seq_few == 1u;  // nothing to join
   if (p.seq_few > 0) e = attn_few_rows<HD>(p, 0, p.seq_cap, alone ? 1u : 0u, st);
   if (alone || e != cudaSuccess) return e;
@@ -1574,7 +1575,9 @@ cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t 
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  // it reads row0 and seq_len before it waits: early only behind this call's own
+  // kernels, which started when the inputs were there
+  at[0].val.programmaticStreamSerializationAllowed = first ? 0 : 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<HD>, p);

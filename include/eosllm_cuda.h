@@ -278,8 +278,8 @@ EOSLLM_CUDA_API int eosi_cuda_kv_q8_read_dev(const eosi_cuda_kv_q8_t *kv, float 
  * pointers may be NULL).  max_len <= 128 * table_stride.  The prefix's pages
  * are read once for all sequences.  Row r, head h of q and out is at
  * r * stride + h * head_dim floats (16-byte aligned, strides multiples of 4
- * and at least n_head * head_dim); rows of out behind the last sequence stay
- * as they were.  n_head is a multiple of kv->n_kv_head.
+ * and at least n_head * head_dim); rows of out outside every sequence stay as
+ * they were, and out does not overlap q.  n_head is a multiple of kv->n_kv_head.
  * f32 in, f32 out: q is held as 24-bit integers (scaled by its row's
  * maximum), a page's probabilities as integers of 23 bits or more (relative to
  * the page's largest), products and sums of both with the int8 cache are exact
@@ -318,7 +318,8 @@ EOSLLM_CUDA_API int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t *kv, const 
  * tokens[i * (max_draft + 1) ...] gets the accepted tokens and the drawn one,
  * n_tokens[i] of them, and 0xffffffff behind them (a row without any weight
  * draws no token).  max_draft = 0 draws one token from p alone (q and drafts
- * may be NULL). */
+ * may be NULL).  n_vocab < 2^31, max_draft <= 65535; p and q rows on 16-byte
+ * boundaries (stride a multiple of 4) are read in wide loads, others work too. */
 EOSLLM_CUDA_API int eosi_cuda_verify_draft_dev(const float *p, const float *q, uint64_t stride,
                                                const uint32_t *drafts, const uint32_t *n_draft, uint32_t max_draft,
                                                const float *u, uint32_t n_seq, uint32_t n_vocab, uint32_t *tokens,

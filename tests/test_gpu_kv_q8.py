@@ -402,6 +402,57 @@ def test_write_attend_verify_in_one_graph(gpu):
     assert gpu.take_device_errors() == 0
 
 
+@pytest.mark.parametrize("counts,prefix", [([1, 2], 0), ([1, 1], 300), ([9, 40], 300), ([70, 3], 0)])
+def test_rows_before_the_first_sequence(gpu, counts, prefix):
+    """row0[0] > 0: rows that belong to nobody, in front."""
+    import torch
+    b = Batch(gpu, 4, 2, 128, prefix, [130, 50], counts, seed=23)
+    skip = 5
+    n = sum(counts)
+    b.qd = torch.cat([torch.ones(skip, 4, 128, device="cuda"), b.qd])
+    b.out = torch.full((skip + n + 2, 4, 128), 3.0, device="cuda")
+    b.row0 = b.c.i32(np.concatenate([[0], np.cumsum(counts)]) + skip)
+    b.batch = gpu.attn_batch(prefix_table=b.ptab, prefix_len=b.plen, max_prefix=prefix, table=b.tab,
+                             table_stride=b.c.width, seq_len=b.len_d, max_len=130, row0=b.row0, n_seq=2,
+                             n_rows=skip + n + 2, max_rows=max(counts))
+    b.qd = torch.cat([b.qd, b.qd[:2]])
+    b.scratch = torch.empty(gpu.kv_q8_attn_scratch_bytes(b.c.pool, b.batch, 4), dtype=torch.uint8, device="cuda")
+    b.run()
+    got = b.out.cpu().numpy()
+    want, tol = b.want()
+    assert np.all(got[:skip] == 3.0) and np.all(got[skip + n:] == 3.0)
+    assert np.all(np.abs(got[skip:skip + n] - want) <= tol)
+    # and the rows written: those of the sequences only
+    k = torch.randn(skip + n + 2, 2, 128, device="cuda")
+    pos = b.c.i32([40, 1])
+    gpu.kv_q8_write_dev(b.c.pool, k, -k, 256, skip + n + 2, b.row0, b.tab, b.c.width, pos, 2)
+    rk, rv = torch.full_like(k, 3.0), torch.full_like(k, 3.0)
+    gpu.kv_q8_read_dev(b.c.pool, rk, rv, 256, skip + n + 2, b.row0, b.tab, b.c.width, pos, 2)
+    for got, x in ((rk, k), (rv, -k)):
+        got = got.cpu().numpy()
+        assert np.array_equal(got[skip:skip + n], stored(x.cpu().numpy())[0][skip:skip + n])
+        assert np.all(got[:skip] == 3.0) and np.all(got[skip + n:] == 3.0)
+    assert gpu.take_device_errors() == 0
+
+
+def test_nothing_to_attend_to_follows_its_inputs(gpu):
+    """No prefix and no own tokens: zeros, with row0 written just before."""
+    import torch
+    b = Batch(gpu, 4, 2, 64, 0, [1, 1], [2, 3], seed=2)
+    batch = gpu.attn_batch(table=b.tab, table_stride=b.c.width, seq_len=b.len_d, max_len=0, row0=b.row0, n_seq=2, n_rows=5,
+                           max_rows=3)
+    b.len_d.zero_()
+    scratch = torch.empty(max(16, gpu.kv_q8_attn_scratch_bytes(b.c.pool, batch, 4)), dtype=torch.uint8, device="cuda")
+    rows = [[0, 2, 5], [0, 3, 5], [1, 3, 4]]
+    for r in rows:
+        b.out.fill_(3.0)
+        b.row0.copy_(b.c.i32(r))
+        gpu.kv_q8_attn_dev(b.c.pool, batch, b.qd, 256, b.out, 256, 4, 0.1, scratch, scratch.numel())
+        got = b.out.cpu().numpy()
+        assert np.all(got[r[0]:r[2]] == 0) and np.all(got[:r[0]] == 3.0) and np.all(got[r[2]:] == 3.0)
+    assert gpu.take_device_errors() == 0
+
+
 def test_two_calls_at_once_with_their_own_scratch(gpu):
     import torch
     a = Batch(gpu, 8, 4, 128, 2000, [100] * 4, [1] * 4, seed=21)

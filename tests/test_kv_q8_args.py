@@ -97,7 +97,7 @@ def test_verify_refusals(cuda_lib, buf):
                                                    n_tokens, None)
 
     for kw in (dict(p=None), dict(q=None), dict(drafts=None), dict(u=None), dict(tokens=None), dict(n_tokens=None),
-               dict(stride=99), dict(vocab=0), dict(kk=1 << 20)):
+               dict(stride=99), dict(vocab=0), dict(kk=1 << 20), dict(vocab=1 << 31, stride=1 << 31)):
         assert st(**kw) == B.EOS_E_INVALID_ARG, kw
     assert st(n_seq=0) == B.EOS_OK
 
