@@ -55,10 +55,8 @@
 namespace eos {
 
 constexpr uint32_t kAttnMaxCtas = 320;    // bound on the grid (scratch is sized with it)
-constexpr uint32_t kAttnThreads = 320;    // 8 softmax warps, a copy warp, a product warp
 constexpr uint32_t kAttnMl = 8;           // floats per partial row: maximum, 3 unused, 4 partial sums
 constexpr float kAttnQMax = 8300000.0f;   // largest query integer (three balanced digits hold 127 * 65793)
-constexpr float kAttnMagic = 12582912.0f; // 1.5 * 2^23
 
 // Division of x < 2^31 by a launch constant: a multiplication (error below
 // 1 / d for these x, so the quotient is exact).
@@ -214,9 +212,21 @@ __device__ __forceinline__ uint64_t attn_desc(uint32_t addr, uint32_t row_bytes)
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)((8u * row_bytes) >> 4) << 32) |
          ((uint64_t)1u << 46) | (type << 61);
 }
-// Instruction descriptor, kind::i8: D s32, A s8, B s8 or u8, both K-major.
-__device__ constexpr uint32_t attn_idesc(bool b_signed, uint32_t n) {
-  return (2u << 4) | (1u << 7) | ((b_signed ? 1u : 0u) << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+// Instruction descriptor, kind::i8: D s32, A and B s8 or u8, both K-major.
+__device__ constexpr uint32_t attn_idesc(bool a_signed, bool b_signed, uint32_t n) {
+  return (2u << 4) | ((a_signed ? 1u : 0u) << 7) | ((b_signed ? 1u : 0u) << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// An operand of bytes 255 throughout: cores of 8 rows x 16 bytes, no swizzle,
+// neighbours 16 bytes apart, so that 128 rows of 32 bytes are kAttnOnes bytes.
+// A product of two adds 32 * 255 * 255 = kAttnBias to every sum: at least the
+// largest negative score sum (128 elements of -128 * 127); two such products
+// cover a value sum (128 tokens of 255 * -127).
+constexpr uint32_t kAttnOnes = 384, kAttnBias = 32u * 255u * 255u;
+static_assert(kAttnBias >= 128u * 128u * 127u && 2u * kAttnBias >= 128u * 255u * 127u &&
+                  2u * kAttnBias + 128u * 255u * 127u < (1u << 23),
+              "biased sums are not negative and below 2^23");
+__device__ __forceinline__ uint64_t attn_ones_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)1u << 32) | ((uint64_t)1u << 46);
 }
 __device__ __forceinline__ void attn_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
                                          uint32_t accumulate) {
@@ -280,15 +290,19 @@ __device__ __forceinline__ float2 attn_mul2(float2 a, float2 b) {
   return attn_unpack(d);
 }
 __device__ __forceinline__ float2 attn_two(float x) { return make_float2(x, x); }
-// s32 sums below 2^22 as floats.
-__device__ __forceinline__ float2 attn_float(uint32_t a, uint32_t b) {
-  return attn_add2(make_float2(__uint_as_float(a + 0x4B400000u), __uint_as_float(b + 0x4B400000u)),
-                   attn_two(-kAttnMagic));
-}
-// D2 256 + D1 + D0 / 256 of three s32 sums, rounded once or twice.
+// (256 D2 + D1 + D0 / 256) 2^-22 of three s32 sums d = D + BIAS, 0 <= d < 2^23:
+// the bits of d, read as a float, are the subnormal d 2^-149, so fma(d, 2^127, c) =
+// d 2^-22 + c takes the bias off, exactly and with no conversion; two roundings,
+// of D1 + D0 / 256 (D0's bias goes with D1's: its 256th part has few bits) and of
+// the sum.
+template <uint32_t BIAS>
 __device__ __forceinline__ float2 attn_join(const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
-  return attn_fma2(attn_float(d2[0], d2[1]), attn_two(256.0f),
-                   attn_fma2(attn_float(d0[0], d0[1]), attn_two(1.0f / 256.0f), attn_float(d1[0], d1[1])));
+  constexpr float two127 = 1.7014118346046923e38f, two119 = 6.646139978924579e35f, unit = 1.0f / 4194304.0f;
+  static_assert(BIAS < (1u << 22) && BIAS % 32u == 0, "BIAS + BIAS / 256 has 24 bits");
+  auto bits = [](const uint32_t* d) { return make_float2(__uint_as_float(d[0]), __uint_as_float(d[1])); };
+  const float2 lo = attn_fma2(bits(d0), attn_two(two119),
+                              attn_fma2(bits(d1), attn_two(two127), attn_two(-((float)BIAS + (float)BIAS / 256.0f) * unit)));
+  return attn_fma2(attn_fma2(bits(d2), attn_two(two127), attn_two(-(float)BIAS * unit)), attn_two(256.0f), lo);
 }
 // Bytes 0, 1 and 2 of four words as three words.
 __device__ __forceinline__ void attn_digits(const uint32_t* b, uint32_t* w) {
@@ -722,6 +736,9 @@ struct AttnGeo {
   static constexpr uint32_t kPanels = HD <= 128u ? 1u : HD / 128u;
   static constexpr uint32_t kQBytes = 3u * RT * HD;      // a job's query digits
   static constexpr uint32_t kCtas = HD <= 128u && RT == 16u ? 2u : 1u;  // per SM
+  static constexpr uint32_t kCols = RT / 16u;           // a half's warps: four for every 16 rows
+  static constexpr uint32_t kWarps = 8u * kCols;        // softmax warps
+  static constexpr uint32_t kThreads = 32u * (kWarps + 2u);
   static constexpr uint32_t kStages = HD == 64u || RT == 32u ? 5u : 3u;  // blocks that shared memory holds
   static constexpr uint32_t kAcc = RT == 16u ? 64u : 128u;      // TMEM columns between accumulators (3 RT used)
   static constexpr uint32_t kTmem = HD <= 128u ? 4u * kAcc : 512u;  // scores of two tiles, values of two tiles
@@ -741,16 +758,16 @@ struct AttnJob {
 
 struct AttnBars {
   uint64_t full[5], empty[5], q_ready, job_free, done;
-  uint64_t s_full[2], s_free[2], p_ready[2], o_full[2], xmax[2];  // per half
+  uint64_t s_full[2], s_free[2], p_ready[2], o_full[2], xmax[2][2];  // per half
   uint32_t tmem, ok[5];
   AttnJob job[2];
 };
 
 template <uint32_t HD, uint32_t RT>
-__global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_attn_kernel(const KvAttnParams p) {
+__global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>::kCtas)) kv_attn_kernel(const KvAttnParams p) {
   using G = AttnGeo<HD, RT>;
   constexpr uint32_t S = G::kStages;
-  constexpr uint32_t NC = RT / 8u;                           // column chunks of 8
+  constexpr uint32_t NC = 2;                                 // a warp's column chunks of 8
   constexpr uint32_t MH = HD <= 128u ? 1u : HD / 128u;       // value products of 128 dimensions
   extern __shared__ uint8_t attn_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(attn_smem_raw) + 1023u) & ~uintptr_t(1023));
@@ -760,12 +777,15 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
   AttnBars& bar = *reinterpret_cast<AttnBars*>(control);
   float* qs = reinterpret_cast<float*>(control + 512u);      // [2][RT] query scales
   float* xm = qs + 2u * RT;                                  // [half][2][4][RT] tile maxima per quarter
+  uint32_t* xtop = reinterpret_cast<uint32_t*>(control + 384u);  // [half][2][cols][4] largest value scale per quarter
+  uint8_t* ones = control + 512u + 72u * RT;
+  static_assert(sizeof(AttnBars) <= 384u && 512u + 72u * RT + kAttnOnes <= G::kControl, "control words overlap");
   uint32_t* cum = reinterpret_cast<uint32_t*>(control + G::kControl);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   // the copy warp's first loads fly while the barriers are set up
   AttnSeq first{0, 0, 0};
   uint32_t prefix_len = 0, rows_end = 0;
-  if (warp == 8) {
+  if (warp == G::kWarps) {
     if (p.prefix_len != nullptr) prefix_len = *p.prefix_len;
     rows_end = kv_row_start(p.rows, p.rows.n_seq);
     if (lane < p.rows.n_seq) first = attn_seq(p, lane);
@@ -775,23 +795,27 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
       mbar_init(&bar.full[s], 1);
       mbar_init(&bar.empty[s], 1);
     }
-    mbar_init(&bar.q_ready, 8);
-    mbar_init(&bar.job_free, 8);
+    mbar_init(&bar.q_ready, G::kWarps);
+    mbar_init(&bar.job_free, G::kWarps);
     mbar_init(&bar.done, 1);
     for (uint32_t h = 0; h < 2u; ++h) {
       mbar_init(&bar.s_full[h], 1);
-      mbar_init(&bar.s_free[h], 4);
-      mbar_init(&bar.p_ready[h], 4);
+      mbar_init(&bar.s_free[h], 4u * G::kCols);
+      mbar_init(&bar.p_ready[h], 4u * G::kCols);
       mbar_init(&bar.o_full[h], 1);
-      mbar_init(&bar.xmax[h], 4);
+      for (uint32_t c = 0; c < G::kCols; ++c) mbar_init(&bar.xmax[h][c], 4);
     }
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == G::kWarps + 1u) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
                  "r"(G::kTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid < kAttnOnes / 4u) {
+    reinterpret_cast<uint32_t*>(ones)[tid] = 0xffffffffu;
+    attn_fence_async();
   }
   attn_fence_before();
   __syncthreads();
@@ -800,7 +824,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
   const uint32_t tmem = bar.tmem;
   // TMEM: scores of half h at h kAcc, value sums at (2 + h MH + mh) kAcc
 
-  if (warp == 8) {
+  if (warp == G::kWarps) {
     // ---- the line's layout: prefix units, then the sequences' (running work in cum) ----
     uint32_t carry = 0;
     AttnPlan pl;
@@ -933,10 +957,11 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
     if (lane == 0)
       for (uint32_t y = x > S ? x - S : 0u; y < x; ++y)
         if (!attn_wait(&bar.full[y % S], (y / S) & 1u)) report(p.err, EOS_DEVERR_DRAIN);
-  } else if (warp == 9) {
+  } else if (warp == G::kWarps + 1u) {
     // ---- products: tile j of a job belongs to half j % 2 ----
     if (lane == 0) {
       bool live = true;
+      const uint64_t ones_desc = attn_ones_desc(smem_u32(ones));
       uint32_t x = 0;               // stages used before the job
       uint32_t ns0 = 0, ns1 = 0;    // score products issued, per half
       uint32_t nv0 = 0, nv1 = 0;    // value products issued
@@ -959,12 +984,13 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
                 ((h ? ns1 : ns0) == 0 || mbar_test(&bar.s_free[h], ((h ? ns1 : ns0) - 1u) & 1u))) {
               attn_fence_after();
               const uint32_t ka = smem_u32(stages + (y % S) * G::kBlock), qa = smem_u32(qop);
-              constexpr uint32_t id = attn_idesc(true, 3u * RT);
+              constexpr uint32_t id = attn_idesc(true, true, 3u * RT);
+              attn_mma(tmem + h * G::kAcc, ones_desc, ones_desc, attn_idesc(false, false, 3u * RT), 0u);
 #pragma unroll
               for (uint32_t ks = 0; ks < HD / 32u; ++ks) {
                 const uint32_t panel = ks / 4u, off = (ks % 4u) * 32u;
                 attn_mma(tmem + h * G::kAcc, attn_desc(ka + panel * kKvPage * 128u + off, G::kQRow),
-                         attn_desc(qa + panel * 3u * RT * 128u + off, G::kQRow), id, ks > 0 ? 1u : 0u);
+                         attn_desc(qa + panel * 3u * RT * 128u + off, G::kQRow), id, 1u);
               }
               attn_commit(&bar.s_full[h]);
               ++(h ? ns1 : ns0);
@@ -980,14 +1006,17 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
               attn_fence_after();
               const uint32_t st = (x + 1u + jo) % S;
               const uint32_t sa = smem_u32(stages + st * G::kBlock);
-              constexpr uint32_t id = attn_idesc(false, 3u * RT);
+              constexpr uint32_t id = attn_idesc(true, false, 3u * RT), bias = attn_idesc(false, false, 3u * RT);
 #pragma unroll
-              for (uint32_t mh = 0; mh < MH; ++mh)
+              for (uint32_t mh = 0; mh < MH; ++mh) {
+                const uint32_t acc = tmem + G::kAcc * (2u + h * MH + mh);
+                attn_mma(acc, ones_desc, ones_desc, bias, 0u);
+                attn_mma(acc, ones_desc, ones_desc, bias, 1u);
 #pragma unroll
                 for (uint32_t qd = 0; qd < 4u; ++qd)
-                  attn_mma(tmem + G::kAcc * (2u + h * MH + mh),
-                           attn_desc(sa + kKvPage * HD + qd * HD * kKvQuarter + mh * 128u * kKvQuarter, 32u),
-                           attn_desc(sa + qd * 32u, 128u), id, qd > 0 ? 1u : 0u);
+                  attn_mma(acc, attn_desc(sa + kKvPage * HD + qd * HD * kKvQuarter + mh * 128u * kKvQuarter, 32u),
+                           attn_desc(sa + qd * 32u, 128u), id, 1u);
+              }
               attn_commit(&bar.o_full[h]);
               attn_commit(&bar.empty[st]);
               ++nv;
@@ -1017,7 +1046,8 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
     }
   } else {
     // ---- softmax and folding: warps 4 h + quarter work on the tiles of half h ----
-    const uint32_t quad = warp & 3u, half = warp >> 2, g = lane >> 2, cq = lane & 3u;
+    const uint32_t quad = warp & 3u, half = (warp >> 2) & 1u, grp = G::kCols == 1u ? 0u : warp >> 3, g = lane >> 2, cq = lane & 3u;
+    const uint32_t c0 = 16u * grp;  // the warp's first column
     uint32_t x = 0;               // stages used before the job
     uint32_t n_own = 0, n_other = 0;  // tiles of this half and of the other before the job
     // job n's queries (in stage y) as three signed digits each, rows warp, warp + 8, ...
@@ -1027,7 +1057,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
       const float* raw = reinterpret_cast<const float*>(stages + (y % S) * G::kBlock);
       if (bar.job[n & 1u].tiles > 0) {
 #pragma unroll
-        for (uint32_t r = warp; r < RT; r += 8u) {
+        for (uint32_t r = warp; r < RT; r += G::kWarps) {
           float scale = 0.0f;
           if (r < rows) {
             float4 v[G::kPanels];
@@ -1040,7 +1070,8 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
             }
             amax = __reduce_max_sync(0xffffffffu, amax);
             const AttnQScale q = attn_query_scale(amax, p.scale_log2);
-            scale = q.scale;
+            // (times 2^17 of the scores' 2^22; a scale that large parts any two scores all the same)
+            scale = q.finite ? fminf(q.scale * 131072.0f, 3e38f) : NAN;
 #pragma unroll
             for (uint32_t pn = 0; pn < G::kPanels; ++pn) {
               uint32_t d[3];
@@ -1073,12 +1104,12 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
       if (!live) break;
       const AttnJob s = bar.job[nj & 1u];
       if (s.tiles == 0) break;
-      const uint32_t nact = (s.rows + 7u) / 8u;  // chunks of 8 columns in use
-      // this thread's columns 8 y + 2 cq + {0, 1}
+      const uint32_t nact = s.rows > c0 ? (s.rows - c0 + 7u) / 8u : 0u;  // chunks of 8 columns in use
+      // this thread's columns c0 + 8 y + 2 cq + {0, 1}
       float2 qsc[NC], m[NC], l[NC], f[NC], o[NC][MH][4];
 #pragma unroll
       for (uint32_t y = 0; y < NC; ++y) {
-        qsc[y] = *reinterpret_cast<const float2*>(qs + (nj & 1u) * RT + 8u * y + 2u * cq);
+        qsc[y] = *reinterpret_cast<const float2*>(qs + (nj & 1u) * RT + c0 + 8u * y + 2u * cq);
         m[y] = attn_two(-INFINITY);
         l[y] = attn_two(0.0f);
         f[y] = attn_two(1.0f);
@@ -1111,12 +1142,12 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
               for (uint32_t e = 0; e < 3u; ++e)
 #pragma unroll
                 for (uint32_t hh = 0; hh < 2u; ++hh)
-                  attn_ld(tmem + G::kAcc * (2u + half * MH + mh) + ((quad * 32u + 16u * hh) << 16) + e * RT + 8u * y,
+                  attn_ld(tmem + G::kAcc * (2u + half * MH + mh) + ((quad * 32u + 16u * hh) << 16) + e * RT + c0 + 8u * y,
                           &r[e][4u * hh]);
               attn_ld_wait();
 #pragma unroll
               for (uint32_t j = 0; j < 4u; ++j)
-                o[y][mh][j] = attn_fma2(attn_join(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), fold[y],
+                o[y][mh][j] = attn_fma2(attn_join<2u * kAttnBias>(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), fold[y],
                                         attn_mul2(o[y][mh][j], f[y]));
             }
           }
@@ -1134,31 +1165,24 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
         const uint32_t tok0 = (s.tile0 + t) * kKvPage;
         const uint8_t* sc = stages + st * G::kBlock + 2u * kKvPage * HD;
         const uint32_t avail = bar.ok[st] ? s.len - tok0 : 0u;  // tokens of the tile (may exceed a page)
-        // unit of the probabilities: a power of two from the tile's largest value scale
-        uint32_t top = 0;
+        // the scales of quarter quad, token `lane`; this thread's four tokens are g + 8 j
+        uint32_t vbits = *reinterpret_cast<const uint32_t*>(sc + quad * 256u + 128u + lane * 4u);
+        float ks[4];
+        {
+          const bool in = quad * 32u + lane < avail, sound = vbits < 0x7f800000u;
+          const float kv = *reinterpret_cast<const float*>(sc + quad * 256u + lane * 4u);
+          const float k1 = in ? (sound ? 32.0f * kv : NAN) : 0.0f;      // a NaN or infinite value row: NaN score
+          vbits = in && sound ? vbits : 0u;
 #pragma unroll
-        for (uint32_t q = 0; q < 4u; ++q) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(sc + q * 256u + 128u + lane * 4u);
-          if (q * 32u + lane < avail && v < 0x7f800000u && v > top) top = v;
+          for (uint32_t j = 0; j < 4u; ++j) ks[j] = __shfl_sync(0xffffffffu, k1, g + 8u * j);
         }
-        top = __reduce_max_sync(0xffffffffu, top) >> 23;
-        top = top < 23u ? 23u : top;
-        const float up = __uint_as_float((276u - top) << 23);           // 2^(22 - exponent)
-        const float unit = __uint_as_float((top - 14u) << 23);          // 256 * 2^(exponent - 22)
-        // this thread's four tokens: quarter quad, g + 8 j
-        float ks[4], vw[4];
-#pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) {
-          const uint32_t u = g + 8u * j;
-          const bool in = quad * 32u + u < avail;
-          const float kv = *reinterpret_cast<const float*>(sc + quad * 256u + u * 4u);
-          const float vv = *reinterpret_cast<const float*>(sc + quad * 256u + 128u + u * 4u);
-          const bool sound = vv < INFINITY;                             // a NaN or infinite value row: NaN score
-          ks[j] = in ? (sound ? kv : NAN) : 0.0f;
-          vw[j] = in && sound ? vv * up : 0.0f;
+        uint32_t* xt = xtop + ((half * 2u + (it & 1u)) * G::kCols + grp) * 4u;
+        {
+          const uint32_t top = __reduce_max_sync(0xffffffffu, vbits);
+          if (lane == 0) xt[quad] = top;
         }
         const bool whole = avail >= kKvPage && tok0 + kKvPage <= common;  // nothing to mask
-        float* xmt = xm + (half * 2u + (it & 1u)) * 4u * RT + 2u * cq;
+        float* xmt = xm + (half * 2u + (it & 1u)) * 4u * RT + c0 + 2u * cq;
         float2 sv[NC][4];
 #pragma unroll
         for (uint32_t y = 0; y < NC; ++y) {
@@ -1168,13 +1192,13 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
           for (uint32_t e = 0; e < 3u; ++e)
 #pragma unroll
             for (uint32_t hh = 0; hh < 2u; ++hh)
-              attn_ld(tmem + half * G::kAcc + ((quad * 32u + 16u * hh) << 16) + e * RT + 8u * y, &r[e][4u * hh]);
+              attn_ld(tmem + half * G::kAcc + ((quad * 32u + 16u * hh) << 16) + e * RT + c0 + 8u * y, &r[e][4u * hh]);
           attn_ld_wait();
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j)
-            sv[y][j] = attn_mul2(attn_join(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), attn_two(ks[j]));
+            sv[y][j] = attn_mul2(attn_join<kAttnBias>(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), attn_two(ks[j]));
           if (!whole) {
-            const uint32_t col = 8u * y + 2u * cq;
+            const uint32_t col = c0 + 8u * y + 2u * cq;
             const uint32_t lim0 = limit(col), lim1 = limit(col + 1u);
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j) {
@@ -1196,16 +1220,26 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&bar.s_free[half]);
-          mbar_arrive(&bar.xmax[half]);
+          mbar_arrive(&bar.xmax[half][grp]);
         }
         if (t > half) live = fold_tile();
-        if (live) live = __all_sync(0xffffffffu, attn_wait(&bar.xmax[half], it & 1u)) != 0;
+        if (live) live = __all_sync(0xffffffffu, attn_wait(&bar.xmax[half][grp], it & 1u)) != 0;
         if (!live) break;
+        // unit of the probabilities: a power of two from the tile's largest value scale
+        float unit, vw[4];
+        {
+          const uint4 t4 = *reinterpret_cast<const uint4*>(xt);
+          const uint32_t top = max(max(max(t4.x, t4.y), max(t4.z, t4.w)) >> 23, 23u);
+          const float v1 = __uint_as_float(vbits) * __uint_as_float((276u - top) << 23);  // times 2^(22 - exponent)
+          unit = __uint_as_float(top << 23);  // 2^exponent: value sums are held in units of 256
+#pragma unroll
+          for (uint32_t j = 0; j < 4u; ++j) vw[j] = __shfl_sync(0xffffffffu, v1, g + 8u * j);
+        }
         uint8_t* pop = stages + st * G::kBlock;  // the probabilities take the place of the keys
 #pragma unroll
         for (uint32_t y = 0; y < NC; ++y) {
           if (y >= nact) break;  // warp-uniform
-          const uint32_t col = 8u * y + 2u * cq;
+          const uint32_t col = c0 + 8u * y + 2u * cq;
           const float2 m0 = *reinterpret_cast<const float2*>(xmt + 8u * y),
                        m1 = *reinterpret_cast<const float2*>(xmt + RT + 8u * y),
                        m2 = *reinterpret_cast<const float2*>(xmt + 2u * RT + 8u * y),
@@ -1279,7 +1313,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
         }
 #pragma unroll
         for (uint32_t z = 0; z < 2u; ++z) {
-          const uint32_t col = 8u * y + 2u * cq + z;
+          const uint32_t col = c0 + 8u * y + 2u * cq + z;
           if (col >= s.rows) continue;
           if (g == 0) {
             pml[col * kAttnMl + 4u + quad] = z ? ls.y : ls.x;
@@ -1290,7 +1324,8 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
             for (uint32_t mh = 0; mh < MH; ++mh)
 #pragma unroll
               for (uint32_t j = 0; j < 4u; ++j)
-                po[(size_t)col * HD + mh * 128u + quad * 32u + g + 8u * j] = z ? o[y][mh][j].y : o[y][mh][j].x;
+                po[(size_t)col * HD + mh * 128u + quad * 32u + g + 8u * j] =
+                    256.0f * (z ? o[y][mh][j].y : o[y][mh][j].x);
           }
         }
       }
@@ -1300,7 +1335,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnGeo<HD, RT>::kCtas)) kv_att
   attn_fence_before();
   __syncthreads();
   pdl_wait();  // the few-rows kernels before this one, see attn_line
-  if (warp == 9)
+  if (warp == G::kWarps + 1u)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kTmem) : "memory");
 }
 
@@ -1541,7 +1576,7 @@ cudaError_t attn_line(const KvAttnParams& p, int num_sms, uint64_t work, cudaStr
   // waits for this one, waits for all
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((uint32_t)grid);
-  cfg.blockDim = dim3(kAttnThreads);
+  cfg.blockDim = dim3(G::kThreads);
   cfg.dynamicSmemBytes = G::smem(p.rows.n_seq);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
