@@ -56,6 +56,7 @@ namespace eos {
 
 constexpr uint32_t kAttnMaxCtas = 320;    // bound on the grid (scratch is sized with it)
 constexpr uint32_t kAttnMl = 8;           // floats per partial row: maximum, 3 unused, 4 partial sums
+constexpr float kAttnLow = -3e38f;        // reference of tiles whose tokens are all hidden: finite, so that no difference is NaN
 constexpr float kAttnQMax = 8300000.0f;   // largest query integer (three balanced digits hold 127 * 65793)
 
 // Division of x < 2^31 by a launch constant: a multiplication (error below
@@ -245,14 +246,57 @@ __device__ __forceinline__ void attn_fence_before() { asm volatile("tcgen05.fenc
 __device__ __forceinline__ void attn_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void attn_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // 16 TMEM lanes x 8 columns: thread t gets r[0..1] = lane t / 4, columns
-// 2 (t % 4) + {0, 1}, and r[2..3] the same columns of lane t / 4 + 8.
+// 2 (t % 4) + {0, 1}, and r[2..3] the same columns of lane t / 4 + 8.  Two: and
+// r[4..7] the same of the 8 columns behind.
 __device__ __forceinline__ void attn_ld(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void attn_ld_two(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void attn_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// use(y, j, d0, d1, d2) with the digit sums (digits RT columns apart) of 32 lanes
+// and the first nact of two chunks of 8 columns: chunk y, lane g + 8 j.  Groups
+// of 16 rows are read chunk by chunk, since often only one is in use; 32 rows by
+// half the lanes, in half as many instructions.
+template <uint32_t RT, typename F>
+__device__ __forceinline__ void attn_sums(uint32_t taddr, uint32_t nact, F use) {
+  if constexpr (RT == 16u) {
+#pragma unroll
+    for (uint32_t y = 0; y < 2u; ++y) {
+      if (y >= nact) break;  // warp-uniform
+      uint32_t r[3][8];
+#pragma unroll
+      for (uint32_t e = 0; e < 3u; ++e)
+#pragma unroll
+        for (uint32_t hh = 0; hh < 2u; ++hh) attn_ld(taddr + ((16u * hh) << 16) + e * RT + 8u * y, &r[e][4u * hh]);
+      attn_ld_wait();
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j) use(y, j, &r[0][2u * j], &r[1][2u * j], &r[2][2u * j]);
+    }
+  } else if (nact > 0) {  // warp-uniform
+#pragma unroll
+    for (uint32_t hh = 0; hh < 2u; ++hh) {
+      uint32_t r[3][8];
+#pragma unroll
+      for (uint32_t e = 0; e < 3u; ++e) attn_ld_two(taddr + ((16u * hh) << 16) + e * RT, r[e]);
+      attn_ld_wait();
+#pragma unroll
+      for (uint32_t y = 0; y < 2u; ++y) {
+        if (y >= nact) break;
+#pragma unroll
+        for (uint32_t j = 0; j < 2u; ++j)
+          use(y, 2u * hh + j, &r[0][4u * y + 2u * j], &r[1][4u * y + 2u * j], &r[2][4u * y + 2u * j]);
+      }
+    }
+  }
+}
 __device__ __forceinline__ void attn_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
@@ -1110,7 +1154,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
 #pragma unroll
       for (uint32_t y = 0; y < NC; ++y) {
         qsc[y] = *reinterpret_cast<const float2*>(qs + (nj & 1u) * RT + c0 + 8u * y + 2u * cq);
-        m[y] = attn_two(-INFINITY);
+        m[y] = attn_two(kAttnLow);
         l[y] = attn_two(0.0f);
         f[y] = attn_two(1.0f);
 #pragma unroll
@@ -1133,24 +1177,12 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         attn_fence_after();
         if (HD >= 128u || quad * 32u < HD) {
 #pragma unroll
-          for (uint32_t y = 0; y < NC; ++y) {
-            if (y >= nact) break;  // warp-uniform
-#pragma unroll
-            for (uint32_t mh = 0; mh < MH; ++mh) {
-              uint32_t r[3][8];
-#pragma unroll
-              for (uint32_t e = 0; e < 3u; ++e)
-#pragma unroll
-                for (uint32_t hh = 0; hh < 2u; ++hh)
-                  attn_ld(tmem + G::kAcc * (2u + half * MH + mh) + ((quad * 32u + 16u * hh) << 16) + e * RT + c0 + 8u * y,
-                          &r[e][4u * hh]);
-              attn_ld_wait();
-#pragma unroll
-              for (uint32_t j = 0; j < 4u; ++j)
-                o[y][mh][j] = attn_fma2(attn_join<2u * kAttnBias>(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), fold[y],
-                                        attn_mul2(o[y][mh][j], f[y]));
-            }
-          }
+          for (uint32_t mh = 0; mh < MH; ++mh)
+            attn_sums<RT>(tmem + G::kAcc * (2u + half * MH + mh) + ((quad * 32u) << 16) + c0, nact,
+                          [&](uint32_t y, uint32_t j, const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
+                            o[y][mh][j] = attn_fma2(attn_join<2u * kAttnBias>(d0, d1, d2), fold[y],
+                                                    attn_mul2(o[y][mh][j], f[y]));
+                          });
         }
         attn_fence_before();
         return true;
@@ -1184,19 +1216,15 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         const bool whole = avail >= kKvPage && tok0 + kKvPage <= common;  // nothing to mask
         float* xmt = xm + (half * 2u + (it & 1u)) * 4u * RT + c0 + 2u * cq;
         float2 sv[NC][4];
+        attn_sums<RT>(tmem + half * G::kAcc + ((quad * 32u) << 16) + c0, nact,
+                      [&](uint32_t y, uint32_t j, const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
+                        sv[y][j] = attn_mul2(attn_join<kAttnBias>(d0, d1, d2), attn_two(ks[j]));
+                      });
+        float2 mx[NC];
 #pragma unroll
         for (uint32_t y = 0; y < NC; ++y) {
-          if (y >= nact) break;  // warp-uniform
-          uint32_t r[3][8];
-#pragma unroll
-          for (uint32_t e = 0; e < 3u; ++e)
-#pragma unroll
-            for (uint32_t hh = 0; hh < 2u; ++hh)
-              attn_ld(tmem + half * G::kAcc + ((quad * 32u + 16u * hh) << 16) + e * RT + c0 + 8u * y, &r[e][4u * hh]);
-          attn_ld_wait();
-#pragma unroll
-          for (uint32_t j = 0; j < 4u; ++j)
-            sv[y][j] = attn_mul2(attn_join<kAttnBias>(&r[0][2u * j], &r[1][2u * j], &r[2][2u * j]), attn_two(ks[j]));
+          mx[y] = attn_two(-INFINITY);
+          if (y >= nact) continue;  // warp-uniform
           if (!whole) {
             const uint32_t col = c0 + 8u * y + 2u * cq;
             const uint32_t lim0 = limit(col), lim1 = limit(col + 1u);
@@ -1207,14 +1235,19 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
               if (tok >= avail || tok0 + tok >= lim1) sv[y][j].y = -INFINITY;
             }
           }
-          float2 mx = make_float2(fmaxf(fmaxf(sv[y][0].x, sv[y][1].x), fmaxf(sv[y][2].x, sv[y][3].x)),
-                                  fmaxf(fmaxf(sv[y][0].y, sv[y][1].y), fmaxf(sv[y][2].y, sv[y][3].y)));
-#pragma unroll
-          for (uint32_t o2 = 4; o2 < 32u; o2 <<= 1) {
-            mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o2));
-            mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o2));
-          }
-          if (g == 0) *reinterpret_cast<float2*>(xmt + quad * RT + 8u * y) = mx;
+          mx[y] = make_float2(fmaxf(fmaxf(sv[y][0].x, sv[y][1].x), fmaxf(sv[y][2].x, sv[y][3].x)),
+                              fmaxf(fmaxf(sv[y][0].y, sv[y][1].y), fmaxf(sv[y][2].y, sv[y][3].y)));
+        }
+        // the four columns' maxima over the eight lanes that share them: each step
+        // halves what a lane still holds, bit 2 of the lane its chunk, bit 3 its column
+        {
+          const bool hi = (lane & 4u) != 0u, odd = (lane & 8u) != 0u;
+          const float2 keep = hi ? mx[1] : mx[0], send = hi ? mx[0] : mx[1];
+          const float kx = fmaxf(keep.x, __shfl_xor_sync(0xffffffffu, send.x, 4));
+          const float ky = fmaxf(keep.y, __shfl_xor_sync(0xffffffffu, send.y, 4));
+          float k1 = fmaxf(odd ? ky : kx, __shfl_xor_sync(0xffffffffu, odd ? kx : ky, 8));
+          k1 = fmaxf(k1, __shfl_xor_sync(0xffffffffu, k1, 16));
+          if (lane < 16u) xmt[quad * RT + (lane & 4u) * 2u + ((lane >> 3) & 1u)] = k1;
         }
         attn_fence_before();
         __syncwarp();
@@ -1247,13 +1280,11 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           // the tile's own reference, rounded up so that no probability exceeds 1
           // (its integers are relative to it: their rounding fades with the tile)
           const float t0 = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x)), t1 = fmaxf(fmaxf(m0.y, m1.y), fmaxf(m2.y, m3.y));
-          const float2 ref = make_float2(t0 == -INFINITY ? t0 : __fmul_ru(t0, qsc[y].x),
-                                         t1 == -INFINITY ? t1 : __fmul_ru(t1, qsc[y].y));
-          const float2 neg = make_float2(ref.x == -INFINITY ? 0.0f : -ref.x, ref.y == -INFINITY ? 0.0f : -ref.y);
+          const float2 ref = make_float2(fmaxf(__fmul_ru(t0, qsc[y].x), kAttnLow), fmaxf(__fmul_ru(t1, qsc[y].y), kAttnLow));
+          const float2 neg = make_float2(-ref.x, -ref.y);
           const float2 nm = make_float2(fmaxf(ref.x, m[y].x), fmaxf(ref.y, m[y].y));
-          const float2 run = make_float2(nm.x == -INFINITY ? 0.0f : nm.x, nm.y == -INFINITY ? 0.0f : nm.y);
-          f[y] = make_float2(attn_ex2(m[y].x - run.x), attn_ex2(m[y].y - run.y));
-          const float2 share = make_float2(attn_ex2(ref.x - run.x), attn_ex2(ref.y - run.y));
+          f[y] = make_float2(attn_ex2(m[y].x - nm.x), attn_ex2(m[y].y - nm.y));
+          const float2 share = make_float2(attn_ex2(ref.x - nm.x), attn_ex2(ref.y - nm.y));
           fold[y] = attn_mul2(share, attn_two(unit));
           m[y] = nm;
           uint32_t b0[4], b1[4], d[3];
