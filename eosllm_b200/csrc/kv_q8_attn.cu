@@ -797,7 +797,9 @@ struct AttnGeo {
 // A piece of a unit as the copy warp hands it to the others.
 struct AttnJob {
   uint32_t tiles;           // 0: no further piece
-  uint32_t tile0, rows, row0, len, n, unit, prefix;
+  uint32_t rows, row0, unit, prefix;
+  uint32_t left;            // tokens from the piece's first page on
+  int32_t seen0;            // of which a sequence's first row sees so many (a prefix's rows: all)
 };
 
 struct AttnBars {
@@ -930,7 +932,9 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           live = false;
         }
         if (live) {
-          bar.job[nj & 1u] = AttnJob{s.tiles, s.tile0, s.rows, s.row0, s.len, s.n, s.unit, is_prefix ? 1u : 0u};
+          const int32_t t0 = (int32_t)(s.tile0 * kKvPage);
+          bar.job[nj & 1u] = AttnJob{s.tiles, s.rows, s.row0, s.unit, is_prefix ? 1u : 0u, s.len - (uint32_t)t0,
+                                     is_prefix ? 0x3fffffff : (int32_t)s.len - (int32_t)s.n + 1 - t0};
           if (more) mbar_arrive_expect_tx(&bar.full[x % S], s.rows * HD * 4u);
           else mbar_arrive(&bar.full[x % S]);
         }
@@ -1150,10 +1154,9 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
       if (s.tiles == 0) break;
       const uint32_t nact = s.rows > c0 ? (s.rows - c0 + 7u) / 8u : 0u;  // chunks of 8 columns in use
       // this thread's columns c0 + 8 y + 2 cq + {0, 1}
-      float2 qsc[NC], m[NC], l[NC], f[NC], o[NC][MH][4];
+      float2 m[NC], l[NC], f[NC], o[NC][MH][4];
 #pragma unroll
       for (uint32_t y = 0; y < NC; ++y) {
-        qsc[y] = *reinterpret_cast<const float2*>(qs + (nj & 1u) * RT + c0 + 8u * y + 2u * cq);
         m[y] = attn_two(kAttnLow);
         l[y] = attn_two(0.0f);
         f[y] = attn_two(1.0f);
@@ -1162,13 +1165,12 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) o[y][mh][j] = attn_two(0.0f);
       }
-      // tokens that column `col` sees; all columns see those below `common`
-      auto limit = [&](uint32_t col) -> uint32_t {
-        if (s.prefix) return s.len;
-        const int64_t seen = (int64_t)s.len - (int64_t)s.n + 1 + (int64_t)attn_div(s.row0 + col, p.by_group);
-        return seen <= 0 ? 0u : (seen < (int64_t)s.len ? (uint32_t)seen : s.len);
+      // tokens from the piece's first page on that column `col` sees; all columns see those below `common`
+      auto limit = [&](uint32_t col) -> int32_t {
+        const AttnJob& job = bar.job[nj & 1u];
+        return min(job.seen0 + (int32_t)attn_div(job.row0 + col, p.by_group), (int32_t)job.left);
       };
-      const uint32_t common = limit(0);
+      const int32_t common = limit(0);
       float2 fold[NC];         // the last tile's probability unit, relative to the running reference
       uint32_t it = n_own;     // tiles of this half so far
       // o = o f + fold * (value product of the tile before)
@@ -1194,9 +1196,9 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
                                            attn_wait(&bar.full[st], (pos / S) & 1u)) != 0;
         if (!live) break;
         attn_fence_after();
-        const uint32_t tok0 = (s.tile0 + t) * kKvPage;
+        const uint32_t tok0 = t * kKvPage;
         const uint8_t* sc = stages + st * G::kBlock + 2u * kKvPage * HD;
-        const uint32_t avail = bar.ok[st] ? s.len - tok0 : 0u;  // tokens of the tile (may exceed a page)
+        const uint32_t avail = bar.ok[st] ? s.left - tok0 : 0u;  // tokens of the tile (may exceed a page)
         // the scales of quarter quad, token `lane`; this thread's four tokens are g + 8 j
         uint32_t vbits = *reinterpret_cast<const uint32_t*>(sc + quad * 256u + 128u + lane * 4u);
         float ks[4];
@@ -1213,7 +1215,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           const uint32_t top = __reduce_max_sync(0xffffffffu, vbits);
           if (lane == 0) xt[quad] = top;
         }
-        const bool whole = avail >= kKvPage && tok0 + kKvPage <= common;  // nothing to mask
+        const bool whole = avail >= kKvPage && (int32_t)(tok0 + kKvPage) <= common;  // nothing to mask
         float* xmt = xm + (half * 2u + (it & 1u)) * 4u * RT + c0 + 2u * cq;
         float2 sv[NC][4];
         attn_sums<RT>(tmem + half * G::kAcc + ((quad * 32u) << 16) + c0, nact,
@@ -1227,12 +1229,12 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           if (y >= nact) continue;  // warp-uniform
           if (!whole) {
             const uint32_t col = c0 + 8u * y + 2u * cq;
-            const uint32_t lim0 = limit(col), lim1 = limit(col + 1u);
+            const int32_t lim0 = limit(col), lim1 = limit(col + 1u);
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j) {
               const uint32_t tok = quad * 32u + g + 8u * j;
-              if (tok >= avail || tok0 + tok >= lim0) sv[y][j].x = -INFINITY;
-              if (tok >= avail || tok0 + tok >= lim1) sv[y][j].y = -INFINITY;
+              if (tok >= avail || (int32_t)(tok0 + tok) >= lim0) sv[y][j].x = -INFINITY;
+              if (tok >= avail || (int32_t)(tok0 + tok) >= lim1) sv[y][j].y = -INFINITY;
             }
           }
           mx[y] = make_float2(fmaxf(fmaxf(sv[y][0].x, sv[y][1].x), fmaxf(sv[y][2].x, sv[y][3].x)),
@@ -1273,6 +1275,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         for (uint32_t y = 0; y < NC; ++y) {
           if (y >= nact) break;  // warp-uniform
           const uint32_t col = c0 + 8u * y + 2u * cq;
+          const float2 qsc = *reinterpret_cast<const float2*>(qs + (nj & 1u) * RT + col);
           const float2 m0 = *reinterpret_cast<const float2*>(xmt + 8u * y),
                        m1 = *reinterpret_cast<const float2*>(xmt + RT + 8u * y),
                        m2 = *reinterpret_cast<const float2*>(xmt + 2u * RT + 8u * y),
@@ -1280,7 +1283,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           // the tile's own reference, rounded up so that no probability exceeds 1
           // (its integers are relative to it: their rounding fades with the tile)
           const float t0 = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x)), t1 = fmaxf(fmaxf(m0.y, m1.y), fmaxf(m2.y, m3.y));
-          const float2 ref = make_float2(fmaxf(__fmul_ru(t0, qsc[y].x), kAttnLow), fmaxf(__fmul_ru(t1, qsc[y].y), kAttnLow));
+          const float2 ref = make_float2(fmaxf(__fmul_ru(t0, qsc.x), kAttnLow), fmaxf(__fmul_ru(t1, qsc.y), kAttnLow));
           const float2 neg = make_float2(-ref.x, -ref.y);
           const float2 nm = make_float2(fmaxf(ref.x, m[y].x), fmaxf(ref.y, m[y].y));
           f[y] = make_float2(attn_ex2(m[y].x - nm.x), attn_ex2(m[y].y - nm.y));
@@ -1291,7 +1294,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           float2 ls = attn_two(0.0f);
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) {
-            const float2 z = attn_fma2(sv[y][j], qsc[y], neg);
+            const float2 z = attn_fma2(sv[y][j], qsc, neg);
             const float2 e = make_float2(attn_ex2(z.x), attn_ex2(z.y));
             ls = attn_add2(ls, e);
             const float2 w = attn_fma2(e, attn_two(vw[j]), attn_two(8388608.0f));
