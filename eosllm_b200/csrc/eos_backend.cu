@@ -83,8 +83,16 @@ int device_info(int dev, DevInfo** out) {
     int cur = 0;
     EOS_CK(cudaGetDevice(&cur), "cudaGetDevice");
     EOS_CK(cudaSetDevice(dev), "cudaSetDevice");
-    cudaError_t e = cudaMalloc(&d.err_d, sizeof(uint32_t));
-    if (e == cudaSuccess) e = cudaMemset(d.err_d, 0, sizeof(uint32_t));
+    // (relaxed, on a stream of its own: the first call on a device may be captured)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaStream_t st = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMalloc(&d.err_d, sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMemsetAsync(d.err_d, 0, sizeof(uint32_t), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (st) cudaStreamDestroy(st);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     cudaSetDevice(cur);
     if (e != cudaSuccess) return cuda_fail(e, "error word");
     d.ready = true;

@@ -453,6 +453,36 @@ def test_nothing_to_attend_to_follows_its_inputs(gpu):
     assert gpu.take_device_errors() == 0
 
 
+FIRST_CALL = """
+import torch
+from eosllm_b200 import backend as B
+pages = torch.empty(2 * B.kv_q8_page_bytes(1, 64), dtype=torch.uint8, device="cuda")
+pool = B.kv_q8_pool(pages, 2, 1, 64)
+k = torch.randn(130, 1, 64, device="cuda")
+out = [torch.zeros_like(k) for _ in range(2)]
+tab, pos = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1], [0]))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    B.kv_q8_write_dev(pool, k, k, 64, 130, None, tab, 2, pos, 1, stream=st)
+    B.kv_q8_read_dev(pool, out[0], out[1], 64, 130, None, tab, 2, pos, 1, stream=st)
+g.replay()
+torch.cuda.synchronize()
+assert float((out[0] - k).abs().max()) <= float(k.abs().max()) / 254 * 1.001 and torch.equal(out[0], out[1])
+assert B.take_device_errors() == 0
+"""
+
+
+def test_first_call_on_a_device_may_be_captured(gpu):
+    """In a process of its own, where nothing has set the library up."""
+    import pathlib
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=pathlib.Path(__file__).parent.parent, timeout=300,
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_two_calls_at_once_with_their_own_scratch(gpu):
     import torch
     a = Batch(gpu, 8, 4, 128, 2000, [100] * 4, [1] * 4, seed=21)
