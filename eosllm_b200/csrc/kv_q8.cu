@@ -44,10 +44,6 @@ __device__ __forceinline__ uint32_t kv_pick_bytes(uint32_t a, uint32_t b, uint32
   const uint32_t sel = e | ((e + 4u) << 4);
   return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
-__device__ __forceinline__ uint32_t kv_absmax4(uint32_t amax, float4 v) {
-  amax = max(max(amax, __float_as_uint(v.x) & 0x7fffffffu), __float_as_uint(v.y) & 0x7fffffffu);
-  return max(max(amax, __float_as_uint(v.z) & 0x7fffffffu), __float_as_uint(v.w) & 0x7fffffffu);
-}
 __device__ __forceinline__ float4 kv_value4(uint32_t w, float s) {
   return make_float4(__fmul_rn((float)(int8_t)w, s), __fmul_rn((float)(int8_t)(w >> 8), s),
                      __fmul_rn((float)(int8_t)(w >> 16), s), __fmul_rn((float)(int8_t)(w >> 24), s));
@@ -94,10 +90,10 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvCopyParams p) {
         if (on) *reinterpret_cast<float4*>((which ? p.v : p.k) + at + c * 128u) = kv_value4(q, s);
       }
     } else {
-      uint32_t amax = 0;
+      float amax = 0.0f;
 #pragma unroll
       for (uint32_t c = 0; c < C; ++c) amax = kv_absmax4(amax, x[which][c]);
-      const KvRowScale s = kv_row_scale(__reduce_max_sync(0xffffffffu, amax));
+      const KvRowScale s = kv_row_scale(amax);
 #pragma unroll
       for (uint32_t c = 0; c < C; ++c) {
         const uint32_t d = lane * 4u + c * 128u, q = kv_quant4(x[which][c], s);
@@ -199,14 +195,14 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
       }
 #pragma unroll
     for (uint32_t j = 0; j < 4u; ++j) {
-      uint32_t ka = 0, va = 0;
+      float ka = 0.0f, va = 0.0f;
 #pragma unroll
       for (uint32_t c = 0; c < C; ++c) {
         ka = kv_absmax4(ka, x[0][j][c]);
         va = kv_absmax4(va, x[1][j][c]);
       }
-      const KvRowScale sk = kv_row_scale(__reduce_max_sync(0xffffffffu, ka));
-      const KvRowScale sv = kv_row_scale(__reduce_max_sync(0xffffffffu, va));
+      const KvRowScale sk = kv_row_scale(ka);
+      const KvRowScale sv = kv_row_scale(va);
       ks[j] = sk.scale;
       vs[j] = sv.scale;
 #pragma unroll
