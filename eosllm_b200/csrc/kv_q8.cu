@@ -23,9 +23,10 @@ struct KvCopyParams {
 // latter two are reported).
 __device__ __forceinline__ uint8_t* kv_locate(const KvCopyParams& p, uint32_t r, uint32_t h, uint32_t hd,
                                               uint32_t& slot) {
-  const uint32_t i = kv_row_seq(p.rows, r);
-  if (i >= p.rows.n_seq) return nullptr;
-  const uint64_t at = (uint64_t)p.pos[i] + (r - kv_row_start(p.rows, i));
+  uint32_t r0, r1, pos;
+  const uint32_t i = kv_find(p.rows, p.pos, [&](uint32_t, uint32_t start) { return start <= r; }, r0, r1, pos);
+  if (i >= p.rows.n_seq || r >= r1) return nullptr;
+  const uint64_t at = (uint64_t)pos + (r - r0);
   if (at >= (uint64_t)p.table_stride * kKvPage) {
     report(p.err, EOS_DEVERR_RANGE);
     return nullptr;
@@ -118,31 +119,44 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvCopyParams p) {
 // byte moves once; reading and writing f32 rows is what bounds it.
 //
 // Quarters of a ragged batch: sequence i's blocks start at row0[i] / 32 + 2 i,
-// which leaves room for the two broken ends; a CTA searches its sequence.
+// which leaves room for the two broken ends; a CTA searches its sequence, and the
+// rows are on their way before its page is known.
 template <uint32_t HD, bool READ>
 __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
   constexpr uint32_t C = HD <= 128u ? 1u : HD / 128u;
   constexpr uint32_t PITCH = 9u;  // words per value row in shared memory
   __shared__ uint32_t vt[HD * PITCH];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, g = tid >> 5, h = blockIdx.y;
-  uint32_t i = 0;
-  {
-    uint32_t lo = 0, hi = p.rows.n_seq;
-    while (hi - lo > 1u) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if (kv_row_start(p.rows, mid) / 32u + 2u * mid <= blockIdx.x) lo = mid;
-      else hi = mid;
-    }
-    i = lo;
-  }
-  const uint32_t r0 = kv_row_start(p.rows, i), r1 = kv_row_start(p.rows, i + 1u), n = r1 > r0 ? r1 - r0 : 0u;
-  const uint64_t pos = p.pos[i];
+  uint32_t r0, r1, first;
+  const uint32_t i = kv_find(p.rows, p.pos, [&](uint32_t x, uint32_t start) { return start / 32u + 2u * x <= blockIdx.x; },
+                             r0, r1, first);
+  if (i >= p.rows.n_seq) return;  // (rows before the first sequence)
+  const uint32_t n = r1 > r0 ? r1 - r0 : 0u;
+  const uint64_t pos = first;
   const uint32_t b0 = r0 / 32u + 2u * i;
-  if (blockIdx.x < b0) return;  // (rows before the first sequence)
   const uint64_t t0 = (pos & ~(uint64_t)31u) + 32ull * (blockIdx.x - b0);  // the quarter's first position
   if (n == 0 || t0 >= pos + n) return;
   uint32_t page = 0xffffffffu;
   if (t0 < (uint64_t)p.table_stride * kKvPage) page = p.table[(size_t)i * p.table_stride + (uint32_t)(t0 / kKvPage)];
+  const bool on = HD >= 128u || lane < HD / 4u;
+  bool in[4];
+  size_t at[4];
+  float4 x[2][4][C];
+#pragma unroll
+  for (uint32_t j = 0; j < 4u; ++j) {
+    const uint64_t t = t0 + g + 8u * j;
+    in[j] = t >= pos && t < pos + n;
+    at[j] = in[j] ? (size_t)(r0 + (uint32_t)(t - pos)) * p.row_stride + h * HD + lane * 4u : 0u;
+    if (!READ)  // the rows fly while the page is looked up
+#pragma unroll
+      for (uint32_t c = 0; c < C; ++c) {
+        x[0][j][c] = x[1][j][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (in[j] && on) {
+          x[0][j][c] = __ldcs(reinterpret_cast<const float4*>(p.k + at[j] + c * 128u));
+          x[1][j][c] = __ldcs(reinterpret_cast<const float4*>(p.v + at[j] + c * 128u));
+        }
+      }
+  }
   if (page >= p.n_pages) {
     if (tid == 0) report(p.err, EOS_DEVERR_RANGE);
     return;
@@ -151,7 +165,6 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
   const uint32_t s0 = (uint32_t)(t0 % kKvPage);
   const bool whole = t0 >= pos && t0 + 32u <= pos + n;
   uint8_t* vq = blk + kKvPage * HD + (s0 / kKvQuarter) * (HD * kKvQuarter);
-  const bool on = HD >= 128u || lane < HD / 4u;
   // value rows of the quarter as 16-byte chunks: chunk x is element x / 2, half x % 2
   auto chunk = [&](uint32_t x) { return vq + (x >> 1) * 32u + (((x & 1u) ^ ((x >> 1) >> 2)) & 1u) * 16u; };
   // the bytes of word w of a value row (tokens w, w + 8, w + 16, w + 24) that this call writes
@@ -173,26 +186,7 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
   }
   uint32_t kw[4][C], vw[4][C];
   float ks[4], vs[4];
-  bool in[4];
-  size_t at[4];
-#pragma unroll
-  for (uint32_t j = 0; j < 4u; ++j) {
-    const uint64_t t = t0 + g + 8u * j;
-    in[j] = t >= pos && t < pos + n;
-    at[j] = in[j] ? (size_t)(r0 + (uint32_t)(t - pos)) * p.row_stride + h * HD + lane * 4u : 0u;
-  }
   if (!READ) {
-    float4 x[2][4][C];
-#pragma unroll
-    for (uint32_t j = 0; j < 4u; ++j)
-#pragma unroll
-      for (uint32_t c = 0; c < C; ++c) {
-        x[0][j][c] = x[1][j][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (in[j] && on) {
-          x[0][j][c] = __ldcs(reinterpret_cast<const float4*>(p.k + at[j] + c * 128u));
-          x[1][j][c] = __ldcs(reinterpret_cast<const float4*>(p.v + at[j] + c * 128u));
-        }
-      }
 #pragma unroll
     for (uint32_t j = 0; j < 4u; ++j) {
       float ka = 0.0f, va = 0.0f;

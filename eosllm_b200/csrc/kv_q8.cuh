@@ -63,17 +63,30 @@ __device__ __forceinline__ uint32_t kv_row_start(const KvRows& b, uint32_t i) {
   const uint32_t r = b.row0 != nullptr ? b.row0[i] : i * b.per_seq;
   return r < b.n_rows ? r : b.n_rows;
 }
-// The sequence of row r (rows before the first or behind the last give n_seq).
-__device__ __forceinline__ uint32_t kv_row_seq(const KvRows& b, uint32_t r) {
-  if (b.row0 == nullptr) return r / b.per_seq;
-  uint32_t lo = 0, hi = b.n_seq;  // start(lo) <= r < start(hi)
-  if (kv_row_start(b, b.n_seq) <= r || r < kv_row_start(b, 0)) return b.n_seq;
-  while (hi - lo > 1u) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (kv_row_start(b, mid) <= r) lo = mid;
-    else hi = mid;
+// The last sequence i for which before(i, its first row) holds -- sequences in
+// order, so these are the first ones -- with its rows [r0, r1) and words[i]; n_seq
+// where there is none.  Warp-uniform; 32 sequences are looked at at once, and
+// what is needed of them comes along, so a batch of up to 31 takes one round trip.
+template <typename F>
+__device__ __forceinline__ uint32_t kv_find(const KvRows& b, const uint32_t* words, F before, uint32_t& r0, uint32_t& r1,
+                                            uint32_t& word) {
+  const uint32_t lane = threadIdx.x & 31u;
+  uint32_t lo = 0, len = b.n_seq;
+  while (len > 32u) {
+    const uint32_t step = (len + 31u) / 32u, i = lo + lane * step;
+    const uint32_t c = __popc(__ballot_sync(0xffffffffu, lane * step < len && before(i, kv_row_start(b, i))));
+    if (c == 0) return b.n_seq;
+    lo += (c - 1u) * step;
+    len = len - (c - 1u) * step < step ? len - (c - 1u) * step : step;
   }
-  return lo;
+  const uint32_t i = lo + lane;
+  const uint32_t start = i <= b.n_seq ? kv_row_start(b, i) : 0u, w = i < b.n_seq ? words[i] : 0u;
+  const uint32_t c = __popc(__ballot_sync(0xffffffffu, lane < len && before(i, start)));
+  if (c == 0) return b.n_seq;
+  r0 = __shfl_sync(0xffffffffu, start, c - 1u);
+  r1 = c < 32u ? __shfl_sync(0xffffffffu, start, c) : kv_row_start(b, lo + c);
+  word = __shfl_sync(0xffffffffu, w, c - 1u);
+  return lo + c - 1u;
 }
 
 // ---- the row quantizer ----------------------------------------------------
