@@ -126,15 +126,16 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
   constexpr uint32_t C = HD <= 128u ? 1u : HD / 128u;
   constexpr uint32_t PITCH = 9u;  // words per value row in shared memory
   __shared__ uint32_t vt[HD * PITCH];
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, g = tid >> 5, h = blockIdx.y;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, g = tid >> 5;
+  const uint32_t block = blockIdx.x / p.n_kv_head, h = blockIdx.x - block * p.n_kv_head;
   uint32_t r0, r1, first;
-  const uint32_t i = kv_find(p.rows, p.pos, [&](uint32_t x, uint32_t start) { return start / 32u + 2u * x <= blockIdx.x; },
+  const uint32_t i = kv_find(p.rows, p.pos, [&](uint32_t x, uint32_t start) { return start / 32u + 2u * x <= block; },
                              r0, r1, first);
   if (i >= p.rows.n_seq) return;  // (rows before the first sequence)
   const uint32_t n = r1 > r0 ? r1 - r0 : 0u;
   const uint64_t pos = first;
   const uint32_t b0 = r0 / 32u + 2u * i;
-  const uint64_t t0 = (pos & ~(uint64_t)31u) + 32ull * (blockIdx.x - b0);  // the quarter's first position
+  const uint64_t t0 = (pos & ~(uint64_t)31u) + 32ull * (block - b0);  // the quarter's first position
   if (n == 0 || t0 >= pos + n) return;
   uint32_t page = 0xffffffffu;
   if (t0 < (uint64_t)p.table_stride * kKvPage) page = p.table[(size_t)i * p.table_stride + (uint32_t)(t0 / kKvPage)];
@@ -287,8 +288,8 @@ template <bool READ>
 cudaError_t copy_launch(const KvPool& kv, const KvCopyParams& p, cudaStream_t st) {
   const KvRows& r = p.rows;
   const uint64_t blocks = (uint64_t)r.n_rows / 32u + 2ull * r.n_seq;
-  if (r.n_rows >= 4ull * r.n_seq && kv.n_kv_head <= 65535u) {
-    const dim3 grid((uint32_t)blocks, kv.n_kv_head);
+  if (r.n_rows >= 4ull * r.n_seq) {
+    const uint32_t grid = (uint32_t)(blocks * kv.n_kv_head);
     if (kv.head_dim == 64) kv_quarter_kernel<64, READ><<<grid, 256, 0, st>>>(p);
     else if (kv.head_dim == 128) kv_quarter_kernel<128, READ><<<grid, 256, 0, st>>>(p);
     else kv_quarter_kernel<256, READ><<<grid, 256, 0, st>>>(p);
