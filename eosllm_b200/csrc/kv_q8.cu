@@ -116,13 +116,19 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvCopyParams p) {
 // four tokens (a 4 x 4 byte transpose in registers).  The words of the 32
 // tokens meet in shared memory (rows of nine words: the lanes' accesses then
 // collide four ways at most) and value rows move as 16 bytes a thread.  Every
-// byte moves once; reading and writing f32 rows is what bounds it.
+// byte moves once; reading and writing f32 rows is what bounds it.  The heads of
+// the same rows are neighbours in the grid, so that what runs together is
+// together in memory (reading 16383 rows x 32 heads: 117 us head by head, 107
+// so, 6.3 TB/s).  A write's registers are held to 64 a thread, four CTAs an SM:
+// at three, 8505 rows x 8 heads took 21.4 us, at four 19.9 (4.4 TB/s; loads,
+// rounding and stores of a CTA follow one another); keys and values in CTAs of
+// their own 24.3.
 //
 // Quarters of a ragged batch: sequence i's blocks start at row0[i] / 32 + 2 i,
 // which leaves room for the two broken ends; a CTA searches its sequence, and the
 // rows are on their way before its page is known.
 template <uint32_t HD, bool READ>
-__global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
+__global__ void __launch_bounds__(256, READ ? (HD > 128u ? 6 : 8) : (HD > 128u ? 2 : 4)) kv_quarter_kernel(const KvCopyParams p) {
   constexpr uint32_t C = HD <= 128u ? 1u : HD / 128u;
   constexpr uint32_t PITCH = 9u;  // words per value row in shared memory
   __shared__ uint32_t vt[HD * PITCH];
@@ -141,20 +147,20 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
   if (t0 < (uint64_t)p.table_stride * kKvPage) page = p.table[(size_t)i * p.table_stride + (uint32_t)(t0 / kKvPage)];
   const bool on = HD >= 128u || lane < HD / 4u;
   bool in[4];
-  size_t at[4];
+  // the warp's first row (may lie before the call's, then it is not touched); the others are 8 rows on each
+  const size_t at0 = (size_t)((uint64_t)r0 + t0 + g - pos) * p.row_stride + h * HD + lane * 4u, step = 8u * p.row_stride;
   float4 x[2][4][C];
 #pragma unroll
   for (uint32_t j = 0; j < 4u; ++j) {
     const uint64_t t = t0 + g + 8u * j;
     in[j] = t >= pos && t < pos + n;
-    at[j] = in[j] ? (size_t)(r0 + (uint32_t)(t - pos)) * p.row_stride + h * HD + lane * 4u : 0u;
     if (!READ)  // the rows fly while the page is looked up
 #pragma unroll
       for (uint32_t c = 0; c < C; ++c) {
         x[0][j][c] = x[1][j][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (in[j] && on) {
-          x[0][j][c] = __ldcs(reinterpret_cast<const float4*>(p.k + at[j] + c * 128u));
-          x[1][j][c] = __ldcs(reinterpret_cast<const float4*>(p.v + at[j] + c * 128u));
+          x[0][j][c] = __ldcs(reinterpret_cast<const float4*>(p.k + at0 + j * step + c * 128u));
+          x[1][j][c] = __ldcs(reinterpret_cast<const float4*>(p.v + at0 + j * step + c * 128u));
         }
       }
   }
@@ -256,8 +262,8 @@ __global__ void __launch_bounds__(256) kv_quarter_kernel(const KvCopyParams p) {
       if (!in[j] || !on) continue;
 #pragma unroll
       for (uint32_t c = 0; c < C; ++c) {
-        __stcs(reinterpret_cast<float4*>(p.k + at[j] + c * 128u), kv_value4(kw[j][c], ks[j]));
-        __stcs(reinterpret_cast<float4*>(p.v + at[j] + c * 128u),
+        __stcs(reinterpret_cast<float4*>(p.k + at0 + j * step + c * 128u), kv_value4(kw[j][c], ks[j]));
+        __stcs(reinterpret_cast<float4*>(p.v + at0 + j * step + c * 128u),
                kv_value4(kv_pick_bytes(w[c][0], w[c][1], w[c][2], w[c][3], j), vs[j]));
       }
     }
