@@ -32,23 +32,26 @@
 // further columns of the same product (N = 3 rows), so a page of keys is one M
 // = 128 (tokens) operand and a page of values one M = 128 (dimensions) operand
 // whatever the number of rows, both as the cache holds them: a page is copied
-// to shared memory and multiplied.  s32 to f32: |sum| < 2^22, so sum + (bits of
-// 1.5 2^23) is a float 1.5 2^23 + sum (an integer and an f32 addition, not the
-// conversion pipe).  The units' tiles (pages) form one line, cut into equal
-// pieces, one per CTA, whatever the mixture of lengths; every CTA computes the
-// line's layout from the lengths.  Joining the digits and the softmax bound it
-// (about 35 instructions per pair of score and output; 48 rows x 4 heads over
-// 65537 tokens: 312 us, memory alone 27); for few rows over a long prefix the
-// page copies do (8 rows over 16384 tokens of 32 heads: 51 us, memory alone
-// 21), and for small calls the chain launch - lengths - table - page.
-// Widening the cache to f16 and multiplying hi and lo halves needs no joining,
-// but the widening and splitting cost as much (340 us, and 112 us for the 8
-// rows).
+// to shared memory and multiplied.  Sums become floats without a conversion: a
+// product of constants first puts a bias on every sum, and a sum that is not
+// negative is a subnormal float, see attn_join (with an integer addition per sum
+// instead: 293 us where this took 261).  The units' tiles (pages) form one line,
+// cut into equal pieces, one per CTA, whatever the mixture of lengths; every CTA
+// computes the line's layout from the lengths.  Joining the digits and the
+// softmax bound it (22 instructions per pair of score and output; 48 rows x 32
+// heads over 65537 tokens of 8 heads: 240 us, memory alone 27; issue slots 55 %
+// taken, the rest waits on the chain score - maximum - exponent); for few rows
+// over a long prefix the page copies do (8 rows over 16384 tokens of 32 heads:
+// 49 us, memory alone 21), and for small calls the chain launch - lengths -
+// table - page.  Widening the cache to f16 and multiplying hi and lo halves needs
+// no joining, but the widening and splitting cost as much (340 us and 112 us for
+// these two, when digits took 346 and 54).
 //
-// A CTA: warps 0..7 score and fold -- four on the even tiles of a piece, four on
-// the odd ones, so that one half's chain of waits is the other's work --, warp
-// 8 copies pages, warp 9 issues the products, whichever is ready first.  A
-// tile's probabilities take the place of its keys in shared memory.
+// A CTA: eight warps for every 16 rows score and fold -- half of them on the even
+// tiles of a piece, half on the odd ones, so that one half's chain of waits is
+// the other's work --, a warp copies pages, and one issues the products,
+// whichever is ready first.  A tile's probabilities take the place of its keys in
+// shared memory.
 #include "eos_kernels.h"
 #include "kv_q8.cuh"
 
@@ -403,10 +406,10 @@ __device__ __forceinline__ float attn_warp_max(float x) {
 // sequence's own tokens, a decode step) take one round trip to memory.
 // Queries as in the tensor-core kernel, probabilities with 8 bits more; s32 sums
 // over 16 dimensions (scores) and over a page (values) are exact.
-// Measured both ways: 8 rows over 16384 tokens of 32 heads 138 us here, 51 on the
-// tensor cores; 384 units of four rows (up to 700 tokens) beside a prefix of
-// 65537, in all 312 us with them here, 306 with them there; one row over 640
-// tokens of 32 heads 4.9 us here (one launch), 10 there.
+// Measured both ways: 8 rows over 16384 tokens of 32 heads 138 us here, 49 on the
+// tensor cores; four rows over 640 tokens of 8 heads 7.5 here, 11.4 there; 128
+// units of four rows over 300 tokens 10.7 and 13.2; 384 of up to 700 tokens beside
+// a prefix of 65537 239 and 233 in all.
 constexpr uint32_t kFewRows = 4;
 constexpr uint32_t kFewThreads = 128;
 
@@ -769,8 +772,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // ---- geometry of a CTA ------------------------------------------------------
 // Row groups of 16 (three digits each: N = 48), two CTAs per SM, for few rows: the
 // page copies of four tiles in flight hide each other's latency.  Groups of 32,
-// one CTA per SM, read a page half as often and share a tile's fixed work: 192
-// rows over 65537 tokens 346 -> 314 us; with 16 rows half its columns would be empty.
+// one CTA per SM, read a page half as often and share a tile's fixed work: 40
+// rows over 65536 tokens of 8 heads 101 -> 95 us, 20 over 16384 of 32 74 -> 60;
+// with 16 rows half its columns would be empty.  Their sixteen warps (two for the
+// same 32 tokens, 16 rows each) took 293 us where eight with 32 rows each took 312.
 // (Two CTAs of 32 do not fit the registers; 64 dimensions leave no room for 96
 // rows of probabilities, 256 none for the value sums.)
 template <uint32_t HD, uint32_t RT>
