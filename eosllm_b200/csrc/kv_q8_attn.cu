@@ -38,7 +38,7 @@
 // instead: 293 us where this took 261).  The units' tiles (pages) form one line,
 // cut into equal pieces, one per CTA, whatever the mixture of lengths; every CTA
 // computes the line's layout from the lengths.  Joining the digits and the
-// softmax bound it (22 instructions per pair of score and output; 48 rows x 32
+// softmax bound it (44 instructions per pair of score and output; 48 rows x 32
 // heads over 65537 tokens of 8 heads: 240 us, memory alone 27; issue slots 55 %
 // taken, the rest waits on the chain score - maximum - exponent); for few rows
 // over a long prefix the page copies do (8 rows over 16384 tokens of 32 heads:
