@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvCopyParams p) {
 // the same rows are neighbours in the grid, so that what runs together is
 // together in memory (reading 16383 rows x 32 heads: 117 us head by head, 107
 // so, 6.3 TB/s).  A write's registers are held to 64 a thread, four CTAs an SM:
-// at three, 8505 rows x 8 heads took 21.4 us, at four 19.9 (4.4 TB/s; loads,
+// at three, 8505 rows x 8 heads took 21.4 us, at four 19.5 (4.5 TB/s; loads,
 // rounding and stores of a CTA follow one another); keys and values in CTAs of
 // their own 24.3.
 //

@@ -95,16 +95,17 @@ __device__ __forceinline__ uint32_t kv_find(const KvRows& b, const uint32_t* wor
 // is off by at most 127 * 2^-24 < 1e-5, so wherever it lies 1e-4 away from a
 // half it decides: it is rounded by adding 1.5 * 2^23, which leaves q in the
 // sum's low byte, and its distance from q is exact.  Otherwise (about one
-// element in 5000) the f64 quotient decides, whose rounding cannot move it
-// across a half (127 x is exact, and a quotient of two floats that is not a
-// half differs from it by more than 2^-33 relative).  A row that holds a NaN
-// or an infinity gets that as its scale and q = 0: it reads back as NaN.
+// element in 5000) 127 x is compared with h max|x|, h the half: products of
+// at most 33 bits, each held exactly as a float and its remainder (fma), whose
+// differences are exact too.  Rows below 2^-100 or above 2^120 are scaled by a
+// power of two first, so that neither 127 / max|x| nor these products leave the
+// range.  A row that holds a NaN or an infinity gets that as its scale and q = 0:
+// it reads back as NaN.
 //
 // Elements go in pairs and maxima in threes: 17 million elements (a prompt batch's
 // keys and values) took 22.7 us with single ones, when issuing bound it.
 struct KvRowScale {
-  float scale, amax, inv;
-  bool special;  // not finite, or below 2^-100 (127 / max|x| may overflow)
+  float scale, amax, inv, factor;  // amax and inv of the row times factor; factor 0: not finite
 };
 // max(|a|, |b|, |c|), NaN if one is
 __device__ __forceinline__ float kv_max3(float a, float b, float c) {
@@ -129,30 +130,37 @@ __device__ __forceinline__ float2 kv_fma2(float2 a, float2 b, float2 c) {
 __device__ __forceinline__ KvRowScale kv_row_scale(float lane_amax) {
   const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(lane_amax) & 0x7fffffffu);
   KvRowScale s;
-  s.amax = __uint_as_float(bits);
-  s.special = !(s.amax >= 7.8886e-31f && bits < 0x7f800000u);
-  s.scale = __fmul_rn(s.amax, 1.0f / 127.0f);
-  s.inv = s.special ? 0.0f : __fdiv_rn(127.0f, s.amax);
+  const float amax = __uint_as_float(bits);
+  s.factor = bits >= 0x7f800000u ? 0.0f : (amax < 7.8886e-31f ? 1.2676506e30f : (amax > 1.329228e36f ? 5.421011e-20f : 1.0f));
+  s.scale = __fmul_rn(amax, 1.0f / 127.0f);
+  s.amax = s.factor > 0.0f ? amax * s.factor : 0.0f;
+  s.inv = s.amax > 0.0f ? __fdiv_rn(127.0f, s.amax) : 0.0f;
   return s;
 }
-static __device__ __noinline__ uint32_t kv_quant4_exact(float4 v, float amax) {
-  const double d = (double)amax;
-  return !(amax > 0.0f && amax < INFINITY)
-             ? 0u
-             : ((uint32_t)((int32_t)rint(127.0 * (double)v.x / d) & 0xff) |
-                ((uint32_t)((int32_t)rint(127.0 * (double)v.y / d) & 0xff) << 8) |
-                ((uint32_t)((int32_t)rint(127.0 * (double)v.z / d) & 0xff) << 16) |
-                ((uint32_t)((int32_t)rint(127.0 * (double)v.w / d) & 0xff) << 24));
+// r = 1.5 2^23 + q of the estimate, o its distance from the estimate: the other neighbour if that is nearer.
+__device__ __forceinline__ float kv_near_half(float x, float r, float o, float amax) {
+  const float sg = copysignf(0.5f, o), h = __fadd_rn(__fsub_rn(r, 12582912.0f), sg);
+  const float a = __fmul_rn(127.0f, x), b = __fmul_rn(h, amax);
+  const float d = __fadd_rn(__fsub_rn(a, b), __fsub_rn(__fmaf_rn(127.0f, x, -a), __fmaf_rn(h, amax, -b)));
+  const bool over = sg > 0.0f ? d > 0.0f : d < 0.0f, odd = (__float_as_uint(r) & 1u) != 0u;
+  return fabsf(o) > 0.4999f && (over || (d == 0.0f && odd)) ? r + 2.0f * sg : r;
 }
 // Four elements as the bytes of a word.
 __device__ __forceinline__ uint32_t kv_quant4(float4 v, const KvRowScale& s) {
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
   const float2 magic = make_float2(kMagic, kMagic), inv = make_float2(s.inv, s.inv), minus = make_float2(-1.0f, -1.0f);
+  if (s.factor != 1.0f) {  // warp-uniform
+    const bool on = s.factor > 0.0f;
+    v = make_float4(on ? v.x * s.factor : 0.0f, on ? v.y * s.factor : 0.0f, on ? v.z * s.factor : 0.0f,
+                    on ? v.w * s.factor : 0.0f);
+  }
   const float2 x0 = make_float2(v.x, v.y), x1 = make_float2(v.z, v.w);
-  const float2 r0 = kv_fma2(x0, inv, magic), r1 = kv_fma2(x1, inv, magic);
+  float2 r0 = kv_fma2(x0, inv, magic), r1 = kv_fma2(x1, inv, magic);
   const float2 o0 = kv_fma2(x0, inv, kv_fma2(r0, minus, magic)), o1 = kv_fma2(x1, inv, kv_fma2(r1, minus, magic));
-  const float off = kv_max3(kv_max3(o0.x, o0.y, o1.x), o1.y, o1.y);
-  if (off > 0.4999f || s.special) return kv_quant4_exact(v, s.amax);
+  if (kv_max3(kv_max3(o0.x, o0.y, o1.x), o1.y, o1.y) > 0.4999f) {
+    r0 = make_float2(kv_near_half(x0.x, r0.x, o0.x, s.amax), kv_near_half(x0.y, r0.y, o0.y, s.amax));
+    r1 = make_float2(kv_near_half(x1.x, r1.x, o1.x, s.amax), kv_near_half(x1.y, r1.y, o1.y, s.amax));
+  }
   return __byte_perm(__byte_perm(__float_as_uint(r0.x), __float_as_uint(r0.y), 0x0040),
                      __byte_perm(__float_as_uint(r1.x), __float_as_uint(r1.y), 0x0040), 0x5410);
 }

@@ -60,6 +60,7 @@ namespace eos {
 constexpr uint32_t kAttnMaxCtas = 320;    // bound on the grid (scratch is sized with it)
 constexpr uint32_t kAttnMl = 8;           // floats per partial row: maximum, 3 unused, 4 partial sums
 constexpr float kAttnLow = -3e38f;        // reference of tiles whose tokens are all hidden: finite, so that no difference is NaN
+constexpr float kAttnFar = 1e6f;          // log2 scores beyond this are compared before they are scaled
 constexpr float kAttnQMax = 8300000.0f;   // largest query integer (three balanced digits hold 127 * 65793)
 
 // Division of x < 2^31 by a launch constant: a multiplication (error below
@@ -611,11 +612,13 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
       const float mt = fmaxf(fmaxf(rd[0][r], rd[1][r]), fmaxf(rd[2][r], rd[3][r]));
-      const float nm = fmaxf(mt == -INFINITY ? mt : __fmul_ru(mt, qscale[r]), m[r]);
+      const float ref = mt == -INFINITY ? mt : __fmul_ru(mt, qscale[r]), nm = fmaxf(ref, m[r]);
       const float neg = nm == -INFINITY ? 0.0f : -nm;
       f[r] = attn_ex2(m[r] + neg);
       m[r] = nm;
-      const float e = attn_ex2(fmaf(z[r], qscale[r], neg));
+      // (scores so large that a rounding of the reference is no common factor any more: relative to the page's largest)
+      const float e = attn_ex2(fabsf(nm) > kAttnFar ? fmaf(z[r] - fmaxf(mt, kAttnLow), qscale[r], ref + neg)
+                                                    : fmaf(z[r], qscale[r], neg));
       l[r] = fmaf(l[r], f[r], e);  // this token's share
       // e vs as 23 bits (the low bytes of 2^23 + ..) and a signed byte of what is left, in 1 / 256
       const float y = vs * up, b = fmaf(e, y, 8388608.0f), rest = fmaf(e, y, 8388608.0f - b);
@@ -1289,7 +1292,10 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           // (its integers are relative to it: their rounding fades with the tile)
           const float t0 = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x)), t1 = fmaxf(fmaxf(m0.y, m1.y), fmaxf(m2.y, m3.y));
           const float2 ref = make_float2(fmaxf(__fmul_ru(t0, qsc.x), kAttnLow), fmaxf(__fmul_ru(t1, qsc.y), kAttnLow));
-          const float2 neg = make_float2(-ref.x, -ref.y);
+          // z = (score - t) c + (t c - ref): the reference's rounding is a common factor as long as it is one
+          const float2 t = make_float2(-fmaxf(t0, kAttnLow), -fmaxf(t1, kAttnLow));
+          const float d0 = __fmaf_rn(-t.x, qsc.x, -ref.x), d1 = __fmaf_rn(-t.y, qsc.y, -ref.y);
+          const float2 dl = make_float2(d0 > -0.5f ? d0 : 0.0f, d1 > -0.5f ? d1 : 0.0f);
           const float2 nm = make_float2(fmaxf(ref.x, m[y].x), fmaxf(ref.y, m[y].y));
           f[y] = make_float2(attn_ex2(m[y].x - nm.x), attn_ex2(m[y].y - nm.y));
           const float2 share = make_float2(attn_ex2(ref.x - nm.x), attn_ex2(ref.y - nm.y));
@@ -1299,7 +1305,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           float2 ls = attn_two(0.0f);
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) {
-            const float2 z = attn_fma2(sv[y][j], qsc, neg);
+            const float2 z = attn_fma2(attn_add2(sv[y][j], t), qsc, dl);
             const float2 e = make_float2(attn_ex2(z.x), attn_ex2(z.y));
             ls = attn_add2(ls, e);
             const float2 w = attn_fma2(e, attn_two(vw[j]), attn_two(8388608.0f));

@@ -285,6 +285,32 @@ def test_softmax_scales(gpu, scale):
     Batch(gpu, 4, 2, 128, 140, [20, 3], [3, 1], seed=17, q_gain=0.5, edit=edit).check()
 
 
+@pytest.mark.parametrize("gain", [1e30, 1e-25])
+def test_large_queries_small_keys_and_the_reverse(gpu, gain):
+    """Scores of ordinary size from factors far apart."""
+    def edit(b):
+        b.q *= np.float32(gain)
+        for x in [b.kp] + b.ks:
+            x *= np.float32(1 / gain)
+    Batch(gpu, 4, 2, 128, 300, [140, 40], [2, 30], seed=19, edit=edit).check()
+
+
+@pytest.mark.parametrize("gain,prefix,counts", [(1e36, 300, [2, 30]), (1e36, 0, [1, 1]), (1e30, 300, [2, 30]), (1e30, 20, [2, 2])])
+def test_scores_beyond_every_exponent(gpu, gain, prefix, counts):
+    """Scores of 1e3 to 1e10: one value row each, no NaN."""
+    def edit(b):
+        b.q *= np.float32(gain)
+        for x in [b.kp] + b.ks:
+            x *= np.float32(1e-29)
+        b.scale = 40.0
+    b = Batch(gpu, 4, 2, 128, prefix, [140, 40], counts, seed=20, edit=edit)
+    got = b.check()
+    vals = np.concatenate([stored(b.vp)[0]] + [stored(v)[0] for v in b.vs])
+    for r in {0, 1, min(10, sum(counts) - 1), sum(counts) - 1}:  # each output is one of the stored value rows
+        for h in range(4):
+            assert np.abs(vals[:, h // 2] - got[r, h]).max(-1).min() <= 1e-5 * np.abs(vals).max()
+
+
 def test_nan_and_infinity_reach_only_rows_that_see_them(gpu):
     def edit(b):
         b.ks[0][3, 0, 5] = np.nan      # seen by every row of sequence 0's heads 0, 1
