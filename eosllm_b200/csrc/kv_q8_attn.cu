@@ -22,10 +22,11 @@
 // rounding anywhere.  A probability p times weight w becomes an integer as the
 // mantissa of the float 2^23 + p w, whose three low bytes are the digits.
 //
-// Scores are compared before the row's query scale and the softmax scale are
-// applied (z = sum * key scale), and the exponent is fma(z, c, -reference): a
-// rounding of c or of the reference is common to the row and cancels.  One
-// pass with a running maximum and sum per row in f32; each tile's value sums
+// Scores are compared before the row's query scale c (which holds the softmax
+// scale) is applied: z = sum * key scale, exponent (z - max z) c plus the exact
+// rest max z c - reference, so a rounding of the reference is common to the row
+// and cancels; where it is no longer small (scores of 1e7) the rest is left out.
+// One pass with a running maximum and sum per row in f32; each tile's value sums
 // are folded into f32 registers.
 //
 // On the tensor cores the products are tcgen05.mma kind::i8.  The digits are
@@ -39,7 +40,7 @@
 // cut into equal pieces, one per CTA, whatever the mixture of lengths; every CTA
 // computes the line's layout from the lengths.  Joining the digits and the
 // softmax bound it (44 instructions per pair of score and output; 48 rows x 32
-// heads over 65537 tokens of 8 heads: 240 us, memory alone 27; issue slots 55 %
+// heads over 65537 tokens of 8 heads: 245 us, memory alone 27; issue slots 55 %
 // taken, the rest waits on the chain score - maximum - exponent); for few rows
 // over a long prefix the page copies do (8 rows over 16384 tokens of 32 heads:
 // 49 us, memory alone 21), and for small calls the chain launch - lengths -
