@@ -78,6 +78,21 @@ def test_write_read(gpu, hd, kvh, counts, pos):
     assert gpu.take_device_errors() == 0
 
 
+@pytest.mark.parametrize("n_seq,most", [(32, 2), (33, 3), (70, 40), (1100, 1), (1100, 12)])
+def test_write_read_many_sequences(gpu, n_seq, most):
+    """More sequences than one look-up holds, empty ones among them, row by row and by quarters."""
+    rng = np.random.default_rng(n_seq + most)
+    counts = rng.integers(0, most + 1, n_seq)
+    pos = rng.integers(0, 100, n_seq)
+    counts[-1], counts[n_seq // 2:n_seq // 2 + 3] = most, 0
+    k, v = rows(rng, int(counts.sum()), 1, 64), rows(rng, int(counts.sum()), 1, 64)
+    c = Cache(gpu, 1, 64, list(pos + counts + 1), seed=3)
+    c.write(k, v, list(counts), list(pos))
+    kr, vr = c.read(list(counts), list(pos))
+    assert same(kr, stored(k)[0]) and same(vr, stored(v)[0])
+    assert gpu.take_device_errors() == 0
+
+
 def test_write_edge_values(gpu):
     """Zeros, subnormals, the largest floats, exact halves (ties), values just
     beside a half, NaN and infinities."""
