@@ -224,13 +224,19 @@ __device__ constexpr uint32_t attn_idesc(bool a_signed, bool b_signed, uint32_t 
 }
 // An operand of bytes 255 throughout: cores of 8 rows x 16 bytes, no swizzle,
 // neighbours 16 bytes apart, so that 128 rows of 32 bytes are kAttnOnes bytes.
-// A product of two adds 32 * 255 * 255 = kAttnBias to every sum: at least the
-// largest negative score sum (128 elements of -128 * 127); two such products
-// cover a value sum (128 tokens of 255 * -127).
+// A product of two adds 32 * 255 * 255 = kAttnBias to every sum, one for every
+// 128 dimensions at least the largest negative score sum (each element -128 *
+// 127); two cover a value sum (128 tokens of 255 * -127).
 constexpr uint32_t kAttnOnes = 384, kAttnBias = 32u * 255u * 255u;
-static_assert(kAttnBias >= 128u * 128u * 127u && 2u * kAttnBias >= 128u * 255u * 127u &&
-                  2u * kAttnBias + 128u * 255u * 127u < (1u << 23),
-              "biased sums are not negative and below 2^23");
+__host__ __device__ constexpr uint32_t attn_score_biases(uint32_t hd) { return hd <= 128u ? 1u : hd / 128u; }
+constexpr bool attn_bias_covers(uint32_t biases, uint64_t sum) {  // biased sums are not negative and below 2^23
+  return (uint64_t)biases * kAttnBias >= sum && (uint64_t)biases * kAttnBias + sum < (1ull << 23);
+}
+static_assert(attn_bias_covers(attn_score_biases(64), 64u * 128u * 127u) &&
+                  attn_bias_covers(attn_score_biases(128), 128u * 128u * 127u) &&
+                  attn_bias_covers(attn_score_biases(256), 256u * 128u * 127u) &&
+                  attn_bias_covers(2u, 128u * 255u * 127u),
+              "a biased sum reads as a subnormal float");
 __device__ __forceinline__ uint64_t attn_ones_desc(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)1u << 32) | ((uint64_t)1u << 46);
 }
@@ -1042,7 +1048,9 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
               attn_fence_after();
               const uint32_t ka = smem_u32(stages + (y % S) * G::kBlock), qa = smem_u32(qop);
               constexpr uint32_t id = attn_idesc(true, true, 3u * RT);
-              attn_mma(tmem + h * G::kAcc, ones_desc, ones_desc, attn_idesc(false, false, 3u * RT), 0u);
+#pragma unroll
+              for (uint32_t b = 0; b < attn_score_biases(HD); ++b)
+                attn_mma(tmem + h * G::kAcc, ones_desc, ones_desc, attn_idesc(false, false, 3u * RT), b);
 #pragma unroll
               for (uint32_t ks = 0; ks < HD / 32u; ++ks) {
                 const uint32_t panel = ks / 4u, off = (ks % 4u) * 32u;
@@ -1229,7 +1237,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         float2 sv[NC][4];
         attn_sums<RT>(tmem + half * G::kAcc + ((quad * 32u) << 16) + c0, nact,
                       [&](uint32_t y, uint32_t j, const uint32_t* d0, const uint32_t* d1, const uint32_t* d2) {
-                        sv[y][j] = attn_mul2(attn_join<kAttnBias>(d0, d1, d2), attn_two(ks[j]));
+                        sv[y][j] = attn_mul2(attn_join<attn_score_biases(HD) * kAttnBias>(d0, d1, d2), attn_two(ks[j]));
                       });
         float2 mx[NC];
 #pragma unroll
