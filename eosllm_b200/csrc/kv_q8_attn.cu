@@ -451,15 +451,15 @@ __device__ __forceinline__ float attn_peer(const float* x, uint32_t rank) {
 // Grid (clusters x CTAs, kv heads, sequences); prefix: one "sequence" of all
 // rows.  direct: there is nothing to join the rows with, write them out.
 template <uint32_t HD, uint32_t R>
-__global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnParams p, uint32_t prefix,
-                                                                  uint32_t n_cta, uint32_t direct) {
+__global__ void __launch_bounds__(kFewThreads, HD <= 128u ? 4 : (R == 1u ? 3 : 2))
+    kv_attn_few_kernel(const KvAttnParams p, uint32_t prefix, uint32_t n_cta, uint32_t direct) {
   constexpr uint32_t CL = HD / 16u;                    // 16-byte chunks of a key row = lanes per token
   constexpr uint32_t DT = HD <= 128u ? 1u : HD / 128u; // dimensions per thread
   constexpr uint32_t QT = HD == 64u ? 2u : 4u;         // quarters of the values per thread
   __shared__ __align__(16) uint32_t qd[R][3][HD / 4u]; // query digits
   __shared__ float qscale[R];
   __shared__ __align__(16) uint8_t pd[R][4][kKvPage];  // probability digits by position
-  __shared__ float red[2][4][R + 1u];                  // per warp: maxima, largest value scale
+  __shared__ float red[2][4][2u * R];                  // per warp: maxima, largest value scales
   __shared__ float cl_o[R][HD], cl_ml[R][2];           // this CTA's sums, for the cluster
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t g = blockIdx.y;
@@ -606,19 +606,27 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
       const float mx = attn_warp_max(z[r]);
       if (lane == 0) red[par][warp][r] = mx;
     }
-    {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vs));
-      if (lane == 0) red[par][warp][R] = __uint_as_float(top);
+    // the largest value scale that a row sees: one for all, or one each where the page ends behind the first row's
+    // tokens (what such a page hides has z = -infinity)
+    const bool cut = !prefix && (int32_t)min(s.len, (pg + 1u) * kKvPage) > seen0;
+#pragma unroll
+    for (uint32_t r = 0; r < R; ++r) {
+      if (r > 0 && !cut) break;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, cut && z[r] == -INFINITY ? 0u : __float_as_uint(vs));
+      if (lane == 0) red[par][warp][R + r] = __uint_as_float(top);
     }
     __syncthreads();
-    const float(*rd)[R + 1u] = red[par];
-    uint32_t top = __float_as_uint(fmaxf(fmaxf(rd[0][R], rd[1][R]), fmaxf(rd[2][R], rd[3][R]))) >> 23;
-    top = top < 23u ? 23u : top;
-    const float up = __uint_as_float((276u - top) << 23), unit = __uint_as_float((top - 22u) << 23);
+    const float(*rd)[2u * R] = red[par];
+    auto exponent = [&](uint32_t r) {
+      const float most = fmaxf(fmaxf(rd[0][R + r], rd[1][R + r]), fmaxf(rd[2][R + r], rd[3][R + r]));
+      return max(__float_as_uint(most) >> 23, 23u);
+    };
+    const uint32_t common = exponent(0);
     float f[R];
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
       const float mt = fmaxf(fmaxf(rd[0][r], rd[1][r]), fmaxf(rd[2][r], rd[3][r]));
+      const uint32_t top = r > 0 && cut ? exponent(r) : common;
       const float ref = mt == -INFINITY ? mt : __fmul_ru(mt, qscale[r]), nm = fmaxf(ref, m[r]);
       const float neg = nm == -INFINITY ? 0.0f : -nm;
       f[r] = attn_ex2(m[r] + neg);
@@ -628,7 +636,8 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
                                                     : fmaf(z[r], qscale[r], neg));
       l[r] = fmaf(l[r], f[r], e);  // this token's share
       // e vs as 23 bits (the low bytes of 2^23 + ..) and a signed byte of what is left, in 1 / 256
-      const float y = vs * up, b = fmaf(e, y, 8388608.0f), rest = fmaf(e, y, 8388608.0f - b);
+      const float y = cut && z[r] == -INFINITY ? 0.0f : vs * __uint_as_float((276u - top) << 23);
+      const float b = fmaf(e, y, 8388608.0f), rest = fmaf(e, y, 8388608.0f - b);
       const uint32_t w = __float_as_uint(b);
       uint8_t* at = &pd[r][0][warp * 32u + kv_v_position(own)];
       at[0] = (uint8_t)w;
@@ -640,6 +649,7 @@ __global__ void __launch_bounds__(kFewThreads) kv_attn_few_kernel(const KvAttnPa
     // values
 #pragma unroll
     for (uint32_t r = 0; r < R; ++r) {
+      const float unit = __uint_as_float(((r > 0 && cut ? exponent(r) : common) - 22u) << 23);
       int32_t a[DT][4];
 #pragma unroll
       for (uint32_t d = 0; d < DT; ++d) a[d][0] = a[d][1] = a[d][2] = a[d][3] = 0;
@@ -824,7 +834,11 @@ struct AttnBars {
   AttnJob job[2];
 };
 
-template <uint32_t HD, uint32_t RT>
+// CAUSAL: some unit's columns see different numbers of tokens (several rows of a sequence).  Without it the columns of
+// a tile share one unit of the probabilities; a unit of their own costs them a product per pair of probabilities (seven
+// sequences of up to 6 rows over 1537 tokens of 32 heads 27.0 us, 26.0 with a shared unit, which let the value rows
+// behind a row's last token coarsen its weights).
+template <uint32_t HD, uint32_t RT, bool CAUSAL>
 __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>::kCtas)) kv_attn_kernel(const KvAttnParams p) {
   using G = AttnGeo<HD, RT>;
   constexpr uint32_t S = G::kStages;
@@ -1187,7 +1201,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         const AttnJob& job = bar.job[nj & 1u];
         return min(job.seen0 + (int32_t)attn_div(job.row0 + col, p.by_group), (int32_t)job.left);
       };
-      const int32_t common = limit(0);
+      const int32_t common = limit(0), most = limit(s.rows - 1u);  // .. and none more than `most`
       float2 fold[NC];         // the last tile's probability unit, relative to the running reference
       uint32_t it = n_own;     // tiles of this half so far
       // o = o f + fold * (value product of the tile before)
@@ -1218,12 +1232,21 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         const uint32_t avail = bar.ok[st] ? s.left - tok0 : 0u;  // tokens of the tile (may exceed a page)
         // the scales of quarter quad, token `lane`; this thread's four tokens are g + 8 j
         uint32_t vbits = *reinterpret_cast<const uint32_t*>(sc + quad * 256u + 128u + lane * 4u);
+        uint32_t vown;  // .. its value scale; vbits: the same if every column sees the token
         float ks[4];
+        // the tile's tokens, those that every column sees and those that one sees; between the two (a cut tile) a
+        // column's largest value scale is its own, so that no row's rounding depends on tokens behind its last
+        const int32_t held = (int32_t)min(avail, kKvPage), least = max(common - (int32_t)tok0, 0),
+                      some = min(most - (int32_t)tok0, held);
+        const bool cut = CAUSAL && least < some;
         {
           const bool in = quad * 32u + lane < avail, sound = vbits < 0x7f800000u;
           const float kv = *reinterpret_cast<const float*>(sc + quad * 256u + lane * 4u);
           const float k1 = in ? (sound ? 32.0f * kv : NAN) : 0.0f;      // a NaN or infinite value row: NaN score
           vbits = in && sound ? vbits : 0u;
+          vown = vbits;
+          if constexpr (CAUSAL)
+            if (cut && (int32_t)(quad * 32u + lane) >= least) vbits = 0u;
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) ks[j] = __shfl_sync(0xffffffffu, k1, g + 8u * j);
         }
@@ -1277,16 +1300,37 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         if (t > half) live = fold_tile();
         if (live) live = __all_sync(0xffffffffu, attn_wait(&bar.xmax[half][grp], it & 1u)) != 0;
         if (!live) break;
-        // unit of the probabilities: a power of two from the tile's largest value scale
-        float unit, vw[4];
+        // unit of the probabilities: a power of two from the largest value scale that a column sees in the tile (`top`:
+        // its exponent), one for all columns unless the tile is cut
+        uint32_t top[NC][2];
+        float vw[4];
         {
           const uint4 t4 = *reinterpret_cast<const uint4*>(xt);
-          const uint32_t top = max(max(max(t4.x, t4.y), max(t4.z, t4.w)) >> 23, 23u);
-          const float v1 = __uint_as_float(vbits) * __uint_as_float((276u - top) << 23);  // times 2^(22 - exponent)
-          unit = __uint_as_float(top << 23);  // 2^exponent: value sums are held in units of 256
+          const uint32_t all = max(max(max(t4.x, t4.y), max(t4.z, t4.w)) >> 23, 23u);
+          const float v1 = CAUSAL ? __uint_as_float(vown)
+                                  : __uint_as_float(vbits) * __uint_as_float((276u - all) << 23);  // times 2^(22 - exponent)
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) vw[j] = __shfl_sync(0xffffffffu, v1, g + 8u * j);
+#pragma unroll
+          for (uint32_t y = 0; y < NC; ++y) top[y][0] = top[y][1] = all;
         }
+        if constexpr (CAUSAL)
+          if (cut) {  // lane l: the largest scale of the tokens from `least` to l behind it (a group's rows are at most 32)
+            const uint32_t tok = (uint32_t)least + lane;
+            uint32_t v = 0;
+            if ((int32_t)tok < some) v = *reinterpret_cast<const uint32_t*>(sc + (tok >> 5) * 256u + 128u + (tok & 31u) * 4u);
+            if (v >= 0x7f800000u) v = 0u;
+#pragma unroll
+            for (uint32_t o = 1; o < 32u; o <<= 1) v = max(v, __shfl_up_sync(0xffffffffu, v, o));
+#pragma unroll
+            for (uint32_t y = 0; y < NC; ++y)
+#pragma unroll
+              for (uint32_t z = 0; z < 2u; ++z) {
+                const int32_t n = limit(c0 + 8u * y + 2u * cq + z) - (int32_t)tok0 - least;
+                const uint32_t w = __shfl_sync(0xffffffffu, v, min(max(n - 1, 0), 31));
+                if (n > 0) top[y][z] = max(top[y][z], w >> 23);
+              }
+          }
         uint8_t* pop = stages + st * G::kBlock;  // the probabilities take the place of the keys
 #pragma unroll
         for (uint32_t y = 0; y < NC; ++y) {
@@ -1308,7 +1352,10 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           const float2 nm = make_float2(fmaxf(ref.x, m[y].x), fmaxf(ref.y, m[y].y));
           f[y] = make_float2(attn_ex2(m[y].x - nm.x), attn_ex2(m[y].y - nm.y));
           const float2 share = make_float2(attn_ex2(ref.x - nm.x), attn_ex2(ref.y - nm.y));
-          fold[y] = attn_mul2(share, attn_two(unit));
+          // 2^exponent: value sums are held in units of 256
+          const float2 un = make_float2(__uint_as_float(top[y][0] << 23), __uint_as_float(top[y][1] << 23));
+          const float2 up = make_float2(__uint_as_float((276u - top[y][0]) << 23), __uint_as_float((276u - top[y][1]) << 23));
+          fold[y] = attn_mul2(share, un);
           m[y] = nm;
           uint32_t b0[4], b1[4], d[3];
           float2 ls = attn_two(0.0f);
@@ -1317,7 +1364,8 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
             const float2 z = attn_fma2(attn_add2(sv[y][j], t), qsc, dl);
             const float2 e = make_float2(attn_ex2(z.x), attn_ex2(z.y));
             ls = attn_add2(ls, e);
-            const float2 w = attn_fma2(e, attn_two(vw[j]), attn_two(8388608.0f));
+            // (a hidden token's probability, 0, takes the unit first, so that the product is 0 too)
+            const float2 w = attn_fma2(CAUSAL ? attn_mul2(e, up) : e, attn_two(vw[j]), attn_two(8388608.0f));
             b0[j] = __float_as_uint(w.x);
             b1[j] = __float_as_uint(w.y);
           }
@@ -1615,11 +1663,11 @@ cudaError_t attn_few_rows(const KvAttnParams& p, uint32_t prefix, uint32_t rows,
   return attn_few<HD, 4>(p, prefix, direct, st);
 }
 
-template <uint32_t HD, uint32_t RT>
-cudaError_t attn_line(const KvAttnParams& p, int num_sms, uint64_t work, cudaStream_t st) {
+template <uint32_t HD, uint32_t RT, bool CAUSAL>
+cudaError_t attn_line_kernel(const KvAttnParams& p, int num_sms, uint64_t work, cudaStream_t st) {
   using G = AttnGeo<HD, RT>;
   static SmemAttr attr;
-  cudaError_t e = ensure_smem_attr((const void*)kv_attn_kernel<HD, RT>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
+  cudaError_t e = ensure_smem_attr((const void*)kv_attn_kernel<HD, RT, CAUSAL>, (int)G::smem(EOS_ATTN_MAX_SEQ), attr);
   if (e != cudaSuccess) return e;
   uint64_t grid = (uint64_t)G::kCtas * (uint32_t)num_sms;
   if (grid > kAttnMaxCtas) grid = kAttnMaxCtas;
@@ -1638,7 +1686,13 @@ cudaError_t attn_line(const KvAttnParams& p, int num_sms, uint64_t work, cudaStr
   at[0].val.programmaticStreamSerializationAllowed = p.seq_few > 0 || p.prefix_few > 0 ? 1 : 0;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_attn_kernel<HD, RT>, p);
+  return cudaLaunchKernelEx(&cfg, kv_attn_kernel<HD, RT, CAUSAL>, p);
+}
+
+template <uint32_t HD, uint32_t RT>
+cudaError_t attn_line(const KvAttnParams& p, int num_sms, uint64_t work, cudaStream_t st) {
+  return p.max_len > 0 && p.seq_few == 0 && p.max_rows > 1u ? attn_line_kernel<HD, RT, true>(p, num_sms, work, st)
+                                                            : attn_line_kernel<HD, RT, false>(p, num_sms, work, st);
 }
 
 template <uint32_t HD>

@@ -26,3 +26,29 @@ def test_queries_along_and_against_the_keys(gpu, hd, count, pattern, opposed):
             turn = np.where(rng.random((x.shape[0], x.shape[1], 1)) < opposed, -1.0, 1.0)
             x[:] = sign * turn * rng.uniform(0.2, 1.0, (x.shape[0], x.shape[1], 1))
     Batch(gpu, 4, 2, hd, 150, [140], [count], seed=hd, edit=edit).check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n,length,prefix", [(2, 90, 0), (2, 129, 40), (4, 130, 0), (3, 300, 200), (7, 131, 40), (20, 90, 0),
+                                             (40, 290, 130)])
+def test_later_tokens_leave_earlier_rows_as_they_are(gpu, hd, n, length, prefix):
+    """Rows of one sequence whose later tokens -- the other drafts, the rest of a
+    prompt -- hold values 1e4 and 1e9 times as large: the earlier rows keep the
+    accuracy of what they see, and are the same to the bit whatever stands there.
+    Up to four rows a head, and more (H = kv heads, and pairs of heads)."""
+    for H in (2, 4):
+        def edit(b):
+            b.vs[0][length - 1] *= np.float32(1e4)
+            b.vs[0][length - n // 2 - 1] *= np.float32(1e9)
+            b.ks[0][length - 1] *= np.float32(3.0)
+        b = Batch(gpu, H, 2, hd, prefix, [length], [n], seed=n + hd, edit=edit)
+        got = b.check()
+        rng = np.random.default_rng(5)
+        for t in {0, n // 2, n - 2}:  # rows 0 .. t see tokens 0 .. length - n + t
+            seen = length - n + t + 1
+            k, v = rows(rng, length - seen, 2, hd), rows(rng, length - seen, 2, hd)
+            b.c.write(k, np.float32(1e-9) * v if t else v, [length - seen], [seen], first=1)
+            b.run()
+            again = b.out.cpu().numpy()[:n]
+            assert np.array_equal(again[:t + 1].view(np.uint32), got[:t + 1].view(np.uint32)), t
+            b.c.write(b.ks[0], b.vs[0], [length], [0], first=1)
