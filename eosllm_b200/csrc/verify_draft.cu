@@ -60,8 +60,10 @@ __device__ __forceinline__ void vd_weights4(const float* p, const float* q, uint
 
 constexpr uint32_t kVdThreads = 512, kVdWarps = kVdThreads / 32, kVdMaxCluster = 8;
 
+__device__ __forceinline__ void vd_cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void vd_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  vd_cluster_wait();
 }
 // Address of a shared variable in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t vd_map(const void* p, uint32_t rank) {
@@ -86,6 +88,8 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
   __shared__ uint32_t s_last[kVdWarps];
   __shared__ double c_sum[kVdMaxCluster];
   __shared__ uint32_t c_last[kVdMaxCluster];
+  // this CTA runs: the others may write into its shared memory (nothing to be made visible yet)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;");
   const uint32_t i = blockIdx.x / n_cta, cta = blockIdx.x % n_cta;
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t kk = a.max_draft;
@@ -123,6 +127,7 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
   const uint32_t lo = s_lo < steps ? s_lo * 128u : a.n_vocab;
   const uint32_t hi = lo + per * 128u < a.n_vocab ? lo + per * 128u : a.n_vocab;
   bool residual = taken < k;
+  vd_cluster_wait();  // every CTA of the cluster runs
   for (;;) {  // (a second time where p_a <= q_a everywhere: draw from p_a)
     double sum = 0.0;
     uint32_t last = 0;  // 1 + the last index with weight
