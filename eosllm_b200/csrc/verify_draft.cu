@@ -81,16 +81,16 @@ __device__ __forceinline__ uint32_t vd_map(const void* p, uint32_t rank) {
 // many sequences, the chain of three reads (draft, its probabilities, the
 // row) for few: so few sequences get eight CTAs each.  One sequence of 4 drafts
 // and 32000 tokens: 5.9 us; 64 of 7: 10.7 us, of which the 8.2 MB read take 1.3.
-template <bool VEC>
-__global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyParams a, uint32_t n_cta) {
+template <bool VEC, uint32_t NC>
+__global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyParams a) {
   __shared__ uint32_t s_taken;
   __shared__ double s_sum[kVdWarps];
   __shared__ uint32_t s_last[kVdWarps];
-  __shared__ double c_sum[kVdMaxCluster];
-  __shared__ uint32_t c_last[kVdMaxCluster];
+  __shared__ double c_sum[NC];
+  __shared__ uint32_t c_last[NC];
   // this CTA runs: the others may write into its shared memory (nothing to be made visible yet)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;");
-  const uint32_t i = blockIdx.x / n_cta, cta = blockIdx.x % n_cta;
+  const uint32_t i = blockIdx.x / NC, cta = blockIdx.x % NC;
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t kk = a.max_draft;
   uint32_t k = a.n_draft != nullptr ? a.n_draft[i] : kk;
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
   const float* pr = prow + taken * a.stride;
   const float* qr = qrow + taken * a.stride;
   // slices in steps of 128 elements (four per lane)
-  const uint32_t steps = (a.n_vocab + 127u) / 128u, per = (steps + n_cta * kVdWarps - 1u) / (n_cta * kVdWarps);
+  const uint32_t steps = (a.n_vocab + 127u) / 128u, per = (steps + NC * kVdWarps - 1u) / (NC * kVdWarps);
   const uint32_t s_lo = (cta * kVdWarps + warp) * per;
   const uint32_t lo = s_lo < steps ? s_lo * 128u : a.n_vocab;
   const uint32_t hi = lo + per * 128u < a.n_vocab ? lo + per * 128u : a.n_vocab;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
       s_last[warp] = last;
     }
     __syncthreads();
-    if (tid < n_cta) {  // this CTA's sum into every CTA
+    if (tid < NC) {  // this CTA's sum into every CTA
       double t = 0.0;
       uint32_t e = 0;
 #pragma unroll
@@ -162,12 +162,14 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(vd_map(&c_last[cta], tid)), "r"(e) : "memory");
     }
     vd_cluster_sync();
-    double total = 0.0, base = 0.0;
-    uint32_t end = 0;
-    for (uint32_t c = 0; c < n_cta; ++c) {
-      if (c == cta) base = total;
-      total += c_sum[c];
-      end = c_last[c] > end ? c_last[c] : end;
+    double sums[NC], total = 0.0;
+    uint32_t ends[NC], end = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < NC; ++c) {
+      sums[c] = c_sum[c];
+      ends[c] = c_last[c];
+      total += sums[c];
+      end = ends[c] > end ? ends[c] : end;
     }
     if (end == 0 && residual) {
       residual = false;
@@ -175,17 +177,23 @@ __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyPa
       continue;
     }
     const double cut = u * total;
-    // the first slice that crosses the cut or, past every rounding, holds the last weight
-    bool before = false;
-    double run = 0.0;
-    for (uint32_t c = 0; c < cta; ++c) {
-      if (c_last[c] != 0 && (run + c_sum[c] > cut || c_last[c] == end)) before = true;
-      run += c_sum[c];
+    // The slice that crosses the cut or, past every rounding, holds the last weight.  Sums in another order may fall on
+    // the other side of the cut, so who draws is decided once: every CTA finds the first CTA by the same additions, and
+    // that one's warps find the first warp, or the last with weight; its last weight in turn where none crosses there.
+    double base = 0.0, run = 0.0;
+    uint32_t chosen = NC;
+#pragma unroll
+    for (uint32_t c = 0; c < NC; ++c) {
+      if (chosen == NC && ends[c] != 0 && (run + sums[c] > cut || ends[c] == end)) {
+        chosen = c;
+        base = run;
+      }
+      run += sums[c];
     }
     uint32_t pick = kVdWarps;
-    if (!before)
+    if (chosen == cta)
       for (uint32_t w = 0; w < kVdWarps; ++w) {
-        if (s_last[w] != 0 && (base + s_sum[w] > cut || s_last[w] == end)) {
+        if (s_last[w] != 0 && (base + s_sum[w] > cut || s_last[w] == c_last[cta])) {
           pick = w;
           break;
         }
@@ -254,8 +262,10 @@ cudaError_t launch_verify_draft(const float* p, const float* q, uint64_t stride,
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return vec ? cudaLaunchKernelEx(&cfg, verify_draft_kernel<true>, a, n_cta)
-             : cudaLaunchKernelEx(&cfg, verify_draft_kernel<false>, a, n_cta);
+  void (*const fn[2][4])(const VerifyParams) = {
+      {verify_draft_kernel<false, 1>, verify_draft_kernel<false, 2>, verify_draft_kernel<false, 4>, verify_draft_kernel<false, 8>},
+      {verify_draft_kernel<true, 1>, verify_draft_kernel<true, 2>, verify_draft_kernel<true, 4>, verify_draft_kernel<true, 8>}};
+  return cudaLaunchKernelEx(&cfg, fn[vec][n_cta == 8u ? 3 : n_cta / 2u], a);
 }
 
 }  // namespace eos
