@@ -812,6 +812,7 @@ struct TextDecoder {
   XRecv* xrecv(int q) const { return reinterpret_cast<XRecv*>(xpeer[q] + xoff_fl); }
   cudaError_t record_step(cudaStream_t s);
   cudaError_t record_step_persistent(cudaStream_t s);
+  cudaError_t record_graph();
   int capture();
   int set_step_mode(int mode);
   KvPool q8_at(uint32_t L) const { return KvPool{q8_pool + (size_t)L * q8_layer, q8_pages, kvl, hd}; }
@@ -1608,7 +1609,12 @@ int TextDecoder::set_cache(int mode) {
   q8 = want;
   if (graph) cudaGraphExecDestroy(graph);
   graph = nullptr;
-  return capture();
+  e = record_graph();
+  if (e == cudaSuccess) return EOS_OK;
+  set_error_message(e == cudaErrorNotSupported
+                        ? "cuda text: the 8-bit cache does not serve this model (n_head must be a multiple of n_kv_head)"
+                        : cudaGetErrorString(e));
+  return e == cudaErrorNotSupported ? EOS_E_UNSUPPORTED : EOS_E_INTERNAL;
 }
 
 void TextDecoder::close_branches() {
@@ -1737,7 +1743,7 @@ cudaError_t TextDecoder::branch_pass(uint32_t per_seq, float temperature) {
   return e;
 }
 
-int TextDecoder::capture() {
+cudaError_t TextDecoder::record_graph() {
   cudaGraph_t g = nullptr;
   const int sm = (int)attn_smem_bytes(hd);
   cudaError_t e = hd == 64    ? cudaFuncSetAttribute(attn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm)
@@ -1763,7 +1769,11 @@ int TextDecoder::capture() {
   }
   if (e == cudaSuccess) e = cudaGraphInstantiate(&graph, g, 0);
   if (g) cudaGraphDestroy(g);
+  return e;
+}
 
+int TextDecoder::capture() {
+  const cudaError_t e = record_graph();
   if (e != cudaSuccess) {
     set_error_message(cudaGetErrorString(e));
     return EOS_E_INTERNAL;

@@ -1746,6 +1746,7 @@ uint64_t kv_attn_work_bound(const KvPool& kv, const KvAttnBatch& b, uint32_t n_h
 cudaError_t launch_kv_attn(const KvPool& kv, const KvAttnBatch& b, const float* q, uint64_t q_stride, float* out,
                            uint64_t out_stride, uint32_t n_head, float scale, void* scratch, int num_sms,
                            uint32_t* err, cudaStream_t st) {
+  if (kv.n_kv_head == 0 || n_head % kv.n_kv_head != 0) return cudaErrorNotSupported;  // whole groups of heads only
   if (b.n_rows == 0 || b.n_seq == 0) return cudaSuccess;
   const AttnSplit s = attn_split(kv, b, n_head);
   uint8_t* ws = static_cast<uint8_t*>(scratch);

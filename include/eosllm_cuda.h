@@ -416,8 +416,8 @@ EOSLLM_CUDA_API int eosi_cuda_text_set_prefill_resident(eosi_cuda_text_t *t, int
  * format), about a quarter of the memory and of the attention's reads; steps,
  * prefill and generation run as before, with every token attending to its
  * context as stored.  Only at position 0, without open branches
- * (EOS_E_INVALID_ARG otherwise); Q8 needs world == 1 and the PER_OP step
- * (EOS_E_UNSUPPORTED). */
+ * (EOS_E_INVALID_ARG otherwise); Q8 needs world == 1, the PER_OP step and
+ * n_head a multiple of n_kv_head (EOS_E_UNSUPPORTED). */
 #define EOSI_CUDA_CACHE_F32 0
 #define EOSI_CUDA_CACHE_Q8 1
 EOSLLM_CUDA_API int eosi_cuda_text_set_cache(eosi_cuda_text_t *t, int mode);

@@ -1,0 +1,21 @@
+"""The decoder's cache modes and branches where a call fails, or ends a range."""
+
+import numpy as np
+import pytest
+
+from oracle.llama import make_llama
+from test_gpu_text_cache import decoder, toks
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("heads,kv,width", [(4, 3, 256), (2, 4, 512)])
+def test_heads_that_kv_heads_do_not_divide_are_refused(gpu, oracle, heads, kv, width):
+    """The f32 cache maps any number of heads to the kv heads, the 8-bit cache
+    whole groups only."""
+    from eosllm_b200.text import TextDecoder
+    d = decoder(make_llama(oracle, max_ctx=16, n_embd=width, n_head=heads, n_kv_head=kv), q8=False)
+    with pytest.raises(gpu.CudaBackendError) as ex:
+        d.set_cache(TextDecoder.CACHE_Q8)
+    assert ex.value.status == gpu.EOS_E_UNSUPPORTED and "multiple of n_kv_head" in str(ex.value)
+    d.close()
