@@ -1590,6 +1590,21 @@ int TextDecoder::set_cache(int mode) {
     if (e == cudaSuccess) e = alloc(&vc, kv_bytes);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   }
+  // the step for the new cache; where that fails too, the old one's stays
+  const cudaGraphExec_t old_graph = graph;
+  const uint32_t old_kernels = step_kernels;
+  if (e == cudaSuccess) {
+    q8 = want;
+    graph = nullptr;
+    e = record_graph();
+    if (e == cudaSuccess) {
+      if (old_graph) cudaGraphExecDestroy(old_graph);
+    } else {
+      q8 = !want;
+      graph = old_graph;
+      step_kernels = old_kernels;
+    }
+  }
   // the cache no longer wanted, or the one that could not be set up
   if ((e == cudaSuccess) == want) {
     release(kc);
@@ -1601,20 +1616,14 @@ int TextDecoder::set_cache(int mode) {
     release(q8_attn);
     release(q8_scratch);
   }
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    set_error_message(cudaGetErrorString(e));
-    return e == cudaErrorMemoryAllocation ? EOS_E_OUT_OF_MEMORY : EOS_E_INTERNAL;
-  }
-  q8 = want;
-  if (graph) cudaGraphExecDestroy(graph);
-  graph = nullptr;
-  e = record_graph();
   if (e == cudaSuccess) return EOS_OK;
-  set_error_message(e == cudaErrorNotSupported
-                        ? "cuda text: the 8-bit cache does not serve this model (n_head must be a multiple of n_kv_head)"
-                        : cudaGetErrorString(e));
-  return e == cudaErrorNotSupported ? EOS_E_UNSUPPORTED : EOS_E_INTERNAL;
+  cudaGetLastError();
+  if (want && e == cudaErrorNotSupported) {
+    set_error_message("cuda text: the 8-bit cache does not serve this model (n_head must be a multiple of n_kv_head)");
+    return EOS_E_UNSUPPORTED;
+  }
+  set_error_message(cudaGetErrorString(e));
+  return e == cudaErrorMemoryAllocation ? EOS_E_OUT_OF_MEMORY : EOS_E_INTERNAL;
 }
 
 void TextDecoder::close_branches() {

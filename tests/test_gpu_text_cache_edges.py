@@ -19,3 +19,24 @@ def test_heads_that_kv_heads_do_not_divide_are_refused(gpu, oracle, heads, kv, w
         d.set_cache(TextDecoder.CACHE_Q8)
     assert ex.value.status == gpu.EOS_E_UNSUPPORTED and "multiple of n_kv_head" in str(ex.value)
     d.close()
+
+
+def test_a_cache_whose_step_cannot_be_recorded_changes_nothing(gpu, oracle):
+    """The failure comes when the new cache is there and the step is recorded for
+    it (three kv heads for four heads): the decoder keeps its cache, its step and
+    its results, however often it is asked."""
+    from eosllm_b200.text import TextDecoder
+    model = make_llama(oracle, max_ctx=16, n_kv_head=3)
+    d = decoder(model, q8=False)
+    first, kernels = [d.step(t) for t in (3, 7)], d.step_kernels
+    for _ in range(3):
+        d.reset()
+        with pytest.raises(gpu.CudaBackendError):
+            d.set_cache(TextDecoder.CACHE_Q8)
+        assert d.cache == TextDecoder.CACHE_F32 and d.step_kernels == kernels
+        for t, w in zip((3, 7), first):
+            assert np.array_equal(d.step(t), w)
+    d.reset()
+    d.set_cache(TextDecoder.CACHE_F32)  # the one it has
+    assert np.array_equal(d.step(3), first[0])
+    d.close()
