@@ -95,7 +95,9 @@ __global__ void __launch_bounds__(1024) logit_probs_kernel(float* x, uint32_t n,
 
 cudaError_t launch_logit_probs(float* logits, uint32_t rows, uint32_t n, float temperature, cudaStream_t st) {
   if (rows == 0) return cudaSuccess;
-  logit_probs_kernel<<<rows, 1024, 0, st>>>(logits, n, temperature > 0.0f ? 1.0f / temperature : 0.0f);
+  // (the reciprocal of a temperature below 2^-128 is no f32; at the largest one different logits are as far apart)
+  const float inv_t = temperature > 0.0f ? fminf(1.0f / temperature, 3.402823466e38f) : 0.0f;
+  logit_probs_kernel<<<rows, 1024, 0, st>>>(logits, n, inv_t);
   return cudaGetLastError();
 }
 

@@ -40,3 +40,19 @@ def test_a_cache_whose_step_cannot_be_recorded_changes_nothing(gpu, oracle):
     d.set_cache(TextDecoder.CACHE_F32)  # the one it has
     assert np.array_equal(d.step(3), first[0])
     d.close()
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-42, 2.9e-39, 1e-38, 1e-30])
+def test_the_smallest_temperatures_draw_the_most_likely_token(gpu, oracle, temperature):
+    """A positive temperature whose reciprocal no f32 holds is a temperature like
+    the others: as it goes to 0 the largest logit takes all."""
+    model = make_llama(oracle, max_ctx=64)
+    d = decoder(model)
+    d.prefill(toks(17, 320, 1))
+    d.fork(2, 8)
+    a = d.branch_step([[5], [9]], [[0.3], [0.999]], temperature=0.0)
+    d.close_branches()
+    d.fork(2, 8)
+    b = d.branch_step([[5], [9]], [[0.3], [0.999]], temperature=temperature)
+    assert [list(x) for x in a] == [list(x) for x in b]
+    d.close()
