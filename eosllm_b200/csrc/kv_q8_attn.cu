@@ -1450,6 +1450,10 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
   const uint32_t RT = p.rt;
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t x = (uint64_t)blockIdx.x * 2u + (threadIdx.x >> 5);
+  // lengths and rows beyond their bounds, where no kernel before this one has looked at the sequences
+  if (x == 0 && p.max_len == 0 && (p.max_prefix == 0 || p.prefix_few > 0))
+    for (uint32_t i = lane; i < p.rows.n_seq; i += 32u)
+      if (p.seq_len[i] > p.max_len || attn_seq(p, i).n > p.max_rows) report(p.err, EOS_DEVERR_RANGE);
   if (x >= (uint64_t)p.rows.n_rows * p.n_head) return;  // warp-uniform
   const uint32_t hw = attn_div((uint32_t)x, p.by_group);  // row * n_kv_head + kv head
   const uint32_t r = attn_div(hw, p.by_kv_head), g = hw - r * p.n_kv_head, hh = (uint32_t)x - hw * p.group;
@@ -1469,7 +1473,7 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
     --i;
   }
   const uint32_t t = r - kv_row_start(p.rows, i);
-  if (t >= p.max_rows) return;  // reported by the attention kernel
+  if (t >= p.max_rows) return;  // (reported)
   const uint32_t seq_len = p.seq_len[i];
   pdl_wait();
   // ids of the row's partials: [first, last] of the prefix and of its sequence

@@ -52,3 +52,29 @@ def test_later_tokens_leave_earlier_rows_as_they_are(gpu, hd, n, length, prefix)
             again = b.out.cpu().numpy()[:n]
             assert np.array_equal(again[:t + 1].view(np.uint32), got[:t + 1].view(np.uint32)), t
             b.c.write(b.ks[0], b.vs[0], [length], [0], first=1)
+
+
+@pytest.mark.parametrize("n,prefix", [(1, 100), (3, 0), (3, 100), (40, 100)])
+def test_lengths_are_reported_without_own_tokens(gpu, n, prefix):
+    """max_len = 0: a sequence length above it is left out and reported, and so
+    are rows beyond max_rows, whether or not there is a prefix."""
+    b = Batch(gpu, 2, 2, 64, prefix, [1] * n, [1] * n, seed=n)
+
+    def call(max_rows, row0):
+        b.row0.copy_(b.c.i32(row0))
+        b.batch = gpu.attn_batch(prefix_table=b.ptab, prefix_len=b.plen, max_prefix=prefix, table=b.tab,
+                                 table_stride=b.c.width, seq_len=b.len_d, max_len=0, row0=b.row0, n_seq=n, n_rows=n,
+                                 max_rows=max_rows)
+        b.scratch = b.c.torch.empty(max(16, gpu.kv_q8_attn_scratch_bytes(b.c.pool, b.batch, 2)),
+                                    dtype=b.c.torch.uint8, device="cuda")
+        b.run()
+        return gpu.take_device_errors()
+
+    every = list(range(n + 1))
+    b.len_d.zero_()
+    assert call(1, every) == 0
+    b.len_d[n - 1] = 1
+    assert call(1, every) == 1 << 5
+    b.len_d.zero_()
+    if n > 1:  # the first sequence has two rows where one is the most, the second none
+        assert call(1, [0, 2] + every[2:]) == 1 << 5
