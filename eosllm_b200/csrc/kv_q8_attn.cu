@@ -735,11 +735,12 @@ __global__ void __launch_bounds__(kFewThreads, HD <= 128u ? 4 : (R == 1u ? 3 : 2
         }
       if (tid >= HD) continue;
       if (direct) {
-        const float inv = ls == 0.0f ? 0.0f : __fdiv_rn(1.0f, ls);
         const uint32_t xr = attn_div(r, p.by_group);
+        const bool none = seen0 + (int32_t)xr <= 0;  // 0, also for a query that is not finite
+        const float inv = ls == 0.0f ? 0.0f : __fdiv_rn(1.0f, ls);
         float* dst = p.out + (size_t)(s.r0 + xr) * p.out_stride + (size_t)(g * p.group + r - xr * p.group) * HD;
 #pragma unroll
-        for (uint32_t d = 0; d < DT; ++d) dst[d * 128u + tid] = acc[d] * inv;
+        for (uint32_t d = 0; d < DT; ++d) dst[d * 128u + tid] = none ? 0.0f : acc[d] * inv;
       } else {
 #pragma unroll
         for (uint32_t d = 0; d < DT; ++d) po[(size_t)r * HD + d * 128u + tid] = acc[d];
@@ -1472,9 +1473,12 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
     if (i == 0 || i > p.rows.n_seq) return;  // before the first sequence or behind the last
     --i;
   }
-  const uint32_t t = r - kv_row_start(p.rows, i);
+  const uint32_t start = kv_row_start(p.rows, i), t = r - start, n_seq_rows = kv_row_start(p.rows, i + 1u) - start;
   if (t >= p.max_rows) return;  // (reported)
   const uint32_t seq_len = p.seq_len[i];
+  // no token: 0, also for a query that is not finite
+  const bool none = (int32_t)min(seq_len, p.max_len) - (int32_t)n_seq_rows + (int32_t)t + 1 <= 0 &&
+                    (p.max_prefix == 0 || *p.prefix_len == 0);
   pdl_wait();
   // ids of the row's partials: [first, last] of the prefix and of its sequence
   struct Part {
@@ -1573,7 +1577,7 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
   float* dst = p.out + (size_t)r * p.out_stride + (size_t)h * HD + lane * E;
 #pragma unroll
-  for (uint32_t e = 0; e < E; ++e) dst[e] = acc[e] * inv;
+  for (uint32_t e = 0; e < E; ++e) dst[e] = none ? 0.0f : acc[e] * inv;
 }
 
 namespace {

@@ -285,7 +285,8 @@ EOSLLM_CUDA_API int eosi_cuda_kv_q8_read_dev(const eosi_cuda_kv_q8_t *kv, float 
  * the page's largest), products and sums of both with the int8 cache are exact
  * integers, and the softmax statistics are f32.  Results do not depend on
  * timing.  A query row or a visible cache row
- * that holds a NaN or an infinity gives a row of NaN.
+ * that holds a NaN or an infinity gives a row of NaN (a row that sees no token
+ * is 0 all the same).
  * scratch: eosi_cuda_kv_q8_attn_scratch_bytes(kv, batch, n_head) bytes, 16-byte
  * aligned, not shared by calls that may overlap. */
 #define EOSI_CUDA_ATTN_MAX_SEQ 1024

@@ -78,3 +78,18 @@ def test_lengths_are_reported_without_own_tokens(gpu, n, prefix):
     b.len_d.zero_()
     if n > 1:  # the first sequence has two rows where one is the most, the second none
         assert call(1, [0, 2] + every[2:]) == 1 << 5
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("H,n,length,prefix", [(2, 3, 1, 0), (2, 3, 0, 0), (4, 9, 4, 0), (4, 9, 0, 0), (2, 40, 30, 0)])
+def test_rows_that_see_nothing_are_zero_whatever_their_query(gpu, bad, H, n, length, prefix):
+    """Rows 0 .. n - length - 1 see no token: 0, also where the query holds a NaN
+    or an infinity and the sequence has tokens for later rows; a row that sees
+    one is NaN."""
+    def edit(b):
+        b.q[:, :, 5] = bad
+    b = Batch(gpu, H, 2, 64, prefix, [length, 3], [n, 1], seed=n, edit=edit)
+    b.run()
+    got = b.out.cpu().numpy()[:n + 1]
+    assert np.all(got[:n - length] == 0) and np.all(np.isnan(got[n - length:]))
+    assert gpu.take_device_errors() == 0
