@@ -25,7 +25,7 @@ __device__ __forceinline__ uint8_t* kv_locate(const KvCopyParams& p, uint32_t r,
                                               uint32_t& slot) {
   uint32_t r0, r1, pos;
   const uint32_t i = kv_find(p.rows, p.pos, [&](uint32_t, uint32_t start) { return start <= r; }, r0, r1, pos);
-  if (i >= p.rows.n_seq || r >= r1) return nullptr;
+  if (i >= p.rows.n_seq || r < r0 || r >= r1) return nullptr;
   const uint64_t at = (uint64_t)pos + (r - r0);
   if (at >= (uint64_t)p.table_stride * kKvPage) {
     report(p.err, EOS_DEVERR_RANGE);

@@ -902,30 +902,32 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
 
   if (warp == G::kWarps) {
     // ---- the line's layout: prefix units, then the sequences' (running work in cum) ----
-    uint32_t carry = 0;
     AttnPlan pl;
     pl.mine = first;
-    for (uint32_t i0 = 0; i0 < p.rows.n_seq; i0 += 32u) {
-      uint32_t w = 0;
-      const bool in = i0 + lane < p.rows.n_seq;
-      if (in && p.seq_few == 0) w = attn_seq_work<RT>(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
-      uint32_t c = w;
-#pragma unroll
-      for (uint32_t o = 1; o < 32u; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, c, o);
-        if (lane >= o) c += t;
-      }
-      if (in) cum[i0 + lane] = carry + c - w;
-      carry += __shfl_sync(0xffffffffu, c, 31);
-    }
-    if (lane == 0) cum[p.rows.n_seq] = carry;
-    __syncwarp();
     pl.prefix = prefix_len < p.max_prefix ? prefix_len : p.max_prefix;
     if (p.prefix_few > 0) pl.prefix = 0;
     pl.rows_p = rows_end;
     pl.tp = attn_ceil(pl.prefix, kKvPage);
     pl.rgp = attn_ceil(pl.rows_p * p.group, RT);
     pl.wp = p.n_kv_head * pl.rgp * attn_cost(pl.tp);
+    // (sequences that share rows -- a row0 that goes down -- could add up to more than the host's bound: the line ends there)
+    const uint32_t most = 0x7fffffffu - pl.wp;
+    uint32_t carry = 0;
+    for (uint32_t i0 = 0; i0 < p.rows.n_seq; i0 += 32u) {
+      uint32_t c = 0;
+      const bool in = i0 + lane < p.rows.n_seq;
+      if (in && p.seq_few == 0) c = attn_seq_work<RT>(p, i0 == 0 ? first : attn_seq(p, i0 + lane));
+#pragma unroll
+      for (uint32_t o = 1; o < 32u; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c = min(c + t, most);
+      }
+      const uint32_t before = __shfl_up_sync(0xffffffffu, c, 1);
+      if (in) cum[i0 + lane] = min(carry + (lane > 0 ? before : 0u), most);
+      carry = min(carry + __shfl_sync(0xffffffffu, c, 31), most);
+    }
+    if (lane == 0) cum[p.rows.n_seq] = carry;
+    __syncwarp();
     const uint32_t total = pl.wp + carry;
     pl.quantum = attn_ceil(total, gridDim.x);
     const uint64_t w_lo = (uint64_t)blockIdx.x * pl.quantum;
@@ -1473,11 +1475,12 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
     if (i == 0 || i > p.rows.n_seq) return;  // before the first sequence or behind the last
     --i;
   }
-  const uint32_t start = kv_row_start(p.rows, i), t = r - start, n_seq_rows = kv_row_start(p.rows, i + 1u) - start;
-  if (t >= p.max_rows) return;  // (reported)
+  const uint32_t start = kv_row_start(p.rows, i), end = kv_row_start(p.rows, i + 1u), t = r - start;
+  if (r < start || r >= end) return;  // (a row0 that goes down)
+  if (t >= p.max_rows) return;        // (reported)
   const uint32_t seq_len = p.seq_len[i];
   // no token: 0, also for a query that is not finite
-  const bool none = (int32_t)min(seq_len, p.max_len) - (int32_t)n_seq_rows + (int32_t)t + 1 <= 0 &&
+  const bool none = (int32_t)min(seq_len, p.max_len) - (int32_t)(end - r) + 1 <= 0 &&
                     (p.max_prefix == 0 || *p.prefix_len == 0);
   pdl_wait();
   // ids of the row's partials: [first, last] of the prefix and of its sequence
@@ -1489,8 +1492,10 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
   auto line = [&](Part& a, const float* o, const float* ml, uint32_t cap, uint32_t unit, uint32_t w, uint32_t tiles,
                   uint32_t row) {
     if (tiles == 0) return;
-    const uint32_t quantum = __ldcg(p.plan);
-    const uint32_t c0 = (w + kAttnStart) / quantum, c1 = (w + kAttnStart + tiles - 1u) / quantum;
+    const uint32_t quantum = max(__ldcg(p.plan), 1u);
+    const uint32_t c0 = min((w + kAttnStart) / quantum, kAttnMaxCtas - 1u),
+                   c1 = min((w + kAttnStart + tiles - 1u) / quantum, kAttnMaxCtas - 1u);
+    if (c1 < c0) return;
     a.n = 2u * (c1 - c0 + 1u);
     a.o_step = cap * HD;
     a.ml_step = cap * kAttnMl;

@@ -251,8 +251,8 @@ EOSLLM_CUDA_API size_t eosi_cuda_kv_q8_page_bytes(uint32_t n_kv_head, uint32_t h
 /* Quantises rows into the cache (write), or the cache's rows as f32 (read):
  * row r, head h at k / v + r * row_stride + h * head_dim floats (16-byte
  * aligned, row_stride a multiple of 4 and at least n_kv_head * head_dim).
- * Sequence i owns rows [row0[i], row0[i + 1]) (row0: n_seq + 1 words; NULL:
- * n_rows / n_seq each), which sit at positions pos[i], pos[i] + 1, ... ;
+ * Sequence i owns rows [row0[i], row0[i + 1]) (row0: n_seq + 1 ascending words;
+ * NULL: n_rows / n_seq each), which sit at positions pos[i], pos[i] + 1, ... ;
  * position j of sequence i lives in page table[i * table_stride + j / 128].
  * Rows behind the last sequence, and every token not written, stay as they
  * were.  Sequences of one call write distinct pages, and calls that write to

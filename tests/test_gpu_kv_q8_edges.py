@@ -93,3 +93,28 @@ def test_rows_that_see_nothing_are_zero_whatever_their_query(gpu, bad, H, n, len
     got = b.out.cpu().numpy()[:n + 1]
     assert np.all(got[:n - length] == 0) and np.all(np.isnan(got[n - length:]))
     assert gpu.take_device_errors() == 0
+
+
+@pytest.mark.parametrize("hd,max_rows", [(64, 9), (128, 40)])
+@pytest.mark.parametrize("row0", [[0, 9, 2, 9, 0], [9, 0, 1, 2, 3], [40, 40, 0, 40, 40], [0, 40, 0, 40, 0],
+                                  [0, 0xFFFFFFFF, 5, 0xFFFFFFFF, 40]])
+def test_row0_that_is_not_ascending(gpu, hd, max_rows, row0):
+    """Row starts that go down or beyond n_rows: which rows are computed is not
+    defined, but nothing outside the batch is touched and the next call is right."""
+    n = 40
+    b = Batch(gpu, 4, 2, hd, 140, [130, 1, 300, 7], [10] * 4, seed=hd)
+    good_batch, good_row0, good_scratch = b.batch, b.row0, b.scratch
+    b.row0 = b.c.i32(row0)
+    b.batch = gpu.attn_batch(prefix_table=b.ptab, prefix_len=b.plen, max_prefix=140, table=b.tab,
+                             table_stride=b.c.width, seq_len=b.len_d, max_len=300, row0=b.row0, n_seq=4, n_rows=n,
+                             max_rows=max_rows)
+    b.scratch = b.c.torch.empty(gpu.kv_q8_attn_scratch_bytes(b.c.pool, b.batch, 4), dtype=b.c.torch.uint8, device="cuda")
+    b.run()
+    b.c.torch.cuda.synchronize()
+    assert np.all(b.out.cpu().numpy()[n:] == 3.0)
+    k = b.c.torch.full((n + 2, 2, hd), 5.0, device="cuda")
+    gpu.kv_q8_read_dev(b.c.pool, k, k.clone(), 2 * hd, n, b.row0, b.tab, b.c.width, b.c.i32([0] * 4), 4)
+    assert bool((k[n:] == 5.0).all())
+    gpu.take_device_errors()
+    b.batch, b.row0, b.scratch = good_batch, good_row0, good_scratch
+    b.check()
