@@ -383,8 +383,9 @@ __device__ __forceinline__ AttnQScale attn_query_scale(uint32_t amax, float scal
   s.finite = amax < 0x7f800000u;
   const float top = fmaxf(__uint_as_float(amax), 1e-30f);
   s.inv = s.finite ? __fdiv_rn(scale_log2 < 0.0f ? -kAttnQMax : kAttnQMax, top) : 0.0f;
-  // (above 0, so that a hidden token's -infinity stays one when the softmax scale is 0)
-  s.scale = s.finite ? fmaxf(__fdiv_rn(top, kAttnQMax) * (256.0f * fabsf(scale_log2)), 1e-37f) : NAN;
+  // (above 0, so that a hidden token's -infinity stays one when the softmax scale is 0; finite: a scale that large
+  // parts any two scores all the same)
+  s.scale = s.finite ? fminf(fmaxf(__fdiv_rn(top, kAttnQMax) * (256.0f * fabsf(scale_log2)), 1e-37f), 3e38f) : NAN;
   return s;
 }
 // Three balanced digits of four elements: bytes of (x + 0x808080) ^ 0x808080.
@@ -1152,7 +1153,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
             }
             amax = __reduce_max_sync(0xffffffffu, amax);
             const AttnQScale q = attn_query_scale(amax, p.scale_log2);
-            // (times 2^17 of the scores' 2^22; a scale that large parts any two scores all the same)
+            // (times 2^17 of the scores' 2^22)
             scale = q.finite ? fminf(q.scale * 131072.0f, 3e38f) : NAN;
 #pragma unroll
             for (uint32_t pn = 0; pn < G::kPanels; ++pn) {

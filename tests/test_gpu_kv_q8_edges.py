@@ -118,3 +118,16 @@ def test_row0_that_is_not_ascending(gpu, hd, max_rows, row0):
     gpu.take_device_errors()
     b.batch, b.row0, b.scratch = good_batch, good_row0, good_scratch
     b.check()
+
+
+@pytest.mark.parametrize("count", [1, 2, 6, 20])
+@pytest.mark.parametrize("q_gain,k_gain,scale", [(4e37, 1e-38, 1e6), (1e37, 1e-36, -1e4), (1e-28, 1e28, 2.0), (3e37, 1e-30, 1e-7)])
+def test_factors_at_the_ends_of_the_range(gpu, count, q_gain, k_gain, scale):
+    """Scores of ordinary size or far apart, from a query, a key and a scale whose
+    products in another order leave the f32 range."""
+    def edit(b):
+        b.q *= np.float32(q_gain)
+        for x in [b.kp] + b.ks:
+            x *= np.float32(k_gain)
+        b.scale = scale
+    Batch(gpu, 4, 2, 64, 150, [40], [count], seed=count, edit=edit).check()
