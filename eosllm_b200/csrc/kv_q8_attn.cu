@@ -967,7 +967,7 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         if (live) {
           const int32_t t0 = (int32_t)(s.tile0 * kKvPage);
           bar.job[nj & 1u] = AttnJob{s.tiles, s.rows, s.row0, s.unit, is_prefix ? 1u : 0u, s.len - (uint32_t)t0,
-                                     is_prefix ? 0x3fffffff : (int32_t)s.len - (int32_t)s.n + 1 - t0};
+                                     is_prefix ? 0x40000000 : (int32_t)s.len - (int32_t)s.n + 1 - t0};
           if (more) mbar_arrive_expect_tx(&bar.full[x % S], s.rows * HD * 4u);
           else mbar_arrive(&bar.full[x % S]);
         }
