@@ -1301,6 +1301,24 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           mbar_arrive(&bar.s_free[half]);
           mbar_arrive(&bar.xmax[half][grp]);
         }
+        uint32_t tail[NC][2] = {};  // a cut tile: the largest value scale from `least` on that a column sees
+        if constexpr (CAUSAL)
+          if (cut) {  // lane l: the largest scale of the tokens from `least` to l behind it (a group's rows are at most 32)
+            const uint32_t tok = (uint32_t)least + lane;
+            uint32_t v = 0;
+            if ((int32_t)tok < some) v = *reinterpret_cast<const uint32_t*>(sc + (tok >> 5) * 256u + 128u + (tok & 31u) * 4u);
+            if (v >= 0x7f800000u) v = 0u;
+#pragma unroll
+            for (uint32_t o = 1; o < 32u; o <<= 1) v = max(v, __shfl_up_sync(0xffffffffu, v, o));
+#pragma unroll
+            for (uint32_t y = 0; y < NC; ++y)
+#pragma unroll
+              for (uint32_t z = 0; z < 2u; ++z) {
+                const int32_t n = limit(c0 + 8u * y + 2u * cq + z) - (int32_t)tok0 - least;
+                const uint32_t w = __shfl_sync(0xffffffffu, v, min(max(n - 1, 0), 31));
+                tail[y][z] = n > 0 ? w : 0u;
+              }
+          }
         if (t > half) live = fold_tile();
         if (live) live = __all_sync(0xffffffffu, attn_wait(&bar.xmax[half][grp], it & 1u)) != 0;
         if (!live) break;
@@ -1316,25 +1334,10 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) vw[j] = __shfl_sync(0xffffffffu, v1, g + 8u * j);
 #pragma unroll
-          for (uint32_t y = 0; y < NC; ++y) top[y][0] = top[y][1] = all;
+          for (uint32_t y = 0; y < NC; ++y)
+#pragma unroll
+            for (uint32_t z = 0; z < 2u; ++z) top[y][z] = CAUSAL ? max(tail[y][z] >> 23, all) : all;
         }
-        if constexpr (CAUSAL)
-          if (cut) {  // lane l: the largest scale of the tokens from `least` to l behind it (a group's rows are at most 32)
-            const uint32_t tok = (uint32_t)least + lane;
-            uint32_t v = 0;
-            if ((int32_t)tok < some) v = *reinterpret_cast<const uint32_t*>(sc + (tok >> 5) * 256u + 128u + (tok & 31u) * 4u);
-            if (v >= 0x7f800000u) v = 0u;
-#pragma unroll
-            for (uint32_t o = 1; o < 32u; o <<= 1) v = max(v, __shfl_up_sync(0xffffffffu, v, o));
-#pragma unroll
-            for (uint32_t y = 0; y < NC; ++y)
-#pragma unroll
-              for (uint32_t z = 0; z < 2u; ++z) {
-                const int32_t n = limit(c0 + 8u * y + 2u * cq + z) - (int32_t)tok0 - least;
-                const uint32_t w = __shfl_sync(0xffffffffu, v, min(max(n - 1, 0), 31));
-                if (n > 0) top[y][z] = max(top[y][z], w >> 23);
-              }
-          }
         uint8_t* pop = stages + st * G::kBlock;  // the probabilities take the place of the keys
 #pragma unroll
         for (uint32_t y = 0; y < NC; ++y) {
@@ -1448,35 +1451,42 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
 // Joins a row's partials: one warp per (row, head), lane l holding HD / 32
 // neighbouring elements.  Weights are relative to the largest maximum; the
 // order of the sums is the line's, so results do not depend on timing.
-template <uint32_t HD>
+template <uint32_t HD, bool LOOK>
 __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) {
   constexpr uint32_t E = HD / 32u;
   const uint32_t RT = p.rt;
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t x = (uint64_t)blockIdx.x * 2u + (threadIdx.x >> 5);
-  // lengths and rows beyond their bounds, where no kernel before this one has looked at the sequences
-  if (x == 0 && p.max_len == 0 && (p.max_prefix == 0 || p.prefix_few > 0))
-    for (uint32_t i = lane; i < p.rows.n_seq; i += 32u)
-      if (p.seq_len[i] > p.max_len || attn_seq(p, i).n > p.max_rows) report(p.err, EOS_DEVERR_RANGE);
+  if constexpr (LOOK)  // lengths and rows beyond their bounds, where no kernel before this one has looked at them
+    if (x == 0)
+      for (uint32_t i = lane; i < p.rows.n_seq; i += 32u)
+        if (p.seq_len[i] > p.max_len || attn_seq(p, i).n > p.max_rows) report(p.err, EOS_DEVERR_RANGE);
   if (x >= (uint64_t)p.rows.n_rows * p.n_head) return;  // warp-uniform
   const uint32_t hw = attn_div((uint32_t)x, p.by_group);  // row * n_kv_head + kv head
   const uint32_t r = attn_div(hw, p.by_kv_head), g = hw - r * p.n_kv_head, hh = (uint32_t)x - hw * p.group;
   const uint32_t h = g * p.group + hh;
   // the row's sequence and the inputs' words: read while the attention still runs
-  uint32_t i = 0;
+  uint32_t i = 0, start, end;
   if (p.rows.row0 == nullptr) {
     i = r / p.rows.per_seq;
+    start = kv_row_start(p.rows, i);
+    end = kv_row_start(p.rows, i + 1u);
   } else {  // sequences that start at or before the row, 32 at a time
-    uint32_t n = 0;
+    uint32_t n = 0, c, first = 0, last = 0;
     for (;; n += 32u) {
-      const uint32_t c = __popc(__ballot_sync(0xffffffffu, n + lane <= p.rows.n_seq && kv_row_start(p.rows, n + lane) <= r));
-      i = n + c;
+      const bool in = n + lane <= p.rows.n_seq;
+      first = in ? kv_row_start(p.rows, n + lane) : 0u;
+      c = __popc(__ballot_sync(0xffffffffu, in && first <= r));
       if (c < 32u) break;
+      last = __shfl_sync(0xffffffffu, first, 31);
     }
+    i = n + c;
     if (i == 0 || i > p.rows.n_seq) return;  // before the first sequence or behind the last
     --i;
+    start = c > 0 ? __shfl_sync(0xffffffffu, first, c - 1u) : last;
+    end = __shfl_sync(0xffffffffu, first, c);
   }
-  const uint32_t start = kv_row_start(p.rows, i), end = kv_row_start(p.rows, i + 1u), t = r - start;
+  const uint32_t t = r - start;
   if (r < start || r >= end) return;  // (a row0 that goes down)
   if (t >= p.max_rows) return;        // (reported)
   const uint32_t seq_len = p.seq_len[i];
@@ -1532,7 +1542,7 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
     }
   }
   // partial k of the row; lane k looks after its weight
-  const uint32_t n = part[0].n + part[1].n;
+  const uint32_t n = none ? 0u : part[0].n + part[1].n;
   auto ml_of = [&](uint32_t k) {
     return k < part[0].n ? part[0].ml + (size_t)k * part[0].ml_step
                          : part[1].ml + (size_t)(k - part[0].n) * part[1].ml_step;
@@ -1583,7 +1593,7 @@ __global__ void __launch_bounds__(64) kv_attn_join_kernel(const KvAttnParams p) 
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
   float* dst = p.out + (size_t)r * p.out_stride + (size_t)h * HD + lane * E;
 #pragma unroll
-  for (uint32_t e = 0; e < E; ++e) dst[e] = none ? 0.0f : acc[e] * inv;
+  for (uint32_t e = 0; e < E; ++e) dst[e] = acc[e] * inv;
 }
 
 namespace {
@@ -1737,7 +1747,8 @@ cudaError_t attn_launch(const KvAttnParams& p, bool line, int num_sms, uint64_t 
   at[0].val.programmaticStreamSerializationAllowed = first ? 0 : 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<HD>, p);
+  return p.seq_few == 0 && !line ? cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<HD, true>, p)
+                                 : cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<HD, false>, p);
 }
 
 }  // namespace
