@@ -39,6 +39,9 @@ enum : uint32_t {
   EOS_DEVERR_RANGE = 1u << 5,       // a page, position or length out of its range was left out
 };
 
+// SMs of a B200, for what is sized on the host before a device is known (scratch) or is a matter of taste (CTAs per unit).
+constexpr uint32_t kSms = 148;
+
 // One second: the bound on every spin-wait in this library's kernels.
 constexpr uint64_t EOS_WAIT_LIMIT_NS = 1000000000ull;
 

@@ -118,11 +118,12 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvCopyParams p) {
 // collide four ways at most) and value rows move as 16 bytes a thread.  Every
 // byte moves once; reading and writing f32 rows is what bounds it.  The heads of
 // the same rows are neighbours in the grid, so that what runs together is
-// together in memory (reading 16383 rows x 32 heads: 117 us head by head, 107
-// so, 6.3 TB/s).  A write's registers are held to 64 a thread, four CTAs an SM:
-// at three, 8505 rows x 8 heads took 21.4 us, at four 19.5 (4.5 TB/s; loads,
-// rounding and stores of a CTA follow one another); keys and values in CTAs of
-// their own 24.3.
+// together in memory (reading 16383 rows x 32 heads: 117 us head by head, 107 to
+// 110 so, 6.2 TB/s).  A write's registers are held to 64 a thread, four CTAs an SM:
+// at three, 8505 rows x 8 heads took 21.4 us, at four 19.9, keys and values in CTAs
+// of their own 24.3 (the same rows each time; other rows each time 20.9, 4.2 TB/s:
+// a CTA's loads, rounding and stores follow one another, and nothing of the next
+// quarter is under way meanwhile).
 //
 // Quarters of a ragged batch: sequence i's blocks start at row0[i] / 32 + 2 i,
 // which leaves room for the two broken ends; a CTA searches its sequence, and the
@@ -290,8 +291,8 @@ KvCopyParams copy_params(const KvPool& kv, const KvRowSet& rs, const float* k, c
 
 // Rows or quarters: a quarter's CTA pays off from about eight rows of a sequence
 // on (its launch covers up to two broken quarters per sequence).  Writing and
-// reading 64 sequences of 8 heads, row by row and by quarters: two rows each 6.9
-// and 12.5 us, four 9.6 and 13.0, eight 13.9 and 13.7.
+// reading 64 sequences of 8 heads, row by row and by quarters: two rows each 7.0
+// and 12.7 us, four 9.4 and 12.4, eight 14.0 and 13.5, sixteen 23.6 and 14.6.
 template <bool READ>
 cudaError_t copy_launch(const KvPool& kv, const KvCopyParams& p, cudaStream_t st) {
   const KvRows& r = p.rows;

@@ -17,10 +17,16 @@
 // Arithmetic.  Keys and values stay the integers they are in the cache: a
 // query row is scaled to integers of 24 bits and split into three signed
 // 8-bit digits, a tile's probabilities (times the value scales) become integers
-// of 23 bits, relative to the tile's own maximum, in three unsigned digits, and
-// every product has exact s32 sums -- no conversion of the cache, no 16-bit
-// rounding anywhere.  A probability p times weight w becomes an integer as the
-// mantissa of the float 2^23 + p w, whose three low bytes are the digits.
+// of 23 bits in three unsigned digits, and every product has exact s32 sums -- no
+// conversion of the cache, no 16-bit rounding anywhere.  A probability p times
+// weight w becomes an integer as the mantissa of the float 2^23 + p w, whose three
+// low bytes are the digits.  Both integers are fixed-point: a query element is
+// held to 2^-24 of its row's largest, a probability times a value scale to 2^-23
+// (few rows: 2^-31) of the largest value scale that the row sees in the page times
+// the page's largest probability.  So a query element, or a value row, far below
+// its neighbours loses low bits (beside a visible value row 1e2 times larger, of
+// whatever probability, an output is 1e-4 of its size off); with rows of like size
+// the errors are those of 32-bit arithmetic.  What a row does not see takes no part.
 //
 // Scores are compared before the row's query scale c (which holds the softmax
 // scale) is applied: z = sum * key scale, exponent (z - max z) c plus the exact
@@ -43,10 +49,12 @@
 // heads over 65537 tokens of 8 heads: 245 us, memory alone 27; issue slots 55 %
 // taken, the rest waits on the chain score - maximum - exponent); for few rows
 // over a long prefix the page copies do (8 rows over 16384 tokens of 32 heads:
-// 49 us, memory alone 21), and for small calls the chain launch - lengths -
+// 48 us, memory alone 21), and for small calls the chain launch - lengths -
 // table - page.  Widening the cache to f16 and multiplying hi and lo halves needs
-// no joining, but the widening and splitting cost as much (340 us and 112 us for
-// these two, when digits took 346 and 54).
+// no joining: as first built it took 340 and 112 us for these two, the digits then
+// 346 and 54.  Most of what has sped the digits up since (sixteen softmax warps,
+// maxima by halving, wider accumulator loads) would serve it too; it was not taken
+// up again.
 //
 // A CTA: eight warps for every 16 rows score and fold -- half of them on the even
 // tiles of a piece, half on the odd ones, so that one half's chain of waits is
@@ -410,15 +418,17 @@ __device__ __forceinline__ float attn_warp_max(float x) {
 // its CTAs' sums through shared memory, so a unit on one cluster is done with
 // one launch.  Reading the cache is what bounds it: 2 HD + 8 bytes per token
 // against 7 HD / 4 dp4a per token and row, so a few rows stay near the
-// memory's time (one row over 16000 tokens of 32 heads: 27.5 us, 4.9 TB/s).  No barrier or tensor memory to set up and several CTAs per
-// SM, each with a page's loads in flight: units of a page or two (a
-// sequence's own tokens, a decode step) take one round trip to memory.
+// memory's time (one row over 16000 tokens of 32 heads: 26.2 us, 5.2 TB/s).  No
+// barrier or tensor memory to set up and several CTAs per SM (four at 128
+// dimensions, by launch bounds), each with a page's loads in flight: units of a
+// page or two (a sequence's own tokens, a decode step) take one round trip to
+// memory.
 // Queries as in the tensor-core kernel, probabilities with 8 bits more; s32 sums
 // over 16 dimensions (scores) and over a page (values) are exact.
-// Measured both ways: 8 rows over 16384 tokens of 32 heads 138 us here, 49 on the
-// tensor cores; four rows over 640 tokens of 8 heads 7.5 here, 11.4 there; 128
-// units of four rows over 300 tokens 10.7 and 13.2; 384 of up to 700 tokens beside
-// a prefix of 65537 239 and 233 in all.
+// Measured both ways: 8 rows over 16384 tokens of 32 heads 131 us here, 48 on the
+// tensor cores; four rows over 640 tokens of 8 heads 7.5 here, 10.4 there; 128
+// units of four rows over 300 tokens 10.7 and 13.5; 384 of up to 700 tokens beside
+// a prefix of 65537 246 and 247 in all; one row over 16000 tokens 26.1 and 37.0.
 constexpr uint32_t kFewRows = 4;
 constexpr uint32_t kFewThreads = 128;
 
@@ -795,9 +805,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // Row groups of 16 (three digits each: N = 48), two CTAs per SM, for few rows: the
 // page copies of four tiles in flight hide each other's latency.  Groups of 32,
 // one CTA per SM, read a page half as often and share a tile's fixed work: 40
-// rows over 65536 tokens of 8 heads 101 -> 95 us, 20 over 16384 of 32 74 -> 60;
-// with 16 rows half its columns would be empty.  Their sixteen warps (two for the
-// same 32 tokens, 16 rows each) took 293 us where eight with 32 rows each took 312.
+// rows over 65536 tokens of 8 heads 99 -> 95 us, 20 over 16384 of 32 74 -> 59, a
+// prompt of 511 tokens 80 -> 69; with 16 rows half its columns would be empty.
+// Their sixteen warps (two for the same 32 tokens, 16 rows each) took 293 us where
+// eight with 32 rows each took 312 (48 rows over 65537 tokens, at the time).
 // (Two CTAs of 32 do not fit the registers; 64 dimensions leave no room for 96
 // rows of probabilities, 256 none for the value sums.)
 template <uint32_t HD, uint32_t RT>
@@ -838,8 +849,8 @@ struct AttnBars {
 
 // CAUSAL: some unit's columns see different numbers of tokens (several rows of a sequence).  Without it the columns of
 // a tile share one unit of the probabilities; a unit of their own costs them a product per pair of probabilities (seven
-// sequences of up to 6 rows over 1537 tokens of 32 heads 27.0 us, 26.0 with a shared unit, which let the value rows
-// behind a row's last token coarsen its weights).
+// sequences of up to 6 rows over 1537 tokens of 32 heads 26.5 us, 26.1 with a shared unit, a prompt of 511 tokens 68.8
+// and 64.7; but a shared one let the value rows behind a row's last token coarsen its weights).
 template <uint32_t HD, uint32_t RT, bool CAUSAL>
 __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>::kCtas)) kv_attn_kernel(const KvAttnParams p) {
   using G = AttnGeo<HD, RT>;
@@ -1613,10 +1624,10 @@ struct AttnSplit {
 // one, which needs no joining kernel, unless the units leave SMs idle (below
 // about four CTAs each) and a CTA would still have four pages to read.
 void attn_clusters(uint64_t units, uint32_t pages, uint32_t& clusters, uint32_t& ctas) {
-  const uint64_t want = 740u / units;
+  const uint64_t want = 5u * kSms / units;
   ctas = (uint32_t)(want < 1u ? 1u : (want > 8u ? 8u : want));
   if (ctas > pages) ctas = pages;
-  const uint64_t most = 592u / (units * ctas), by_pages = pages / (ctas * 4u);
+  const uint64_t most = 4u * kSms / (units * ctas), by_pages = pages / (ctas * 4u);
   clusters = (uint32_t)(most < by_pages ? most : by_pages);
   if (clusters < 1u) clusters = 1u;
 }

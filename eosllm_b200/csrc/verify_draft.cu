@@ -8,8 +8,10 @@
 // the first rejection, at a, one token is drawn from max(p_a - q_a, 0), or,
 // where that leaves nothing, from p_a; after k acceptances it is drawn from
 // p_k.  The draw is the lowest v with C_v > u_K C_last for the running sum C
-// of the weights in f64 (weights that are not positive and finite count 0).
+// of the weights in f64 (weights that are not positive and finite count 0; where
+// u C_last lies within rounding of a running sum, a neighbour of it may be drawn).
 // Tokens so drawn are distributed as the target's own.
+#include "eos_common.cuh"
 #include "eos_kernels.h"
 
 namespace eos {
@@ -80,7 +82,9 @@ __device__ __forceinline__ uint32_t vd_map(const void* p, uint32_t rank) {
 // more (from L1 or L2).  Reading one or two rows once is what bounds it for
 // many sequences, the chain of three reads (draft, its probabilities, the
 // row) for few: so few sequences get eight CTAs each.  One sequence of 4 drafts
-// and 32000 tokens: 5.9 us; 64 of 7: 10.7 us, of which the 8.2 MB read take 1.3.
+// and 32000 tokens: 5.8 us; 64 of 7: 10.3 us, of which the 8.2 MB read take 1.3;
+// the rest are the two reads before it and the barriers between (64 sequences:
+// per instruction a warp waits ten slots at barriers and six on memory).
 template <bool VEC, uint32_t NC>
 __global__ void __launch_bounds__(kVdThreads) verify_draft_kernel(const VerifyParams a) {
   __shared__ uint32_t s_taken;
@@ -249,7 +253,7 @@ cudaError_t launch_verify_draft(const float* p, const float* q, uint64_t stride,
   const VerifyParams a{p, q, stride, drafts, n_draft, u, max_draft, n_vocab, tokens, n_token};
   // as many CTAs per sequence (1, 2, 4 or 8) as keep two per SM, each warp with a step to do
   uint32_t n_cta = 1;
-  while (n_cta < kVdMaxCluster && 2ull * n_cta * n_seq <= 296u && 2u * n_cta * kVdWarps * 128u <= n_vocab) n_cta *= 2u;
+  while (n_cta < kVdMaxCluster && 2ull * n_cta * n_seq <= 2u * kSms && 2u * n_cta * kVdWarps * 128u <= n_vocab) n_cta *= 2u;
   const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0 && stride % 4u == 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(n_seq * n_cta);

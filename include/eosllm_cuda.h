@@ -281,10 +281,15 @@ EOSLLM_CUDA_API int eosi_cuda_kv_q8_read_dev(const eosi_cuda_kv_q8_t *kv, float 
  * and at least n_head * head_dim); rows of out outside every sequence stay as
  * they were, and out does not overlap q.  n_head is a multiple of kv->n_kv_head.
  * f32 in, f32 out: q is held as 24-bit integers (scaled by its row's
- * maximum), a page's probabilities as integers of 23 bits or more (relative to
- * the page's largest), products and sums of both with the int8 cache are exact
- * integers, and the softmax statistics are f32.  Results do not depend on
- * timing.  A query row or a visible cache row
+ * maximum, at least 1e-30), the probabilities times the value rows' scales as
+ * integers of 23 bits (up to four rows a kv head: 31), products and sums of both with the
+ * int8 cache are exact integers, and the softmax statistics are f32.  The
+ * latter integers' unit is, page by page, 2^-23 (2^-31) of the largest value
+ * scale that the row sees there times its largest probability there: a visible
+ * value row far larger than the others costs them low bits, whatever its own
+ * probability (1e2 times larger: about 1e-4 of the output; few rows 3e-7).
+ * Tokens that a row does not see have no influence on it at all.  Results do
+ * not depend on timing.  A query row or a visible cache row
  * that holds a NaN or an infinity gives a row of NaN (a row that sees no token
  * is 0 all the same).
  * scratch: eosi_cuda_kv_q8_attn_scratch_bytes(kv, batch, n_head) bytes, 16-byte
@@ -314,8 +319,9 @@ EOSLLM_CUDA_API int eosi_cuda_kv_q8_attn_dev(const eosi_cuda_kv_q8_t *kv, const 
  * drawn with the last number of the row, u[i * (max_draft + 1) + max_draft]:
  * from max(p_a - q_a, 0) after a rejection at a (from p_a where that is 0
  * everywhere), else from p of row n_draft[i].  The draw is the lowest v whose
- * running sum of weights exceeds u times the whole sum; sums are f64, so the
- * rows need not sum to 1; weights that are not positive and finite count 0.
+ * running sum of weights exceeds u times the whole sum; sums are f64, added in
+ * a fixed order (within their rounding of a running sum, a neighbour of that
+ * token may be drawn), and the rows need not sum to 1; weights that are not positive and finite count 0.
  * tokens[i * (max_draft + 1) ...] gets the accepted tokens and the drawn one,
  * n_tokens[i] of them, and 0xffffffff behind them (a row without any weight
  * draws no token).  max_draft = 0 draws one token from p alone (q and drafts
@@ -418,7 +424,8 @@ EOSLLM_CUDA_API int eosi_cuda_text_set_prefill_resident(eosi_cuda_text_t *t, int
  * prefill and generation run as before, with every token attending to its
  * context as stored.  Only at position 0, without open branches
  * (EOS_E_INVALID_ARG otherwise); Q8 needs world == 1, the PER_OP step and
- * n_head a multiple of n_kv_head (EOS_E_UNSUPPORTED). */
+ * n_head a multiple of n_kv_head (EOS_E_UNSUPPORTED).  A call that fails leaves
+ * the decoder as it was. */
 #define EOSI_CUDA_CACHE_F32 0
 #define EOSI_CUDA_CACHE_Q8 1
 EOSLLM_CUDA_API int eosi_cuda_text_set_cache(eosi_cuda_text_t *t, int mode);
