@@ -1699,6 +1699,7 @@ int TextDecoder::fork(uint32_t n, uint32_t max_new, uint32_t max_draft) {
   if (e == cudaSuccess && wout_pf == nullptr) {
     e = alloc(&wout_pf, prefill_operand_bytes(V, E));
     if (e == cudaSuccess) e = launch_prefill_w_prep(wout, V, E, wout_pf, st);
+    if (e != cudaSuccess) release(wout_pf);  // not prepared: the next fork starts over
   }
   // the last, partly filled page of the main cache into every sequence
   for (uint32_t L = 0; L < m.n_layer && br.rem > 0 && e == cudaSuccess; ++L)
