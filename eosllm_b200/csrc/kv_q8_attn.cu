@@ -405,6 +405,15 @@ __device__ __forceinline__ void attn_query_digits(float4 v, const AttnQScale& s,
     b[e] = (uint32_t)((s.finite ? __float2int_rn(f[e] * s.inv) : 0) + 0x808080) ^ 0x808080u;
   attn_digits(b, d);
 }
+// Weights (probability times value scale) as integers: the largest value scale
+// at hand becomes kAttnWeight -- 2^23 less what the roundings of the quotient may
+// add --, whatever its mantissa: with powers of two only, the integers of a page
+// were half as long at worst, and outputs 1.2e-6 off where 32-bit arithmetic was
+// 0.5e-6.  The quotient is within 2 units in its last place, for all of a page.
+constexpr float kAttnWeight = 8388604.0f;
+__device__ __forceinline__ float attn_weight_top(float v) { return fmaxf(v, 4.930381e-32f); }  // 2^-104: a finite quotient
+__device__ __forceinline__ float attn_weight_scale(float top) { return __fdividef(kAttnWeight, top); }
+__device__ __forceinline__ float attn_weight_unit(float top) { return top * (4194304.0f / kAttnWeight); }  // sums in 2^22
 __device__ __forceinline__ float attn_warp_max(float x) {
 #pragma unroll
   for (uint32_t b = 16; b > 0; b >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
@@ -1333,21 +1342,21 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
         if (t > half) live = fold_tile();
         if (live) live = __all_sync(0xffffffffu, attn_wait(&bar.xmax[half][grp], it & 1u)) != 0;
         if (!live) break;
-        // unit of the probabilities: a power of two from the largest value scale that a column sees in the tile (`top`:
-        // its exponent), one for all columns unless the tile is cut
-        uint32_t top[NC][2];
-        float vw[4];
+        // unit of the probabilities: from the largest value scale that a column sees in the tile (`top`), one for all
+        // columns unless the tile is cut
+        float top[NC][2], inv = 0.0f, vw[4];
         {
           const uint4 t4 = *reinterpret_cast<const uint4*>(xt);
-          const uint32_t all = max(max(max(t4.x, t4.y), max(t4.z, t4.w)) >> 23, 23u);
-          const float v1 = CAUSAL ? __uint_as_float(vown)
-                                  : __uint_as_float(vbits) * __uint_as_float((276u - all) << 23);  // times 2^(22 - exponent)
+          const float all = attn_weight_top(__uint_as_float(max(max(t4.x, t4.y), max(t4.z, t4.w))));
+          if constexpr (!CAUSAL) inv = attn_weight_scale(all);
+          const float v1 = CAUSAL ? __uint_as_float(vown) : __uint_as_float(vbits) * inv;
 #pragma unroll
           for (uint32_t j = 0; j < 4u; ++j) vw[j] = __shfl_sync(0xffffffffu, v1, g + 8u * j);
 #pragma unroll
           for (uint32_t y = 0; y < NC; ++y)
 #pragma unroll
-            for (uint32_t z = 0; z < 2u; ++z) top[y][z] = CAUSAL ? max(tail[y][z] >> 23, all) : all;
+            for (uint32_t z = 0; z < 2u; ++z)
+              top[y][z] = CAUSAL ? fmaxf(__uint_as_float(tail[y][z]), all) : all;
         }
         uint8_t* pop = stages + st * G::kBlock;  // the probabilities take the place of the keys
 #pragma unroll
@@ -1370,9 +1379,8 @@ __global__ void __launch_bounds__((AttnGeo<HD, RT>::kThreads), (AttnGeo<HD, RT>:
           const float2 nm = make_float2(fmaxf(ref.x, m[y].x), fmaxf(ref.y, m[y].y));
           f[y] = make_float2(attn_ex2(m[y].x - nm.x), attn_ex2(m[y].y - nm.y));
           const float2 share = make_float2(attn_ex2(ref.x - nm.x), attn_ex2(ref.y - nm.y));
-          // 2^exponent: value sums are held in units of 256
-          const float2 un = make_float2(__uint_as_float(top[y][0] << 23), __uint_as_float(top[y][1] << 23));
-          const float2 up = make_float2(__uint_as_float((276u - top[y][0]) << 23), __uint_as_float((276u - top[y][1]) << 23));
+          const float2 un = make_float2(attn_weight_unit(top[y][0]), attn_weight_unit(top[y][1]));
+          const float2 up = make_float2(attn_weight_scale(top[y][0]), attn_weight_scale(top[y][1]));
           fold[y] = attn_mul2(share, un);
           m[y] = nm;
           uint32_t b0[4], b1[4], d[3];

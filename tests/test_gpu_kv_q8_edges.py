@@ -131,3 +131,75 @@ def test_factors_at_the_ends_of_the_range(gpu, count, q_gain, k_gain, scale):
             x *= np.float32(k_gain)
         b.scale = scale
     Batch(gpu, 4, 2, 64, 150, [40], [count], seed=count, edit=edit).check()
+
+
+def value_whose_scale_is_just_below_a_power_of_two():
+    for up in range(-40, 40):
+        a = np.float32(127.0 * (2.0 - 2.0 ** -23)) * np.float32(1 + up * 2.0 ** -24)
+        if (np.float32(a * (np.float32(1.0) / np.float32(127.0))).view(np.uint32) & 0x7FFFFF) == 0x7FFFFF:
+            return a
+    raise AssertionError
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("prefix,length,count", [(0, 1, 1), (1, 1, 3), (1, 4, 20), (200, 30, 3), (200, 30, 20), (300, 130, 40)])
+def test_a_value_scale_just_below_a_power_of_two(gpu, hd, prefix, length, count):
+    """A weight is rounded as probability 1 times the largest value scale of its
+    page, whose mantissa is all ones; queries of 0 give every token that
+    probability exactly, the others give it to one."""
+    big = value_whose_scale_is_just_below_a_power_of_two()
+
+    def edit(b):
+        b.q[::2] = 0
+        for x in [b.vp] + b.vs:
+            x[:] = np.clip(x, -100, 100)
+            x[::3, :, hd // 2] = big
+    Batch(gpu, 4, 2, hd, prefix, [length], [count], seed=count + hd, spread=0.0, edit=edit).check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("top", [1.01, 1.4, 1.98])
+def test_weights_use_their_integers_whole(gpu, hd, top):
+    """The rounding of probabilities times value scales, on rows where little else
+    is rounded (queries of 1 and -1 are integers of any unit): one page, and the
+    largest value scale anywhere between two powers of two.
+
+    Bound.  A weight is off by up to half of u = vs_max / 8388604, evenly spread:
+    u^2 / 12 in the mean square, times the square of the value integer, summed over
+    the tokens.  A probability is off by ex2's 2^-22.5 at most, 2^-23.5 in the root
+    mean square, and by the f32 roundings of its score z (in log2 units): the sum,
+    the difference and the product, each 2^-24 |z| / sqrt(3) or less.  The rest (the
+    sum of probabilities, folding, the quotient) is four times 2^-24 of the output or
+    less.  Every part but the first is an upper bound, so the root mean square over
+    24 x 2 x hd outputs (6144 weights, 1 % of it) is below their sum's; a unit of a
+    power of two doubles the first part at worst."""
+    rng = np.random.default_rng(hd)
+    tokens = 128
+
+    def edit(b):
+        b.q[:] = np.where(rng.random(b.q.shape) < 0.5, -1.0, 1.0)
+        b.scale = 1.5 * 0.125 * (64 / hd) ** 0.5
+        s = rng.uniform(0.3, 1.0, (tokens, 2, 1))
+        s[5] = top
+        b.vp[:] = b.vp / np.abs(b.vp).max(-1, keepdims=True) * 127 * s
+    b = Batch(gpu, 2, 2, hd, tokens, [0], [24], seed=hd, spread=0.0, edit=edit)
+    b.run()
+    got = b.out.cpu().numpy()[:24].astype(np.float64)
+    k, (v, vs) = stored(b.kp)[0].astype(np.float64), stored(b.vp)
+    v, vs = v.astype(np.float64), vs.astype(np.float64)
+    err, pred = [], []
+    for r in range(24):
+        for h in range(2):
+            z = (k[:, h] @ b.q[r, h].astype(np.float64)) * b.scale
+            z -= z.max()
+            p = np.exp(z)
+            out = p @ v[:, h] / p.sum()
+            z2 = np.log2(np.e) * (np.abs(z) + np.abs(z).max())
+            rho2 = 2.0 ** -47 + 3 * (np.log(2) * 2.0 ** -24 * z2) ** 2 / 3
+            ints = v[:, h] / vs[:, h, None]
+            var = (vs[:, h].max() / 8388604) ** 2 / 12 * (ints ** 2).sum(0) + ((p[:, None] * v[:, h]) ** 2 * rho2[:, None]).sum(0)
+            err.append(got[r, h] - out)
+            pred.append(var / p.sum() ** 2 + (4 * 2.0 ** -24 * out) ** 2)
+    err, pred = np.sqrt(np.mean(np.square(err))), np.sqrt(np.mean(pred))
+    assert err <= pred, (err, pred, err / pred)
+    assert gpu.take_device_errors() == 0
